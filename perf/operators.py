@@ -268,7 +268,7 @@ def _own_sparse(st, case):
 def _own_compact(st, case):
     from daric_b200.evict import compact
     compact(st["copier"], st["names"], st["keep"], st["flat_table"], seg_blk_off=st["table_off"],
-            mode="flexible" if case["rotate"] else "none")
+            per_head=case["per_head"], mode="flexible" if case["rotate"] else "none")
     return st["cache"]
 
 
