@@ -71,6 +71,30 @@ SIGNATURES: dict[str, tuple] = {
     "daric_score_select_noalloc": (
         C.c_int, [_vp, C.c_int64, C.c_int64, C.c_int64, _i64p, _i64p, _i64p, _i64p, C.c_int, C.c_float,
                   _vp, C.c_int64, _i64p, C.c_int64, _vp, _vp, _vp, C.c_int64, _i64p, C.c_int, _vp]),
+    "daric_attend_workspace": (C.c_int, [C.c_int, C.c_int64, C.POINTER(C.c_int64)]),
+    "daric_copier_tree_attention": (
+        C.c_int, [_vp, C.c_char_p, C.c_int, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                  _vp, C.c_int64, C.c_int64, C.c_int64, _vp, _vp, _vp, C.c_int64, C.c_float,
+                  _vp, C.c_int64, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, C.c_int, _vp]),
+    "daric_copier_sparse_attention": (
+        C.c_int, [_vp, C.c_char_p, C.c_int, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                  _vp, C.c_int64, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, C.c_int64, _vp, _vp, C.c_float,
+                  _vp, C.c_int64, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, C.c_int, _vp]),
+    "daric_copier_page_bounds": (
+        C.c_int, [_vp, C.c_char_p, C.c_int, _vp, C.c_int64, C.c_int64, C.c_int64, _vp, _vp, _vp, C.c_int, _vp]),
+    "daric_select_pages_workspace": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_int64)]),
+    "daric_select_pages": (
+        C.c_int, [_vp, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64,
+                  _vp, C.c_int64, C.c_int64, C.c_int64, _vp, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _vp,
+                  _vp, C.c_int64, C.c_int, _vp]),
+    "daric_scores_workspace": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_int64)]),
+    "daric_copier_attention_scores": (
+        C.c_int, [_vp, C.c_char_p, C.c_int, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                  _vp, C.c_int64, C.c_int64, C.c_int64, _vp, _vp, _vp, C.c_int64, _vp, C.c_int64, C.c_float,
+                  _vp, C.c_int64, C.c_int64, _vp, C.c_int, _vp, C.c_int64, C.c_int, _vp]),
+    "daric_copier_compact": (
+        C.c_int, [_vp, C.c_int64, C.POINTER(C.c_char_p), C.c_int, C.c_int, C.c_int64, C.c_int, _vp, C.c_int64,
+                  _vp, C.c_int64, C.c_int64, _i64p, _i64p, _i64p, _i64p, _vp, C.c_int64, C.c_int, _vp]),
     "daric_ptrs_to_slots": (
         C.c_int, [C.c_int64, _i64p, _i64p, _i64p, _vp, C.c_int64, C.c_int64, _vp, _vp, C.c_int, _vp]),
 }

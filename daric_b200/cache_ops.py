@@ -108,6 +108,7 @@ class CacheCopier:
         self._h = h
         self._layers: dict[str, torch.Tensor] = {}
         self._tables: dict[str, torch.Tensor] = {}
+        self._page_first: dict[str, bool] = {}
         self._store: Optional[torch.Tensor] = None
 
     def __del__(self):
@@ -126,6 +127,7 @@ class CacheCopier:
             self._h, name.encode(), C.c_void_p(tensor.data_ptr()), tensor.device.index, tensor.dim(), sp, tp,
             tensor.element_size(), int(bool(is_page_first))))
         self._layers[name] = tensor
+        self._page_first[name] = bool(is_page_first)
         self._tables.pop(name, None)
 
     def register_store(self, buffer: torch.Tensor) -> None:

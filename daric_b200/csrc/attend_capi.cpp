@@ -1,0 +1,455 @@
+// C entries of the operators over the paged KV cache: attention, block
+// selection and eviction. Arguments are checked here; nothing waits for the
+// GPU, allocates device memory or uploads a descriptor, so every call can be
+// captured into a graph (after the first call on a device).
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <string>
+#include <vector>
+
+#include "attend.h"
+
+using namespace daric;
+
+namespace {
+
+template <class F>
+int guard(F&& f) {
+  try {
+    f();
+    clear_error();
+    return DARIC_OK;
+  } catch (const Error& e) {
+    record_error(e.code, e.what());
+    return e.code;
+  } catch (const std::exception& e) {
+    record_error(DARIC_ERR_STATE, e.what());
+    return DARIC_ERR_STATE;
+  } catch (...) {
+    record_error(DARIC_ERR_STATE, "unknown error");
+    return DARIC_ERR_STATE;
+  }
+}
+
+struct OnDevice {
+  int prev = -1;
+  explicit OnDevice(int dev) {
+    DARIC_CUDA(cudaGetDevice(&prev));
+    if (prev == dev) prev = -1;
+    else DARIC_CUDA(cudaSetDevice(dev));
+  }
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+bool aligned(const void* p, int64_t a, int64_t b, int64_t n) {
+  return (uintptr_t)p % n == 0 && a % n == 0 && b % n == 0;
+}
+
+// The arguments that every call over a batch of query rows shares.
+SeqBatch seq_batch(const int32_t* table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                   const int32_t* seq_lens, const int32_t* cu_q, int64_t num_rows, int64_t q_heads, int64_t kv_heads,
+                   int64_t page_size) {
+  SeqBatch b{};
+  DARIC_CHECK(num_seqs >= 1 && num_rows >= 0 && table_cols >= 1, "batch sizes must be positive");
+  DARIC_CHECK(num_seqs <= 65535, "at most 65535 sequences per call");
+  DARIC_CHECK(table_cols * page_size <= INT32_MAX, "block table reaches past int32 positions");
+  DARIC_CHECK(table && seq_lens, "NULL block table or lengths");
+  DARIC_CHECK(table_ld >= table_cols || num_seqs == 1, "block table rows overlap");
+  DARIC_CHECK(q_heads >= kv_heads && q_heads % kv_heads == 0,
+              "query heads (" + std::to_string(q_heads) + ") must be a multiple of KV heads (" +
+                  std::to_string(kv_heads) + ")");
+  DARIC_CHECK(num_rows * q_heads <= INT32_MAX, "too many query rows");
+  DARIC_CHECK(cu_q || num_rows % num_seqs == 0, "query rows must divide evenly over the sequences without cu_q");
+  b.table = table;
+  b.table_ld = table_ld;
+  b.table_cols = (int32_t)table_cols;
+  b.seq_lens = seq_lens;
+  b.cu_q = cu_q;
+  b.num_seqs = (int32_t)num_seqs;
+  b.num_rows = (int32_t)num_rows;
+  b.rows_each = (int32_t)(num_rows / num_seqs);
+  b.group = (int32_t)(q_heads / kv_heads);
+  return b;
+}
+
+int check_layer(const LayerRef& L, int kv_dtype, int64_t head_dim, int device, const char* what) {
+  DARIC_CHECK(L.device == device, std::string(what) + ": the tensors must be on the KV cache's device");
+  DARIC_CHECK(kv_dtype == DARIC_DTYPE_BF16 || kv_dtype == DARIC_DTYPE_F16,
+              std::string(what) + ": the KV cache must be bfloat16 or float16");
+  DARIC_CHECK(L.elem_size == 2, std::string(what) + ": kv_dtype does not match the registered element size");
+  DARIC_CHECK(L.kv.head_dim == head_dim, std::string(what) + ": query head dimension " + std::to_string(head_dim) +
+                                             " differs from the KV cache's " + std::to_string(L.kv.head_dim));
+  return kv_dtype;
+}
+
+void check_scale(float scale) {
+  DARIC_CHECK(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
+}
+
+constexpr int kAttendCtasPerSm = 1;
+
+// Row-tile variant: the query heads of one KV head times the rows of a
+// sequence (their mean: the lengths are on the device) in 16s.
+int attend_variant(const SeqBatch& b, bool sparse) {
+  const int64_t rows = sparse ? b.group : (int64_t)((b.num_rows + b.num_seqs - 1) / b.num_seqs) * b.group;
+  if (rows <= 16) return 1;
+  if (rows <= 32 || sparse) return 2;
+  return 4;
+}
+
+size_t attend_bytes(int grid, int rows, int head_dim) {
+  return (size_t)grid * (2 * (size_t)rows * head_dim * 4 + 2 * (size_t)rows * 8 + 16);
+}
+
+// Lays the attention's workspace out: descriptors, maxima and sums, outputs.
+void attend_workspace(AttendLaunch& p, int grid, int rows, void* ws, int64_t ws_bytes) {
+  DARIC_CHECK(ws && (uintptr_t)ws % 16 == 0, "workspace must be a 16-byte aligned device buffer");
+  DARIC_CHECK((int64_t)attend_bytes(grid, rows, p.kv.head_dim) <= ws_bytes, "workspace is too small");
+  uint8_t* w = (uint8_t*)ws;
+  p.desc = reinterpret_cast<int4*>(w);
+  p.part_ml = reinterpret_cast<float2*>(w + (size_t)grid * 16);
+  p.part = reinterpret_cast<float*>(w + (size_t)grid * 16 + (size_t)grid * 2 * rows * 8);
+}
+
+}  // namespace
+
+extern "C" {
+
+int daric_attend_workspace(int device, int64_t head_dim, int64_t* out_bytes) {
+  return guard([&] {
+    DARIC_CHECK(out_bytes, "out_bytes is NULL");
+    DARIC_CHECK(head_dim > 0 && head_dim <= 256, "head dimension must be at most 256");
+    *out_bytes = (int64_t)attend_bytes(device_info(device).sm_count * kAttendCtasPerSm, attend_rows(4), (int)head_dim);
+  });
+}
+
+int daric_copier_tree_attention(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
+                                int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
+                                const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                                const int32_t* seq_lens, const int32_t* cu_q, const int64_t* tree_mask,
+                                int64_t mask_words, float scale, void* out, int64_t out_row, int64_t out_head,
+                                float* lse, int64_t lse_row, void* workspace, int64_t workspace_bytes, int device,
+                                void* stream) {
+  return guard([&] {
+    const LayerRef L = layer_ref(copier, layer_name);
+    check_layer(L, kv_dtype, head_dim, device, "tree_attention");
+    check_scale(scale);
+    AttendLaunch p{};
+    p.kv = L.kv;
+    p.sq = seq_batch(block_table, table_ld, num_seqs, table_cols, seq_lens, cu_q, num_rows, q_heads, L.kv.heads,
+                     L.kv.page_size);
+    if (num_rows == 0) return;
+    DARIC_CHECK(q && out, "NULL query or output");
+    DARIC_CHECK(!tree_mask || mask_words >= 1, "tree mask needs at least one word per row");
+    DARIC_CHECK(aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
+    DARIC_CHECK(aligned(out, out_row * 2, out_head * 2, 16), "output rows must be 16-byte aligned");
+    const DeviceInfo di = device_info(device);
+    p.sq.mask = reinterpret_cast<const uint64_t*>(tree_mask);
+    p.sq.mask_words = (int32_t)mask_words;
+    p.sq.err = di.err;
+    p.q = (const uint8_t*)q;
+    p.q_row = q_row * 2;
+    p.q_head = q_head * 2;
+    p.out = (uint8_t*)out;
+    p.out_row = out_row * 2;
+    p.out_head = out_head * 2;
+    p.lse = lse;
+    p.lse_row = lse_row;
+    p.scale = scale;
+    // tiles of the whole batch are counted in 32 bits
+    const int rg = attend_variant(p.sq, false), rows = attend_rows(rg);
+    const double tiles = (double)L.kv.heads * ((double)num_rows * p.sq.group / rows + (double)num_seqs) *
+                         ((double)table_cols * L.kv.page_size / 16.0 + 1.0);
+    DARIC_CHECK(tiles < 4.0e9, "tree_attention: the batch has too many tiles for one call");
+    DARIC_CHECK((int64_t)num_rows * p.sq.group / rows < (1 << 18), "tree_attention: too many query rows");
+    const int grid = di.sm_count * kAttendCtasPerSm;
+    attend_workspace(p, grid, rows, workspace, workspace_bytes);
+    OnDevice on(device);
+    launch_attend(p, kv_dtype, rg, grid, (cudaStream_t)stream);
+  });
+}
+
+int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
+                                  int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
+                                  const int32_t* pages, int64_t pages_row, int64_t pages_head, int64_t k,
+                                  const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                                  const int32_t* seq_lens, const int32_t* cu_q, float scale, void* out,
+                                  int64_t out_row, int64_t out_head, float* lse, int64_t lse_row, void* workspace,
+                                  int64_t workspace_bytes, int device, void* stream) {
+  return guard([&] {
+    const LayerRef L = layer_ref(copier, layer_name);
+    check_layer(L, kv_dtype, head_dim, device, "sparse_attention");
+    check_scale(scale);
+    AttendLaunch p{};
+    p.kv = L.kv;
+    p.sq = seq_batch(block_table, table_ld, num_seqs, table_cols, seq_lens, cu_q, num_rows, q_heads, L.kv.heads,
+                     L.kv.page_size);
+    if (num_rows == 0) return;
+    DARIC_CHECK(q && out && pages, "NULL query, output or page list");
+    DARIC_CHECK(k >= 1 && k * L.kv.page_size <= INT32_MAX, "sparse_attention: page lists must have at least one entry");
+    DARIC_CHECK(aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
+    DARIC_CHECK(aligned(out, out_row * 2, out_head * 2, 16), "output rows must be 16-byte aligned");
+    const DeviceInfo di = device_info(device);
+    p.sq.err = di.err;
+    p.q = (const uint8_t*)q;
+    p.q_row = q_row * 2;
+    p.q_head = q_head * 2;
+    p.out = (uint8_t*)out;
+    p.out_row = out_row * 2;
+    p.out_head = out_head * 2;
+    p.lse = lse;
+    p.lse_row = lse_row;
+    p.pages = pages;
+    p.pages_row = pages_row;
+    p.pages_head = pages_head;
+    p.k = (int32_t)k;
+    p.scale = scale;
+    const int rg = attend_variant(p.sq, true), rows = attend_rows(rg);
+    const double tiles = (double)L.kv.heads * (double)num_rows * ((double)p.sq.group / rows + 1.0) *
+                         ((double)k * L.kv.page_size / 16.0 + 1.0);
+    DARIC_CHECK(tiles < 4.0e9, "sparse_attention: the batch has too many tiles for one call");
+    const int grid = di.sm_count * kAttendCtasPerSm;
+    attend_workspace(p, grid, rows, workspace, workspace_bytes);
+    OnDevice on(device);
+    launch_attend(p, kv_dtype, rg, grid, (cudaStream_t)stream);
+  });
+}
+
+int daric_copier_page_bounds(daric_copier* copier, const char* layer_name, int kv_dtype, const int32_t* block_table,
+                             int64_t table_ld, int64_t num_seqs, int64_t table_cols, const int32_t* seq_lens,
+                             const int32_t* start, void* bounds, int device, void* stream) {
+  return guard([&] {
+    const LayerRef L = layer_ref(copier, layer_name);
+    check_layer(L, kv_dtype, L.kv.head_dim, device, "page_bounds");
+    BoundsLaunch p{};
+    p.kv = L.kv;
+    p.sq = seq_batch(block_table, table_ld, num_seqs, table_cols, seq_lens, nullptr, 0, L.kv.heads, L.kv.heads,
+                     L.kv.page_size);
+    DARIC_CHECK(bounds && (uintptr_t)bounds % 16 == 0, "bounds must be a 16-byte aligned device buffer");
+    const DeviceInfo di = device_info(device);
+    p.sq.err = di.err;
+    p.start = start;
+    p.bounds = (uint8_t*)bounds;
+    OnDevice on(device);
+    launch_page_bounds(p, kv_dtype, di.sm_count, (cudaStream_t)stream);
+  });
+}
+
+int daric_select_pages_workspace(int64_t num_rows, int64_t kv_heads, int64_t table_cols, int64_t* out_bytes) {
+  return guard([&] {
+    DARIC_CHECK(out_bytes, "out_bytes is NULL");
+    DARIC_CHECK(num_rows >= 0 && kv_heads >= 1 && table_cols >= 1 && table_cols <= (1 << 20), "select_pages: sizes out of range");
+    const int64_t items = num_rows * kv_heads;
+    *out_bytes = items * 4 * (table_cols + (table_cols + kScoreChunk - 1) / kScoreChunk) + 16;
+  });
+}
+
+int daric_select_pages(const void* q, int kv_dtype, int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads,
+                       int64_t head_dim, const void* bounds, int64_t num_pages, int64_t kv_heads,
+                       const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                       const int32_t* seq_lens, const int32_t* cu_q, int64_t block_size, int64_t k, int64_t first,
+                       int64_t last, int32_t* out, void* workspace, int64_t workspace_bytes, int device,
+                       void* stream) {
+  return guard([&] {
+    DARIC_CHECK(kv_dtype == DARIC_DTYPE_BF16 || kv_dtype == DARIC_DTYPE_F16,
+                "select_pages: the bounds must be bfloat16 or float16");
+    DARIC_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256,
+                "select_pages: head dimension must be 64, 128 or 256, got " + std::to_string(head_dim));
+    DARIC_CHECK(kv_heads >= 1 && kv_heads < 4096 && num_pages >= 1 && num_pages <= INT32_MAX, "bounds sizes out of range");
+    DARIC_CHECK(block_size >= 1 && block_size <= 1024, "block size must be in [1, 1024]");
+    DARIC_CHECK(first >= 0 && last >= 1 && k >= 1 && first + last <= k && k <= INT32_MAX,
+                "select_pages: k must hold the first and last pages that are always taken (last >= 1)");
+    DARIC_CHECK(table_cols <= (1 << 20), "select_pages: at most 1048576 pages per sequence");
+    SelectPagesLaunch p{};
+    p.sq = seq_batch(block_table, table_ld, num_seqs, table_cols, seq_lens, cu_q, num_rows, q_heads, kv_heads,
+                     block_size);
+    if (num_rows == 0) return;
+    DARIC_CHECK(q && bounds && out, "NULL query, bounds or output");
+    DARIC_CHECK(aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
+    DARIC_CHECK((uintptr_t)bounds % 16 == 0, "bounds must be 16-byte aligned");
+    DARIC_CHECK(workspace && (uintptr_t)workspace % 4 == 0, "workspace must be a device buffer");
+    const int64_t items = num_rows * kv_heads;
+    const int64_t chunks = (table_cols + kScoreChunk - 1) / kScoreChunk;
+    DARIC_CHECK(items * 4 * (table_cols + chunks) <= workspace_bytes, "workspace is too small");
+    const DeviceInfo di = device_info(device);
+    p.sq.err = di.err;
+    p.q = (const uint8_t*)q;
+    p.q_row = q_row * 2;
+    p.q_head = q_head * 2;
+    p.bounds = (const uint8_t*)bounds;
+    p.num_pages = (int32_t)num_pages;
+    p.heads = (int32_t)kv_heads;
+    p.head_dim = (int32_t)head_dim;
+    p.page_size = (int32_t)block_size;
+    p.k = (int32_t)k;
+    p.first = (int32_t)first;
+    p.last = (int32_t)last;
+    p.keys = (uint32_t*)workspace;
+    p.mags = (float*)workspace + items * table_cols;
+    p.out = out;
+    OnDevice on(device);
+    launch_select_pages(p, kv_dtype, (cudaStream_t)stream);
+  });
+}
+
+int daric_scores_workspace(int64_t num_rows, int64_t q_heads, int64_t table_cols, int64_t block_size,
+                           int64_t* out_bytes) {
+  return guard([&] {
+    DARIC_CHECK(out_bytes, "out_bytes is NULL");
+    DARIC_CHECK(num_rows >= 0 && q_heads >= 1 && table_cols >= 1 && block_size >= 1, "sizes out of range");
+    const int64_t splits = std::min<int64_t>((table_cols * block_size + kScoreKeys - 1) / kScoreKeys, 64);
+    *out_bytes = num_rows * q_heads * (splits * 8 + 4) + 16;
+  });
+}
+
+int daric_copier_attention_scores(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
+                                  int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
+                                  const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                                  const int32_t* seq_lens, const int32_t* cu_q, const int64_t* tree_mask,
+                                  int64_t mask_words, const float* lse, int64_t lse_row, float scale, float* scores,
+                                  int64_t scores_row, int64_t scores_cols, const int64_t* col_off, int accumulate,
+                                  void* workspace, int64_t workspace_bytes, int device, void* stream) {
+  return guard([&] {
+    const LayerRef L = layer_ref(copier, layer_name);
+    check_layer(L, kv_dtype, head_dim, device, "attention_scores");
+    check_scale(scale);
+    ScoresLaunch p{};
+    p.kv = L.kv;
+    p.sq = seq_batch(block_table, table_ld, num_seqs, table_cols, seq_lens, cu_q, num_rows, q_heads, L.kv.heads,
+                     L.kv.page_size);
+    DARIC_CHECK(scores && col_off && (q || num_rows == 0), "NULL query, scores or column offsets");
+    DARIC_CHECK(!tree_mask || mask_words >= 1, "tree mask needs at least one word per row");
+    DARIC_CHECK(num_rows == 0 || aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
+    DARIC_CHECK(scores_cols >= 0 && (scores_row >= scores_cols || L.kv.heads == 1), "score rows overlap");
+    const int64_t tiles = (table_cols * L.kv.page_size + kScoreKeys - 1) / kScoreKeys;
+    DARIC_CHECK(tiles <= 65535, "attention_scores: sequences of at most 33.5M positions");
+    const DeviceInfo di = device_info(device);
+    p.sq.err = di.err;
+    p.sq.mask = reinterpret_cast<const uint64_t*>(tree_mask);
+    p.sq.mask_words = (int32_t)mask_words;
+    p.q = (const uint8_t*)q;
+    p.q_row = q_row * 2;
+    p.q_head = q_head * 2;
+    p.lse = lse;
+    p.lse_row = lse_row;
+    p.scores = scores;
+    p.scores_row = scores_row;
+    p.scores_cols = scores_cols;
+    p.col_off = col_off;
+    p.accumulate = accumulate ? 1 : 0;
+    p.scale = scale;
+    p.splits = (int32_t)std::min<int64_t>(tiles, 64);
+    if (num_rows == 0) p.lse = scores;  // no rows: never read, and nothing to join
+    if (!p.lse) {
+      DARIC_CHECK(workspace && (uintptr_t)workspace % 8 == 0, "workspace must be an 8-byte aligned device buffer");
+      DARIC_CHECK(num_rows * q_heads * ((int64_t)p.splits * 8 + 4) <= workspace_bytes, "workspace is too small");
+      p.part = (float2*)workspace;
+      p.lse_work = (float*)workspace + num_rows * q_heads * p.splits * 2;
+    }
+    OnDevice on(device);
+    launch_scores(p, kv_dtype, (cudaStream_t)stream);
+  });
+}
+
+int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* const* layer_names, int kv_dtype,
+                         int mode, int64_t lists, int per_head, const int32_t* idx, int64_t idx_row,
+                         const int32_t* count,
+                         int64_t count_row, int64_t num_segs, const int64_t* out_off, const int64_t* seg_cap,
+                         const int64_t* seg_blk_off, const int64_t* dst_start, const int32_t* block_table,
+                         int64_t block_table_numel, int device, void* stream) {
+  return guard([&] {
+    DARIC_CHECK(copier, "copier is NULL");
+    DARIC_CHECK(mode == DARIC_ROPE_NONE || mode == DARIC_ROPE_FLEXIBLE, "compact: mode must be NONE or FLEXIBLE");
+    if (num_layers <= 0 || num_segs <= 0) return;
+    DARIC_CHECK(layer_names && idx && count && out_off && seg_cap && seg_blk_off, "NULL argument");
+    DARIC_CHECK(block_table != nullptr, "block_table is NULL");
+    std::vector<LayerRef> all;
+    for (int64_t l = 0; l < num_layers; ++l) all.push_back(layer_ref(copier, layer_names[l]));
+    const LayerRef& A = all[0];
+    const bool rotate = mode == DARIC_ROPE_FLEXIBLE;
+    int es = 0;
+    switch (kv_dtype) {
+      case DARIC_DTYPE_F32: es = 4; break;
+      case DARIC_DTYPE_F16:
+      case DARIC_DTYPE_BF16: es = 2; break;
+      case DARIC_DTYPE_FP8_E4M3: es = 1; break;
+      default: throw Error(DARIC_ERR_INVALID, "compact: unknown KV dtype");
+    }
+    for (int64_t l = 0; l < num_layers; ++l) {
+      const LayerRef& L = all[l];
+      DARIC_CHECK(L.device == device, "compact: the tensors must be on the KV cache's device");
+      DARIC_CHECK(L.elem_size == es, "compact: kv_dtype does not match the registered element size");
+      DARIC_CHECK(L.kv.page_size == A.kv.page_size && L.kv.heads == A.kv.heads && L.kv.head_dim == A.kv.head_dim &&
+                      L.kv.num_pages == A.kv.num_pages,
+                  "compact: layers of one call must share block size, blocks, heads and head dimension");
+      if (rotate) {
+        DARIC_CHECK(L.table, std::string("layer has no rotary table (register_rotary): ") + layer_names[l]);
+        DARIC_CHECK(L.tab_dtype == A.tab_dtype && L.neox == A.neox && L.half_rot == A.half_rot &&
+                        L.max_pos == A.max_pos && L.kv_dtype == kv_dtype,
+                    "compact: layers of one call must share the rotary style and table shape");
+      }
+      for (int64_t m = 0; m < l; ++m)
+        DARIC_CHECK(all[m].kv.base != L.kv.base, "compact: a layer is named twice");
+    }
+    const int64_t H = A.kv.heads, per_layer = per_head ? H : 1;
+    DARIC_CHECK(lists == per_layer || lists == num_layers * per_layer,
+                "compact: the selection must have one row per layer, or one for all layers (times the KV heads with "
+                "per_head); got " + std::to_string(lists) + " rows for " + std::to_string(num_layers) + " layers and " +
+                    std::to_string(H) + " heads");
+    const bool shared = lists == per_layer;
+    CompactLaunch p{};
+    p.idx = idx;
+    p.idx_row = idx_row;
+    p.count = count;
+    p.count_row = count_row;
+    p.block_table = block_table;
+    p.table_numel = block_table_numel;
+    const DeviceInfo di = device_info(device);
+    p.err = di.err;
+    p.num_pages = A.kv.num_pages;
+    p.page_size = A.kv.page_size;
+    p.heads = A.kv.heads;
+    p.head_dim = A.kv.head_dim;
+    p.page_div = A.kv.page_div;
+    p.per_head = per_head ? 1 : 0;
+    p.shared = shared;
+    p.rotate = rotate;
+    p.neox = A.neox;
+    p.half_rot = A.half_rot;
+    p.table_row = A.table_row;
+    p.max_pos = A.max_pos;
+    for (int64_t s = 0; s < num_segs; ++s) {
+      DARIC_CHECK(out_off[s] >= 0 && seg_cap[s] >= 0 && seg_blk_off[s] >= 0 && (!dst_start || dst_start[s] >= 0),
+                  "negative segment field at segment " + std::to_string(s));
+      DARIC_CHECK(out_off[s] + seg_cap[s] <= idx_row || lists == 1, "segment " + std::to_string(s) + " exceeds the selection's row");
+      DARIC_CHECK(seg_cap[s] + (dst_start ? dst_start[s] : 0) <= INT32_MAX, "positions exceed int32");
+    }
+    OnDevice on(device);
+    for (int64_t l0 = 0; l0 < num_layers; l0 += kCompactLayers) {
+      p.layer0 = (int32_t)l0;
+      p.num_layers = (int32_t)std::min<int64_t>(kCompactLayers, num_layers - l0);
+      for (int l = 0; l < p.num_layers; ++l) {
+        const LayerRef& L = all[l0 + l];
+        p.layers[l] = CompactLayer{L.kv.base, L.table, L.kv.page_stride, L.kv.tok_stride, L.kv.head_stride, L.kv.v_off};
+      }
+      for (int64_t s0 = 0; s0 < num_segs; s0 += kCompactSegs) {
+        p.num_segs = (int32_t)std::min<int64_t>(kCompactSegs, num_segs - s0);
+        for (int s = 0; s < p.num_segs; ++s)
+          p.segs[s] = CompactSeg{seg_blk_off[s0 + s], out_off[s0 + s], (int32_t)seg_cap[s0 + s],
+                                 (int32_t)(dst_start ? dst_start[s0 + s] : 0), (int32_t)(s0 + s)};
+        // few CTAs: their rows are split by columns (pieces of 64 bytes still
+        // move whole sectors)
+        const int64_t ctas = (int64_t)p.heads * 2 * p.num_segs * p.num_layers;
+        const int row = A.kv.head_dim * es;
+        p.slices = 1;
+        while (p.slices < 4 && row / (p.slices * 2) >= 64 && ctas * p.slices < 3 * (int64_t)di.sm_count) p.slices *= 2;
+        launch_compact(p, kv_dtype, A.tab_dtype, (cudaStream_t)stream);
+      }
+    }
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,563 @@
+// Block selection for sparse attention over the paged KV cache.
+//
+// page_bounds: mn[d], mx[d] = smallest and largest key value of dimension d
+// over the tokens of a page, per KV head. Bound: the K bytes read. One warp
+// per (page, head): a row of a key is D / 8 lanes of 16 bytes, the page's
+// rows are loaded before any is reduced, and the two-lane minimum and maximum
+// instructions of the 16-bit types (NaN propagates) keep it at a few
+// instructions per 16 bytes.
+//
+// select_pages: for query row n, KV head h and page g
+//   u = max over the heads of h's group of  sum_d max(q_d, 0) mx_d + min(q_d, 0) mn_d,
+// an upper bound of q . k over the page's keys. This is a matrix product of
+// (max(q, 0), min(q, 0)) with the stored (mx, mn) rows, so the bounds go from
+// global memory straight into matrix fragments (16 bytes a thread; the order
+// of the summed dimension is the same for both operands, so any order is
+// right) and no shared memory, unpacking or shuffle stands beside the loads.
+// Bound: the bytes of the bounds.
+//
+// The k pages of highest u are those of exact arithmetic, ties to the lower
+// page: |fp32 result - exact| <= E = 2^-14 * max over pages of
+// sum |q_d| |bound_d| (256 * 2 products of one sum, each addition off by at
+// most 2^-23 of the largest partial sum; the products are exact in fp32). A page whose
+// fp32 score is over 2E above the k-th is in, one 2E below it is out, and the
+// few between are scored again in 64 bits (products of 16-bit values are
+// exact there).
+#include "attend_common.cuh"
+
+#include <algorithm>
+
+namespace daric {
+namespace {
+using namespace att;
+
+// ------------------------------------------------------------- bounds --
+template <class T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+  static __device__ __forceinline__ uint32_t mn(uint32_t a, uint32_t b) {
+    V r = __hmin2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint32_t mx(uint32_t a, uint32_t b) {
+    V r = __hmax2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+  static constexpr uint32_t kPosInf = 0x7f807f80u, kNegInf = 0xff80ff80u;
+};
+template <>
+struct Pair<__half> {
+  using V = __half2;
+  static __device__ __forceinline__ uint32_t mn(uint32_t a, uint32_t b) {
+    V r = __hmin2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint32_t mx(uint32_t a, uint32_t b) {
+    V r = __hmax2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+  static constexpr uint32_t kPosInf = 0x7c007c00u, kNegInf = 0xfc00fc00u;
+};
+
+constexpr int kBoundWarps = 8;
+
+template <class T, int D>
+__global__ void __launch_bounds__(kBoundWarps * 32) bounds_kernel(const __grid_constant__ BoundsLaunch p) {
+  constexpr int CH = D / 8;
+  constexpr int TPI = 32 / CH;  // tokens a warp reads at a time
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.y, H = p.kv.heads, bs = p.kv.page_size;
+  Seq s;
+  s.rows = 0;
+  s.len = __ldg(&p.sq.seq_lens[b]);
+  clamp_len(p.sq, bs, s);
+  const int start = p.start ? max(__ldg(&p.start[b]), 0) : 0;
+  const int p0 = (int)fdiv((uint32_t)start, p.kv.page_div);
+  const int pages = (s.len + bs - 1) / bs - p0;
+  const int c = lane % CH, t0 = lane / CH;
+  for (int64_t w = (int64_t)blockIdx.x * kBoundWarps + warp; w < (int64_t)pages * H;
+       w += (int64_t)gridDim.x * kBoundWarps) {
+    const int pg = p0 + (int)(w / H), h = (int)(w % H);
+    const int blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
+    if (blk < 0 || blk >= p.kv.num_pages) {
+      if (lane == 0) atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+      continue;
+    }
+    const uint8_t* src = p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)h * p.kv.head_stride + c * 16;
+    const int n = min(bs, s.len - pg * bs);
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo[e] = Pair<T>::kPosInf;
+      hi[e] = Pair<T>::kNegInf;
+    }
+    for (int t = t0; t < n; t += 8 * TPI) {
+      uint4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {  // a token past the end repeats one that is in
+        const int tt = t + u * TPI < n ? t + u * TPI : t;
+        v[u] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)tt * p.kv.tok_stride));
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(&v[u]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = Pair<T>::mn(lo[e], x[e]);
+          hi[e] = Pair<T>::mx(hi[e], x[e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = CH; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = Pair<T>::mn(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+        hi[e] = Pair<T>::mx(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+      }
+    if (lane < CH) {
+      uint4* dst = reinterpret_cast<uint4*>(p.bounds + ((int64_t)blk * H + h) * (4 * D)) + lane;
+      dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      dst[CH] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    }
+  }
+}
+
+// ------------------------------------------------------------- scores --
+// Order-preserving key of a score; every NaN is the largest key.
+__device__ __forceinline__ uint32_t key_of(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  if (k == 0xffffffffu) return __int_as_float(0x7fffffff);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ unsigned long long key64_of(double f) {
+  if (f != f) return ~0ull;
+  if (f == 0.0) f = 0.0;  // -0 and 0 are one value
+  const unsigned long long u = (unsigned long long)__double_as_longlong(f);
+  return (u >> 63) ? ~u : (u | (1ull << 63));
+}
+
+// Query row n against its sequence: pages it can see (0: no sequence).
+struct RowView {
+  int seq, pages;
+};
+__device__ __forceinline__ RowView row_view(const SeqBatch& sq, int page_size, int n) {
+  RowView v{find_seq(sq, n), 0};
+  if (v.seq < 0) return v;
+  Seq s = load_seq(sq, v.seq);
+  clamp_len(sq, page_size, s);
+  const int pos = s.ctx + (n - s.row0);
+  v.pages = pos < 0 || pos >= s.len ? 0 : pos / page_size + 1;
+  return v;
+}
+
+// The part of q that meets the stored minima (sign bit set) or maxima.
+__device__ __forceinline__ uint32_t q_part(uint32_t w, bool maxima) {
+  const uint32_t lo = w & 0xffffu, hi = w >> 16;
+  const uint32_t a = ((lo >> 15) != 0) != maxima ? lo : 0u, b = ((hi >> 15) != 0) != maxima ? hi : 0u;
+  return a | (b << 16);
+}
+
+constexpr int kScoreWarps = 8;
+
+template <class T, int D>
+__global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const __grid_constant__ SelectPagesLaunch p) {
+  constexpr int KB = D / 16;  // 64-byte pieces of (mn, mx): 2 D elements of 2 bytes
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = blockIdx.x, h = blockIdx.z, chunk = blockIdx.y;
+  const int g = lane >> 2, t = lane & 3;
+  __shared__ float s_mag[kScoreWarps];
+  const RowView rv = row_view(p.sq, p.page_size, n);
+  if (rv.pages <= p.k || chunk * kScoreChunk >= rv.pages) return;  // every page is taken, or none is here
+  const int group = p.sq.group;
+  const int32_t* trow = p.sq.table + (int64_t)rv.seq * p.sq.table_ld;
+  uint32_t* keys = p.keys + ((int64_t)n * p.heads + h) * p.sq.table_cols;
+  float mag = 0.f;
+  for (int it = 0; it < kScoreChunk / (kScoreWarps * 16); ++it) {
+    const int g0 = chunk * kScoreChunk + (it * kScoreWarps + warp) * 16;
+    if (g0 >= rv.pages) break;
+    // rows g and g + 8 of the tile: two pages
+    uint4 a[2][KB];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int pg = g0 + g + 8 * r;
+      int blk = pg < rv.pages ? __ldg(&trow[pg]) : -1;
+      if (pg < rv.pages && (blk < 0 || blk >= p.num_pages)) {
+        atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+        blk = -1;
+      }
+      const uint4* src = reinterpret_cast<const uint4*>(p.bounds + ((int64_t)max(blk, 0) * p.heads + h) * (4 * D)) + t;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) a[r][k] = blk >= 0 ? __ldg(src + 4 * k) : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t best[2] = {0u, 0u};
+    for (int q0 = 0; q0 < group; q0 += 8) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      const bool real = q0 + g < group;
+      const uint4* qp = reinterpret_cast<const uint4*>(
+          p.q + (int64_t)n * p.q_row + (int64_t)(h * group + (real ? q0 + g : 0)) * p.q_head) + t;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const bool maxima = k >= KB / 2;
+        uint4 w = real ? __ldg(qp + 4 * (k - (maxima ? KB / 2 : 0))) : make_uint4(0, 0, 0, 0);
+        w = make_uint4(q_part(w.x, maxima), q_part(w.y, maxima), q_part(w.z, maxima), q_part(w.w, maxima));
+        const uint4 u = a[0][k], v = a[1][k];
+        constexpr uint32_t M = 0x7fff7fffu;
+        { uint32_t f[4] = {u.x, v.x, u.y, v.y}; Mma<T>::run(x, f, w.x, w.y); }
+        { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x, f, w.z, w.w); }
+        { uint32_t f[4] = {u.x & M, v.x & M, u.y & M, v.y & M}; Mma<T>::run(y, f, w.x & M, w.y & M); }
+        { uint32_t f[4] = {u.z & M, v.z & M, u.w & M, v.w & M}; Mma<T>::run(y, f, w.z & M, w.w & M); }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (q0 + 2 * t + (e & 1) < group) {
+          best[e >> 1] = max(best[e >> 1], key_of(x[e]));
+          // a NaN or infinite magnitude stays the largest
+          mag = (y[e] <= mag) ? mag : (y[e] == y[e] ? y[e] : __int_as_float(0x7f800000));
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
+      best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
+      const int pg = g0 + g + 8 * r;
+      if (t == 0 && pg < rv.pages) keys[pg] = best[r];
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+  if (lane == 0) s_mag[warp] = mag;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kScoreWarps; ++w) mag = fmaxf(mag, s_mag[w]);
+    p.mags[((int64_t)n * p.heads + h) * gridDim.y + chunk] = mag;
+  }
+}
+
+// ------------------------------------------------------------- select --
+constexpr int kBins = 2048;
+constexpr int kNear = 256;  // candidates ranked against each other at once
+
+// Block-wide exclusive prefix sum; *total gets the sum. All threads call it.
+__device__ __forceinline__ int block_prefix(int v, int* total, int* sm) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sm[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = lane < nw ? sm[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    if (lane < nw) sm[lane] = w;
+  }
+  __syncthreads();
+  *total = sm[nw - 1];
+  return x - v + (warp > 0 ? sm[warp - 1] : 0);
+}
+
+// Digit of the rem-th largest entry of hist[0, bins), and the entries above it.
+__device__ __forceinline__ void find_digit(const uint32_t* hist, int bins, int rem, int* s_digit, int* s_above, int* sm) {
+  const int per = (bins + blockDim.x - 1) / blockDim.x;
+  int mine = 0;
+  for (int i = 0; i < per; ++i) {  // thread 0 owns the highest digits
+    const int d = bins - 1 - ((int)threadIdx.x * per + i);
+    if (d >= 0) mine += (int)hist[d];
+  }
+  int total;
+  int above = block_prefix(mine, &total, sm);
+  if (above < rem && rem <= above + mine) {
+    for (int i = 0; i < per; ++i) {
+      const int d = bins - 1 - ((int)threadIdx.x * per + i);
+      if (d < 0) break;
+      if (above < rem && rem <= above + (int)hist[d]) {
+        *s_digit = d;
+        *s_above = above;
+      }
+      above += (int)hist[d];
+    }
+  }
+  __syncthreads();
+}
+
+// Score of a page in 64 bits (all lanes of a warp call it with one page).
+template <class T, int D>
+__device__ __forceinline__ unsigned long long exact_key(const SelectPagesLaunch& p, int n, int h, int blk) {
+  const int lane = threadIdx.x & 31, group = p.sq.group;
+  const uint16_t* bd = reinterpret_cast<const uint16_t*>(p.bounds + ((int64_t)max(blk, 0) * p.heads + h) * (4 * D));
+  unsigned long long best = 0;
+  for (int e = 0; e < group; ++e) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + (int64_t)n * p.q_row + (int64_t)(h * group + e) * p.q_head);
+    double u = 0.0;
+    for (int d = lane; d < D; d += 32) {
+      const double qv = (double)Mma<T>::widen(__ldg(&q[d]));
+      const double lo = blk >= 0 ? (double)Mma<T>::widen(__ldg(&bd[d])) : 0.0;
+      const double hi = blk >= 0 ? (double)Mma<T>::widen(__ldg(&bd[D + d])) : 0.0;
+      u += (qv > 0.0 ? qv : 0.0) * hi + (qv < 0.0 ? qv : 0.0) * lo;
+      if (qv != qv) u = qv;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    const unsigned long long k = key64_of(u);
+    best = k > best ? k : best;
+  }
+  return best;
+}
+
+template <class T, int D>
+__global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, int chunks, int staged) {
+  extern __shared__ uint32_t dyn[];  // [bitmap words | staged keys]
+  __shared__ uint32_t hist[kBins];
+  __shared__ int sm[32];
+  __shared__ int s_digit, s_above, s_near;
+  __shared__ float s_e;
+  __shared__ int near_page[kNear];
+  __shared__ unsigned long long near_key[kNear];
+  const int n = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  const RowView rv = row_view(p.sq, p.page_size, n);
+  if (rv.seq < 0) return;  // a row behind the last sequence
+  int32_t* out = p.out + ((int64_t)n * p.heads + h) * p.k;
+  const int P = rv.pages;
+  if (P <= p.k) {
+    for (int i = tid; i < p.k; i += blockDim.x) out[i] = i < P ? i : -1;
+    return;
+  }
+  const int64_t item = (int64_t)n * p.heads + h;
+  const uint32_t* gkeys = p.keys + item * p.sq.table_cols;
+  const int words = (P + 31) / 32;
+  uint32_t* taken = dyn;
+  uint32_t* skeys = dyn + (p.sq.table_cols + 31) / 32;
+  const int32_t* trow = p.sq.table + (int64_t)rv.seq * p.sq.table_ld;
+  // eligible pages [e0, e1); the ones before and after are always taken
+  const int e0 = p.first, e1 = P - p.last;
+  const int kk = p.k - p.first - p.last;
+  if (tid == 0) s_near = 0;
+  float mag = 0.f;
+  for (int i = tid; i < (P + kScoreChunk - 1) / kScoreChunk; i += blockDim.x) mag = fmaxf(mag, p.mags[item * chunks + i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+  if (lane == 0) sm[warp] = __float_as_int(mag);
+  if (staged)
+    for (int i = tid; i < P; i += blockDim.x) skeys[i] = gkeys[i];
+  for (int i = tid; i < words; i += blockDim.x) taken[i] = 0;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < nw; ++w) mag = fmaxf(mag, __int_as_float(sm[w]));
+    s_e = mag * 6.103515625e-05f;  // E = 2^-14 of the largest magnitude
+  }
+  __syncthreads();
+  auto key_at = [&](int i) { return staged ? skeys[i] : gkeys[i]; };
+  const float E = s_e;
+
+  if (kk > 0) {
+    // k-th largest fp32 key: digits of 11, 11 and 10 bits
+    uint32_t prefix = 0, mask = 0;
+    int rem = kk;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
+      for (int i = tid; i < kBins; i += blockDim.x) hist[i] = 0;
+      __syncthreads();
+      for (int i = e0 + tid; i < e1; i += blockDim.x) {
+        const uint32_t k = key_at(i);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (uint32_t)(bins - 1)], 1u);
+      }
+      __syncthreads();
+      find_digit(hist, bins, rem, &s_digit, &s_above, sm);
+      prefix |= (uint32_t)s_digit << shift;
+      mask |= (uint32_t)(bins - 1) << shift;
+      rem -= s_above;
+      __syncthreads();
+    }
+    // pages certainly in, and those whose order against the k-th fp32 cannot tell
+    const float t = value_of(prefix);
+    const bool wide = !(E < 1e38f) || !(fabsf(t) < 1e38f);  // infinities or NaN about: settle all in 64 bits
+    const float hi = t + 2.f * E, lo = t - 2.f * E;
+    int in = 0, near = 0;
+    for (int i0 = e0; i0 < e1; i0 += blockDim.x) {
+      const int i = i0 + tid;
+      bool sure = false, maybe = false;
+      if (i < e1) {
+        const float v = value_of(key_at(i));
+        sure = !wide && v > hi;
+        maybe = wide || (v >= lo && v <= hi);
+      }
+      if (sure) atomicOr(&taken[i >> 5], 1u << (i & 31));
+      if (maybe) {
+        const int at = atomicAdd(&s_near, 1);
+        if (at < kNear) near_page[at] = i;
+      }
+      in += sure;
+      near += maybe;
+    }
+    int n_in, n_near;
+    block_prefix(in, &n_in, sm);
+    block_prefix(near, &n_near, sm);
+    const int need = kk - n_in;  // of the candidates
+    if (n_near <= need) {
+      for (int i = tid; i < n_near && i < kNear; i += blockDim.x) atomicOr(&taken[near_page[i] >> 5], 1u << (near_page[i] & 31));
+      if (n_near > kNear)
+        for (int i = e0 + tid; i < e1; i += blockDim.x) {
+          const float v = value_of(key_at(i));
+          if (wide || (v >= lo && v <= hi)) atomicOr(&taken[i >> 5], 1u << (i & 31));
+        }
+    } else if (n_near <= kNear) {
+      for (int i = warp; i < n_near; i += nw) {
+        const int blk = __ldg(&trow[near_page[i]]);
+        const unsigned long long k = exact_key<T, D>(p, n, h, blk >= 0 && blk < p.num_pages ? blk : -1);
+        if (lane == 0) near_key[i] = k;
+      }
+      __syncthreads();
+      for (int i = tid; i < n_near; i += blockDim.x) {
+        int better = 0;
+        for (int j = 0; j < n_near; ++j)
+          better += near_key[j] > near_key[i] || (near_key[j] == near_key[i] && near_page[j] < near_page[i]);
+        if (better < need) atomicOr(&taken[near_page[i] >> 5], 1u << (near_page[i] & 31));
+      }
+    } else {
+      // many candidates (pages alike): radix selection over their 64-bit
+      // keys, scored anew in every pass so that nothing has to be stored
+      unsigned long long pre = 0, msk = 0;
+      int left = need;
+      for (int pass = 0; pass < 8; ++pass) {
+        const int shift = 56 - 8 * pass;
+        for (int i = tid; i < 256; i += blockDim.x) hist[i] = 0;
+        __syncthreads();
+        for (int i = e0 + warp; i < e1; i += nw) {
+          const float v = value_of(key_at(i));
+          if (!(wide || (v >= lo && v <= hi))) continue;
+          const int blk = __ldg(&trow[i]);
+          const unsigned long long k = exact_key<T, D>(p, n, h, blk >= 0 && blk < p.num_pages ? blk : -1);
+          if (lane == 0 && (k & msk) == pre) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        find_digit(hist, 256, left, &s_digit, &s_above, sm);
+        pre |= (unsigned long long)s_digit << shift;
+        msk |= 255ull << shift;
+        left -= s_above;
+        __syncthreads();
+      }
+      // keys above the k-th are in; of the equal ones the `left` lowest pages:
+      // their places are found in page order by one warp per 32 pages
+      uint32_t* equal = hist;  // bitmap of a span of pages
+      for (int s0 = e0; s0 < e1; s0 += kBins * 32) {
+        const int s1 = min(e1, s0 + kBins * 32);
+        for (int i = tid; i < kBins; i += blockDim.x) equal[i] = 0;
+        __syncthreads();
+        for (int i = s0 + warp; i < s1; i += nw) {
+          const float v = value_of(key_at(i));
+          if (!(wide || (v >= lo && v <= hi))) continue;
+          const int blk = __ldg(&trow[i]);
+          const unsigned long long k = exact_key<T, D>(p, n, h, blk >= 0 && blk < p.num_pages ? blk : -1);
+          if (lane == 0) {
+            if (k > pre) atomicOr(&taken[i >> 5], 1u << (i & 31));
+            if (k == pre) atomicOr(&equal[(i - s0) >> 5], 1u << ((i - s0) & 31));
+          }
+        }
+        __syncthreads();
+        if (tid == 0) {
+          for (int w = 0; w < kBins && left > 0; ++w)
+            for (uint32_t m = equal[w]; m && left > 0; m &= m - 1, --left) {
+              const int i = s0 + w * 32 + (__ffs((int)m) - 1);
+              atomicOr(&taken[i >> 5], 1u << (i & 31));
+            }
+          s_near = left;
+        }
+        __syncthreads();
+        left = s_near;
+        __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+  // the pages that are always taken, then the list in ascending order
+  for (int i = tid; i < p.first + p.last; i += blockDim.x) {
+    const int pg = i < p.first ? i : P - p.last + (i - p.first);
+    atomicOr(&taken[pg >> 5], 1u << (pg & 31));
+  }
+  __syncthreads();
+  const int per = (words + blockDim.x - 1) / blockDim.x;
+  int mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int w = tid * per + i;
+    if (w < words) mine += __popc(taken[w]);
+  }
+  int total;
+  int at = block_prefix(mine, &total, sm);
+  for (int i = 0; i < per; ++i) {
+    const int w = tid * per + i;
+    if (w >= words) break;
+    for (uint32_t m = taken[w]; m; m &= m - 1) {
+      if (at < p.k) out[at] = w * 32 + (__ffs((int)m) - 1);
+      ++at;
+    }
+  }
+  for (int i = total + tid; i < p.k; i += blockDim.x) out[i] = -1;
+}
+
+template <class T, int D>
+void bounds_d(const BoundsLaunch& p, int sm_count, cudaStream_t s) {
+  const int64_t items = (int64_t)p.sq.table_cols * p.kv.heads;
+  int64_t x = (items + kBoundWarps - 1) / kBoundWarps;
+  // about eight CTAs per SM over all sequences; the warps stride over the rest
+  x = std::min<int64_t>(x, std::max<int64_t>(1, (int64_t)sm_count * 16 / p.sq.num_seqs));
+  bounds_kernel<T, D><<<dim3((unsigned)x, (unsigned)p.sq.num_seqs), kBoundWarps * 32, 0, s>>>(p);
+  DARIC_CUDA(cudaGetLastError());
+}
+
+template <class T, int D>
+void select_d(const SelectPagesLaunch& p, cudaStream_t s) {
+  const int chunks = (p.sq.table_cols + kScoreChunk - 1) / kScoreChunk;
+  if (p.sq.table_cols > p.k) {
+    page_score_kernel<T, D>
+        <<<dim3((unsigned)p.sq.num_rows, (unsigned)chunks, (unsigned)p.heads), kScoreWarps * 32, 0, s>>>(p);
+    DARIC_CUDA(cudaGetLastError());
+  }
+  // keys are staged in shared memory while they fit
+  const int words = (p.sq.table_cols + 31) / 32;
+  const int staged = p.sq.table_cols <= 40960;
+  const int bytes = (words + (staged ? p.sq.table_cols : 0)) * 4;
+  // a thread per eight keys, so that short tables keep many CTAs on an SM
+  const int threads = std::min(1024, std::max(128, (p.sq.table_cols / 8 + 31) / 32 * 32));
+  DARIC_CUDA(cudaFuncSetAttribute(page_select_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 190 * 1024));
+  page_select_kernel<T, D><<<dim3((unsigned)p.sq.num_rows, (unsigned)p.heads), threads, bytes, s>>>(p, chunks, staged);
+  DARIC_CUDA(cudaGetLastError());
+}
+
+}  // namespace
+
+#define DARIC_BY_DIM(F, T, ...)                        \
+  switch (dim) {                                       \
+    case 64: F<T, 64>(__VA_ARGS__); return;            \
+    case 128: F<T, 128>(__VA_ARGS__); return;          \
+    case 256: F<T, 256>(__VA_ARGS__); return;          \
+  }
+
+void launch_page_bounds(const BoundsLaunch& p, int dtype, int sm_count, cudaStream_t s) {
+  const int dim = p.kv.head_dim;
+  if (dtype == DARIC_DTYPE_BF16) { DARIC_BY_DIM(bounds_d, __nv_bfloat16, p, sm_count, s) }
+  if (dtype == DARIC_DTYPE_F16) { DARIC_BY_DIM(bounds_d, __half, p, sm_count, s) }
+  throw Error(DARIC_ERR_INVALID, "page_bounds: bfloat16 or float16 keys of 64, 128 or 256");
+}
+
+void launch_select_pages(const SelectPagesLaunch& p, int dtype, cudaStream_t s) {
+  const int dim = p.head_dim;
+  if (dtype == DARIC_DTYPE_BF16) { DARIC_BY_DIM(select_d, __nv_bfloat16, p, s) }
+  if (dtype == DARIC_DTYPE_F16) { DARIC_BY_DIM(select_d, __half, p, s) }
+  throw Error(DARIC_ERR_INVALID, "select_pages: bfloat16 or float16 keys of 64, 128 or 256");
+}
+
+}  // namespace daric

@@ -20,6 +20,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "attend.h"
 #include "internal.h"
 
 using namespace daric;
@@ -1273,6 +1274,72 @@ void record_error(int code, const char* msg) {
   g_last_error = msg;
 }
 void clear_error() { g_last_error.clear(); }
+
+DeviceInfo device_info(int device) {
+  DeviceCtx& dc = device_ctx(device);
+  return DeviceInfo{dc.sm_count, dc.err_word};
+}
+
+// K and V rows of a layer by its sizes and strides, as register_rotary finds
+// them (adapter.py:311-368): 5-D, page-first 5-D or packed 4-D.
+LayerRef layer_ref(daric_copier* c, const char* name) {
+  DARIC_CHECK(c != nullptr, "copier is NULL");
+  const LayerHost& L = find_layer(c, name);
+  const auto& s = L.sizes;
+  const auto& st = L.strides;
+  const int64_t es = L.es;
+  LayerRef r{};
+  KvView& v = r.kv;
+  int64_t bs = 0, heads = 0, dim = 0;
+  v.base = L.data;
+  if (s.size() == 5) {
+    const int kv = L.page_first ? 1 : 0;
+    DARIC_CHECK(s[kv] == 2, "5-D KV cache must hold K and V (a dimension of 2): " + L.name);
+    v.page_stride = st[1 - kv] * es;
+    v.v_off = st[kv] * es;
+    bs = s[2];
+    heads = s[3];
+    dim = s[4];
+    v.tok_stride = st[2] * es;
+    v.head_stride = st[3] * es;
+    DARIC_CHECK(st[4] == 1 || dim == 1, "KV cache head dimension must have stride 1: " + L.name);
+  } else if (s.size() == 4) {
+    DARIC_CHECK(L.page_first && s[3] % 2 == 0,
+                "4-D KV cache must be page-first (blocks, heads, block_size, 2 * head_dim): " + L.name);
+    v.page_stride = st[0] * es;
+    heads = s[1];
+    bs = s[2];
+    dim = s[3] / 2;
+    v.head_stride = st[1] * es;
+    v.tok_stride = st[2] * es;
+    v.v_off = dim * es;
+    DARIC_CHECK(st[3] == 1, "KV cache packed dimension must have stride 1: " + L.name);
+  } else {
+    throw Error(DARIC_ERR_INVALID, "KV cache must be 5-D or packed 4-D to hold K and V rows: " + L.name);
+  }
+  DARIC_CHECK(bs >= 1 && bs <= 1024, "block size must be in [1, 1024]");
+  DARIC_CHECK(heads >= 1 && heads < 4096, "KV heads must be in [1, 4095]");
+  DARIC_CHECK((uintptr_t)L.data % 16 == 0 && v.page_stride % 16 == 0 && v.tok_stride % 16 == 0 &&
+                  v.head_stride % 16 == 0 && v.v_off % 16 == 0 && dim * es % 16 == 0,
+              "KV cache rows must be 16-byte aligned: " + L.name);
+  v.num_pages = L.num_pages;
+  v.page_size = (int32_t)bs;
+  v.heads = (int32_t)heads;
+  v.head_dim = (int32_t)dim;
+  v.page_div = make_fastdiv((uint32_t)bs);
+  r.device = L.device;
+  r.elem_size = es;
+  r.kv_dtype = L.has_rot ? L.kv_dtype : -1;
+  if (L.has_rot) {
+    r.table = L.dev.table;
+    r.table_row = L.dev.table_row;
+    r.max_pos = L.dev.max_pos;
+    r.tab_dtype = L.tab_dtype;
+    r.neox = L.neox;
+    r.half_rot = L.dev.half_rot;
+  }
+  return r;
+}
 }  // namespace daric
 
 // ===================================================================== C ==

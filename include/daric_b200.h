@@ -284,6 +284,111 @@ DARIC_API int daric_ptrs_to_slots(int64_t num_ranges, const int64_t* range_start
                         int64_t block_table_numel, int64_t block_size, int32_t* out_idx,
                         int64_t* out_slot, int device, void* stream);
 
+/* ======================================================================== */
+/* Attention, block selection and eviction over the paged KV cache          */
+/* (no counterpart in the reference).                                       */
+/*                                                                          */
+/* The batch of a call: sequence b has seq_lens[b] cache positions, position */
+/* p in slot block_table[b*table_ld + p/bs]*bs + p%bs; its query rows are    */
+/* q rows [cu_q[b], cu_q[b+1]) (cu_q NULL: num_rows/num_seqs each) and stand */
+/* at its last positions. All of these are device arrays: nothing is read   */
+/* on the host, no call waits for the GPU, allocates device memory or        */
+/* uploads anything, so calls may be captured into graphs (the first call   */
+/* on a device before any capture). A block id outside the layer counts as   */
+/* keys that do not exist (device error bit 1); lengths past the block table */
+/* and rows outside q are cut off (bit 4). Query heads are a multiple of the */
+/* layer's KV heads; head hq reads KV head hq / (q_heads / kv_heads).        */
+/* Layers: 5-D, page-first 5-D and packed 4-D, dtype BF16 or F16, head_dim   */
+/* 64, 128 or 256 (compact: every dtype, any head_dim of whole 16-byte       */
+/* vectors). Row and head strides of q and out are in elements, their rows   */
+/* 16-byte aligned. Workspaces belong to one call at a time.                 */
+/* ======================================================================== */
+
+/* Bytes of workspace of one tree_attention or sparse_attention call. */
+DARIC_API int daric_attend_workspace(int device, int64_t head_dim, int64_t* out_bytes);
+
+/* Softmax attention of each query row over its sequence. Row j of a sequence
+ * with T rows and length s sees positions < s - T and, of the last T, token i
+ * where bit i%64 of tree_mask[row*mask_words + i/64] is set (tree_mask NULL:
+ * i <= j). out [num_rows, q_heads, head_dim] in the layer's dtype; lse
+ * [num_rows, q_heads] fp32 (may be NULL), natural log. A row that sees nothing
+ * gets 0 and -inf; rows outside every sequence are not written. */
+DARIC_API int daric_copier_tree_attention(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
+                                int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
+                                const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                                const int32_t* seq_lens, const int32_t* cu_q, const int64_t* tree_mask,
+                                int64_t mask_words, float scale, void* out, int64_t out_row, int64_t out_head,
+                                float* lse, int64_t lse_row, void* workspace, int64_t workspace_bytes, int device,
+                                void* stream);
+
+/* The same over listed pages: pages[n*pages_row + h*pages_head + e], e < k,
+ * are page numbers (block-table columns) of query row n and KV head h;
+ * negative entries are empty, one past the block table is skipped (bit 4), a
+ * page listed twice counts twice. A row sees listed positions up to its own. */
+DARIC_API int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
+                                  int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
+                                  const int32_t* pages, int64_t pages_row, int64_t pages_head, int64_t k,
+                                  const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                                  const int32_t* seq_lens, const int32_t* cu_q, float scale, void* out,
+                                  int64_t out_row, int64_t out_head, float* lse, int64_t lse_row, void* workspace,
+                                  int64_t workspace_bytes, int device, void* stream);
+
+/* bounds[block][head][0 / 1][d] = smallest / largest K value of dimension d
+ * over the page's tokens below seq_lens, for every page that holds a position
+ * in [start[b], seq_lens[b]) (start NULL: 0). Contiguous, layer dtype. */
+DARIC_API int daric_copier_page_bounds(daric_copier* copier, const char* layer_name, int kv_dtype, const int32_t* block_table,
+                             int64_t table_ld, int64_t num_seqs, int64_t table_cols, const int32_t* seq_lens,
+                             const int32_t* start, void* bounds, int device, void* stream);
+
+/* Bytes of workspace of one select_pages call. */
+DARIC_API int daric_select_pages_workspace(int64_t num_rows, int64_t kv_heads, int64_t table_cols, int64_t* out_bytes);
+
+/* out[n][h][0..k) = pages of row n and KV head h, ascending, padded with -1:
+ * of the pages up to the row's own position the first `first` and the last
+ * `last` (>= 1), then those of highest
+ *   max over the head's query heads of sum_d max(q_d min_d, q_d max_d),
+ * in the order of exact arithmetic, ties to the lower page, NaN highest. */
+DARIC_API int daric_select_pages(const void* q, int kv_dtype, int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads,
+                       int64_t head_dim, const void* bounds, int64_t num_pages, int64_t kv_heads,
+                       const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                       const int32_t* seq_lens, const int32_t* cu_q, int64_t block_size, int64_t k, int64_t first,
+                       int64_t last, int32_t* out, void* workspace, int64_t workspace_bytes, int device,
+                       void* stream);
+
+/* Bytes of workspace of one attention_scores call without an lse. */
+DARIC_API int daric_scores_workspace(int64_t num_rows, int64_t q_heads, int64_t table_cols, int64_t block_size,
+                           int64_t* out_bytes);
+
+/* scores[h*scores_row + col_off[b] + p] (accumulate: +)= sum over the rows of
+ * sequence b that see p and the query heads of KV head h of
+ * exp(scale q.k_p - lse). lse as tree_attention returned it for the same rows
+ * and mask; NULL: computed here (needs the workspace). Rows with lse -inf add
+ * nothing. A sequence whose columns reach outside [0, scores_cols) is left
+ * out (bit 4). */
+DARIC_API int daric_copier_attention_scores(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
+                                  int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
+                                  const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,
+                                  const int32_t* seq_lens, const int32_t* cu_q, const int64_t* tree_mask,
+                                  int64_t mask_words, const float* lse, int64_t lse_row, float scale, float* scores,
+                                  int64_t scores_row, int64_t scores_cols, const int64_t* col_off, int accumulate,
+                                  void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+/* Kept tokens move to the front, in place: token n of list r and segment s,
+ * idx[r*idx_row + out_off[s] + n] for n < min(count[r*count_row + s],
+ * seg_cap[s]), goes to position dst_start[s] + n (NULL: n) of the block table
+ * at block_table + seg_blk_off[s], K and V. lists = num_layers (or 1 for all
+ * layers), times the KV heads with per_head (row layer*heads + head).
+ * Positions ascend and are >= dst_start[s] + n; an entry that breaks this is
+ * left out (bit 4), as is one outside the block table (4), with a bad block
+ * id (1) or outside the rotary table (2). mode FLEXIBLE turns K from its old
+ * to its new position by the layers' rotary tables, in fp32, rounded once.
+ * Host arrays: out_off, seg_cap, seg_blk_off, dst_start (num_segs). */
+DARIC_API int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* const* layer_names, int kv_dtype,
+                         int mode, int64_t lists, int per_head, const int32_t* idx, int64_t idx_row,
+                         const int32_t* count, int64_t count_row, int64_t num_segs, const int64_t* out_off,
+                         const int64_t* seg_cap, const int64_t* seg_blk_off, const int64_t* dst_start,
+                         const int32_t* block_table, int64_t block_table_numel, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
