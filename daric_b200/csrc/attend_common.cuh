@@ -7,8 +7,22 @@
 
 #include "attend.h"
 
+#include <atomic>
+
 namespace daric {
 namespace att {
+
+// Raises a kernel's dynamic shared memory limit once per device (the current
+// one); `done` is the caller's static mask of devices.
+template <class K>
+void allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  DARIC_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  DARIC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

@@ -36,12 +36,12 @@ constexpr int kThreads = 128;
 template <int D, int RG>
 struct Geom {
   static constexpr int KG = 4 / RG;                                     // key groups
-  static constexpr int KT = RG == 4 ? (D > 128 ? 32 : 64) : (D > 128 && RG == 1 ? 16 : 32);  // keys of a chunk
+  static constexpr int KT = RG == 1 ? 16 : 32;                          // keys of a chunk
   static constexpr int KPW = KT / RG;                                   // keys a warp loads of a chunk
   static constexpr int TILE = KT * KG;                                  // keys of a tile
   static constexpr int PITCH = D * 2 + 16;
   static constexpr int STAGE = 2 * KT * PITCH;
-  static constexpr int S = (KG * STAGE * 4 <= 200 * 1024) ? 4 : 3;
+  static constexpr int S = D > 128 && RG == 4 ? 4 : 3;                  // stages of a ring
   static constexpr int ROWS = 16 * RG;
   static constexpr int RING = KG * S * STAGE;
   static constexpr int QB = ROWS * PITCH;
@@ -65,7 +65,7 @@ __device__ __forceinline__ int tiles_of(const AttendLaunch& p, const Seq& s) {
 }
 
 template <class T, int D, int RG, bool SPARSE>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ AttendLaunch p) {
+__global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) attend_kernel(const __grid_constant__ AttendLaunch p) {
   using G = Geom<D, RG>;
   constexpr int CH = D / 8;  // 16-byte vectors of a row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -195,55 +195,66 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     const int32_t* trow = p.sq.table + (int64_t)seq_id * p.sq.table_ld;
     const int32_t* prow = SPARSE ? p.pages + (int64_t)sg.b * p.pages_row + (int64_t)sg.h * p.pages_head : nullptr;
     const int64_t head_off = (int64_t)sg.h * p.kv.head_stride;
-    int nxt_blk = -1, nxt_in = 0;
-    bool nxt_some = false;
-    auto lookup = [&](int c) {  // block of key `lane` (of this warp's share) of chunk c
-      nxt_some = false;
+    // A warp's share of a chunk lies in one page when the page size is a
+    // multiple of it: one lookup and one address serve all its rows. Else
+    // lane i looks key i up and the rows' addresses go round by shuffles.
+    const bool one = p.kv.page_size % G::KPW == 0;
+    int nxt_blk = -1, nxt_in = 0, nxt_n = 0;  // block, first row in it, rows (one) or 1 / 0 (else)
+    auto lookup = [&](int c) {                // of this warp's share of chunk c
+      nxt_n = 0;
       nxt_blk = -1;
-      if (lane < G::KPW && c < n) {
-        const int i = (tile0 + c) * G::TILE + kg * G::KT + rg * G::KPW + lane;
+      if (c < n && (one || lane < G::KPW)) {
+        const int i = (tile0 + c) * G::TILE + kg * G::KT + rg * G::KPW + (one ? 0 : lane);
         const int e = (int)fdiv((uint32_t)i, p.kv.page_div);
         nxt_in = i - e * p.kv.page_size;
-        int pg = e;
-        bool ok;
+        int pg = e, left = sg.s.len - i;
         if (SPARSE) {
-          pg = e < p.k ? __ldg(&prow[e]) : -1;
-          ok = pg >= 0 && seq_id >= 0;
-          if (ok && pg >= p.sq.table_cols) {
+          pg = e < p.k && seq_id >= 0 ? __ldg(&prow[e]) : -1;
+          if (pg >= p.sq.table_cols) {
             atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
-            ok = false;
+            pg = -1;
           }
-          ok = ok && (int64_t)pg * p.kv.page_size + nxt_in <= qpos;
-        } else {
-          ok = i < sg.s.len;
+          left = pg < 0 ? 0 : qpos + 1 - pg * p.kv.page_size - nxt_in;
         }
-        if (ok) {
+        if (left > 0) {
           nxt_blk = __ldg(&trow[pg]);
-          nxt_some = true;
+          nxt_n = one ? min(left, G::KPW) : 1;
         }
       }
     };
     auto issue = [&](int stage) {  // copies of the chunk that lookup() saw last
-      bool ok = nxt_some;
+      const uint32_t dst = smem_u32(ring) + stage * G::STAGE + rg * G::KPW * G::PITCH;
+      bool ok = nxt_n > 0;
       if (ok && (nxt_blk < 0 || nxt_blk >= p.kv.num_pages)) {
         atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
         ok = false;
       }
-      const unsigned valid = __ballot_sync(0xffffffffu, ok);
-      if (lane == 0) s_valid[kg][stage][rg] = valid;
       const int64_t off = ok ? (int64_t)nxt_blk * p.kv.page_stride + (int64_t)nxt_in * p.kv.tok_stride + head_off : 0;
-      const uint32_t dst = smem_u32(ring) + stage * G::STAGE + rg * G::KPW * G::PITCH;
-      constexpr int VECS = G::KPW * CH;
-#pragma unroll 4
-      for (int v0 = 0; v0 < VECS; v0 += 32) {
-        const int v = v0 + lane;
-        const int r = v / CH, c = v % CH;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r & 31);
-        if (VECS % 32 == 0 || v < VECS) {
+      constexpr int RPI = 32 / CH;  // rows a warp copies at a time
+      const int r0 = lane / CH, c16 = (lane % CH) * 16;
+      const uint32_t d0 = dst + r0 * G::PITCH + c16;
+      if (one) {
+        const int rows = ok ? nxt_n : 0;
+        if (lane == 0) s_valid[kg][stage][rg] = (uint32_t)((1ull << rows) - 1);
+        const uint8_t* src = p.kv.base + off + r0 * p.kv.tok_stride + c16;
+#pragma unroll
+        for (int i = 0; i < G::KPW / RPI; ++i) {
+          const bool in = r0 + i * RPI < rows;
+          const uint8_t* k = in ? src + i * RPI * p.kv.tok_stride : p.kv.base;
+          cp16(d0 + i * RPI * G::PITCH, k, in);
+          cp16(d0 + (G::KT + i * RPI) * G::PITCH, in ? k + p.kv.v_off : k, in);
+        }
+      } else {
+        const unsigned valid = __ballot_sync(0xffffffffu, ok);
+        if (lane == 0) s_valid[kg][stage][rg] = valid;
+#pragma unroll 2
+        for (int i = 0; i < G::KPW / RPI; ++i) {
+          const int r = r0 + i * RPI;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
           const bool in = (valid >> r) & 1;
-          const uint8_t* src = p.kv.base + o + c * 16;
-          cp16(dst + r * G::PITCH + c * 16, src, in);
-          cp16(dst + G::KT * G::PITCH + r * G::PITCH + c * 16, in ? src + p.kv.v_off : src, in);
+          const uint8_t* k = p.kv.base + o + (in ? c16 : 0);
+          cp16(d0 + i * RPI * G::PITCH, k, in);
+          cp16(d0 + (G::KT + i * RPI) * G::PITCH, in ? k + p.kv.v_off : k, in);
         }
       }
     };
@@ -533,7 +544,8 @@ template <class T, int D, int RG, bool SPARSE>
 void launch_one(const AttendLaunch& p, int grid, cudaStream_t s) {
   auto kern = attend_kernel<T, D, RG, SPARSE>;
   constexpr int bytes = Geom<D, RG>::SMEM;
-  DARIC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  static std::atomic<uint64_t> done{0};
+  allow_smem(kern, bytes, done);
   kern<<<grid, kThreads, bytes, s>>>(p);
   DARIC_CUDA(cudaGetLastError());
   join_kernel<T, D, RG><<<dim3((unsigned)grid, 4 * RG), 128, 0, s>>>(p);

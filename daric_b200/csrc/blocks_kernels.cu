@@ -532,7 +532,8 @@ void select_d(const SelectPagesLaunch& p, cudaStream_t s) {
   const int bytes = (words + (staged ? p.sq.table_cols : 0)) * 4;
   // a thread per eight keys, so that short tables keep many CTAs on an SM
   const int threads = std::min(1024, std::max(128, (p.sq.table_cols / 8 + 31) / 32 * 32));
-  DARIC_CUDA(cudaFuncSetAttribute(page_select_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 190 * 1024));
+  static std::atomic<uint64_t> done{0};
+  allow_smem(page_select_kernel<T, D>, 190 * 1024, done);
   page_select_kernel<T, D><<<dim3((unsigned)p.sq.num_rows, (unsigned)p.heads), threads, bytes, s>>>(p, chunks, staged);
   DARIC_CUDA(cudaGetLastError());
 }
