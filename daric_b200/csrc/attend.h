@@ -51,6 +51,7 @@ struct SeqBatch {
   const uint64_t* mask;   // [N, mask_words] drafted-token bits, null: causal
   int32_t mask_words;
   int32_t group;          // query heads per KV head
+  FastDiv group_div;
   int32_t* err;
 };
 
@@ -117,8 +118,9 @@ struct ScoresLaunch {
   float2* part;
   float* lse_work;
   int32_t splits;
+  int32_t sm_count;
 };
-constexpr int kScoreKeys = 512;  // keys of a CTA
+constexpr int kLseKeys = 256;  // keys of a split
 void launch_scores(const ScoresLaunch& p, int dtype, cudaStream_t s);
 
 // Kept tokens of up to kCompactSegs segments move to the front of their
@@ -151,10 +153,12 @@ struct CompactLaunch {
   int32_t shared;          // one list for all layers
   int32_t rotate, neox, half_rot;
   int64_t table_row, max_pos;
-  int32_t slices;          // CTAs a row is split over by columns
+  // pieces of the rows (launch_compact): turning columns, then those that move
+  int32_t turn_pieces, turn_heads, turn_slices, slices;
+  int32_t vecs, rot_vecs, tail0;  // 16-byte vectors of a row, turning tasks, first K vector that only moves
   CompactSeg segs[kCompactSegs];
   CompactLayer layers[kCompactLayers];
 };
-void launch_compact(const CompactLaunch& p, int kv_dtype, int tab_dtype, cudaStream_t s);
+void launch_compact(CompactLaunch& p, int kv_dtype, int tab_dtype, int elem, int sm_count, cudaStream_t s);
 
 }  // namespace daric

@@ -72,6 +72,7 @@ SeqBatch seq_batch(const int32_t* table, int64_t table_ld, int64_t num_seqs, int
   b.num_rows = (int32_t)num_rows;
   b.rows_each = (int32_t)(num_rows / num_seqs);
   b.group = (int32_t)(q_heads / kv_heads);
+  b.group_div = make_fastdiv((uint32_t)b.group);
   return b;
 }
 
@@ -302,7 +303,7 @@ int daric_scores_workspace(int64_t num_rows, int64_t q_heads, int64_t table_cols
   return guard([&] {
     DARIC_CHECK(out_bytes, "out_bytes is NULL");
     DARIC_CHECK(num_rows >= 0 && q_heads >= 1 && table_cols >= 1 && block_size >= 1, "sizes out of range");
-    const int64_t splits = std::min<int64_t>((table_cols * block_size + kScoreKeys - 1) / kScoreKeys, 64);
+    const int64_t splits = (table_cols * block_size + kLseKeys - 1) / kLseKeys;
     *out_bytes = num_rows * q_heads * (splits * 8 + 4) + 16;
   });
 }
@@ -326,8 +327,8 @@ int daric_copier_attention_scores(daric_copier* copier, const char* layer_name, 
     DARIC_CHECK(!tree_mask || mask_words >= 1, "tree mask needs at least one word per row");
     DARIC_CHECK(num_rows == 0 || aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
     DARIC_CHECK(scores_cols >= 0 && (scores_row >= scores_cols || L.kv.heads == 1), "score rows overlap");
-    const int64_t tiles = (table_cols * L.kv.page_size + kScoreKeys - 1) / kScoreKeys;
-    DARIC_CHECK(tiles <= 65535, "attention_scores: sequences of at most 33.5M positions");
+    const int64_t splits = (table_cols * L.kv.page_size + kLseKeys - 1) / kLseKeys;
+    DARIC_CHECK(splits <= 65535, "attention_scores: sequences of at most 16.7M positions");
     const DeviceInfo di = device_info(device);
     p.sq.err = di.err;
     p.sq.mask = reinterpret_cast<const uint64_t*>(tree_mask);
@@ -343,7 +344,8 @@ int daric_copier_attention_scores(daric_copier* copier, const char* layer_name, 
     p.col_off = col_off;
     p.accumulate = accumulate ? 1 : 0;
     p.scale = scale;
-    p.splits = (int32_t)std::min<int64_t>(tiles, 64);
+    p.splits = (int32_t)splits;
+    p.sm_count = di.sm_count;
     if (num_rows == 0) p.lse = scores;  // no rows: never read, and nothing to join
     if (!p.lse) {
       DARIC_CHECK(workspace && (uintptr_t)workspace % 8 == 0, "workspace must be an 8-byte aligned device buffer");
@@ -387,6 +389,9 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
       DARIC_CHECK(L.kv.page_size == A.kv.page_size && L.kv.heads == A.kv.heads && L.kv.head_dim == A.kv.head_dim &&
                       L.kv.num_pages == A.kv.num_pages,
                   "compact: layers of one call must share block size, blocks, heads and head dimension");
+      // places of tokens are kept in 32 bits of 16 bytes
+      DARIC_CHECK((double)L.kv.num_pages * (double)L.kv.page_stride < 60.0 * (1ll << 30),
+                  "compact: layers of less than 60 GiB");
       if (rotate) {
         DARIC_CHECK(L.table, std::string("layer has no rotary table (register_rotary): ") + layer_names[l]);
         DARIC_CHECK(L.tab_dtype == A.tab_dtype && L.neox == A.neox && L.half_rot == A.half_rot &&
@@ -409,6 +414,7 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
     p.count_row = count_row;
     p.block_table = block_table;
     p.table_numel = block_table_numel;
+    DARIC_CHECK((int64_t)A.kv.head_dim * es <= 4096, "compact: rows of at most 4096 bytes");
     const DeviceInfo di = device_info(device);
     p.err = di.err;
     p.num_pages = A.kv.num_pages;
@@ -419,8 +425,8 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
     p.per_head = per_head ? 1 : 0;
     p.shared = shared;
     p.rotate = rotate;
-    p.neox = A.neox;
-    p.half_rot = A.half_rot;
+    p.neox = rotate ? A.neox : 1;
+    p.half_rot = rotate ? A.half_rot : 0;
     p.table_row = A.table_row;
     p.max_pos = A.max_pos;
     for (int64_t s = 0; s < num_segs; ++s) {
@@ -442,13 +448,7 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
         for (int s = 0; s < p.num_segs; ++s)
           p.segs[s] = CompactSeg{seg_blk_off[s0 + s], out_off[s0 + s], (int32_t)seg_cap[s0 + s],
                                  (int32_t)(dst_start ? dst_start[s0 + s] : 0), (int32_t)(s0 + s)};
-        // few CTAs: their rows are split by columns (pieces of 64 bytes still
-        // move whole sectors)
-        const int64_t ctas = (int64_t)p.heads * 2 * p.num_segs * p.num_layers;
-        const int row = A.kv.head_dim * es;
-        p.slices = 1;
-        while (p.slices < 4 && row / (p.slices * 2) >= 64 && ctas * p.slices < 3 * (int64_t)di.sm_count) p.slices *= 2;
-        launch_compact(p, kv_dtype, A.tab_dtype, (cudaStream_t)stream);
+        launch_compact(p, kv_dtype, A.tab_dtype, es, di.sm_count, (cudaStream_t)stream);
       }
     }
   });

@@ -7,11 +7,12 @@
 // sum stays in the four threads that hold its row: no atomics, one fixed order
 // of additions. A warp holds 32 keys in registers (16 bytes a thread straight
 // from the cache: both operands take the head dimension in the same permuted
-// order, which leaves the products alone) and passes all query rows by them.
+// order, which leaves the products alone) and passes all query rows by them
+// (16 keys where the rows are few).
 // Bound: the K bytes for a few rows, the matrix and exp2 rates for many.
 //
 // Without an lse, lse_kernel first runs the same products and keeps the
-// maximum and the sum of each query row over the 512 keys of a CTA;
+// maximum and the sum of each query row over the 256 keys of a CTA;
 // lse_join_kernel joins them. K is read twice then (the second time from the
 // L2 cache for prompts up to about 100 MB of keys).
 //
@@ -28,61 +29,77 @@
 #include "device_common.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace daric {
 namespace {
 using namespace att;
 
 constexpr int kSW = 8;  // warps of a score CTA
-constexpr int kKeysWarp = 32;
-static_assert(kScoreKeys % (kSW * kKeysWarp) == 0, "whole rounds");
 
-// 32 keys of a warp: pages, then the rows in fragment order.
-template <int D>
-struct KeyTile {
-  static constexpr int KB = D / 32;  // 64-byte pieces of a row
-  uint4 a[4][KB];                    // rows g, g + 8, g + 16, g + 24
-  unsigned valid;                    // bit r: this thread's row g + 8 r exists
-};
-
-template <int D>
-__device__ __forceinline__ void load_keys(const ScoresLaunch& p, const Seq& s, int b, int h, int key0, KeyTile<D>& kt) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int pos = key0 + lane;
-  int64_t off = -1;
-  if (pos < s.len) {
-    const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
-    const int blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
-    if (blk >= 0 && blk < p.kv.num_pages)
-      off = (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
-            (int64_t)h * p.kv.head_stride;
-    else
-      atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+// Address of the keys of a tile: M * 16 keys of a warp, lane i looks key i up.
+template <int M>
+__device__ __forceinline__ int64_t key_offset(const ScoresLaunch& p, const Seq& s, int b, int h, int key0) {
+  const int pos = key0 + (int)(threadIdx.x & (16 * M - 1));
+  if (pos >= s.len) return -1;
+  const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
+  const int blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
+  if (blk < 0 || blk >= p.kv.num_pages) {
+    atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+    return -1;
   }
-  kt.valid = 0;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int64_t o = __shfl_sync(0xffffffffu, off, g + 8 * r);
-    if (o >= 0) kt.valid |= 1u << r;
-#pragma unroll
-    for (int k = 0; k < KeyTile<D>::KB; ++k)
-      kt.a[r][k] = o >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.kv.base + o) + 4 * k + t) : make_uint4(0, 0, 0, 0);
-  }
+  return (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
+         (int64_t)h * p.kv.head_stride;
 }
 
-// Products of 32 keys and 8 query rows: x[m][e], m = 16-key half.
-template <class T, int D>
-__device__ __forceinline__ void key_products(const KeyTile<D>& kt, const uint8_t* qrow, bool real, float (&x)[2][4]) {
-  const int t = threadIdx.x & 3;
+// M * 16 keys in fragment order: rows g, g + 8 (, g + 16, g + 24).
+template <int D, int M>
+struct KeyTile {
+  static constexpr int KB = D / 32;  // 64-byte pieces of a row
+  uint4 a[2 * M][KB];
+  unsigned valid;                    // bit r: this thread's row g + 8 r exists
+
+  __device__ __forceinline__ void load(const ScoresLaunch& p, int64_t off) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    valid = 0;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int r = 0; r < 2 * M; ++r) {
+      const int64_t o = __shfl_sync(0xffffffffu, off, g + 8 * r);
+      if (o >= 0) valid |= 1u << r;
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+        a[r][k] = o >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.kv.base + o) + 4 * k + t) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+// Eight query rows in fragment order: pair i0 + g of the sequence.
+template <int D>
+struct QueryTile {
+  static constexpr int KB = D / 32;
+  uint4 w[KB];
+  __device__ __forceinline__ void load(const ScoresLaunch& p, const Seq& s, int h, int i0, int pairs) {
+    const int lane = threadIdx.x & 31, i = i0 + (lane >> 2), t = lane & 3;
+    const bool real = i < pairs;
+    const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
+    const uint4* q = reinterpret_cast<const uint4*>(p.q + (int64_t)(s.row0 + j) * p.q_row +
+                                                    (int64_t)(h * p.sq.group + i - j * p.sq.group) * p.q_head) + t;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) w[k] = real ? __ldg(q + 4 * k) : make_uint4(0, 0, 0, 0);
+  }
+};
+
+template <class T, int D, int M>
+__device__ __forceinline__ void key_products(const KeyTile<D, M>& kt, const QueryTile<D>& qt, float (&x)[M][4]) {
+#pragma unroll
+  for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[m][e] = 0.f;
 #pragma unroll
-  for (int k = 0; k < KeyTile<D>::KB; ++k) {
-    const uint4 w = real ? __ldg(reinterpret_cast<const uint4*>(qrow) + 4 * k + t) : make_uint4(0, 0, 0, 0);
+  for (int k = 0; k < D / 32; ++k) {
+    const uint4 w = qt.w[k];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    for (int m = 0; m < M; ++m) {
       const uint4 u = kt.a[2 * m][k], v = kt.a[2 * m + 1][k];
       { uint32_t f[4] = {u.x, v.x, u.y, v.y}; Mma<T>::run(x[m], f, w.x, w.y); }
       { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x[m], f, w.z, w.w); }
@@ -90,8 +107,12 @@ __device__ __forceinline__ void key_products(const KeyTile<D>& kt, const uint8_t
   }
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kSW * 32) weight_kernel(const __grid_constant__ ScoresLaunch p) {
+// A CTA takes `iters` rounds of kSW tiles of M * 16 keys. With M = 1 (few
+// query rows) the next round's keys are on their way while a round is worked
+// on; with M = 2 (many) the next eight query rows are.
+template <class T, int D, int M>
+__global__ void __launch_bounds__(kSW * 32, D > 128 ? 1 : (M == 1 ? 2 : 1)) weight_kernel(const __grid_constant__ ScoresLaunch p, int iters) {
+  constexpr int KEYS = 16 * M;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group;
   Seq s = load_seq(p.sq, b);
@@ -102,28 +123,37 @@ __global__ void __launch_bounds__(kSW * 32) weight_kernel(const __grid_constant_
     return;
   }
   const int pairs = s.rows * group;
-  for (int it = 0; it < kScoreKeys / (kSW * kKeysWarp); ++it) {
-    const int key0 = blockIdx.y * kScoreKeys + (it * kSW + warp) * kKeysWarp;
-    if (key0 >= s.len) return;
-    KeyTile<D> kt;
-    load_keys<D>(p, s, b, h, key0, kt);
-    const bool draft = key0 + kKeysWarp > s.ctx;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};  // keys g, g + 8, g + 16, g + 24
+  int key0 = (int)blockIdx.y * iters * kSW * KEYS + warp * KEYS;
+  if (key0 >= s.len) return;
+  KeyTile<D, M> kt, nx;
+  kt.load(p, key_offset<M>(p, s, b, h, key0));
+  int64_t off = iters > 1 ? key_offset<M>(p, s, b, h, key0 + kSW * KEYS) : -1;
+  QueryTile<D> qt;
+  qt.load(p, s, h, 0, pairs);
+  for (int it = 0; it < iters && key0 < s.len; ++it, key0 += kSW * KEYS) {
+    if (M == 1 && it + 1 < iters) {
+      nx.load(p, off);
+      off = it + 2 < iters ? key_offset<M>(p, s, b, h, key0 + 2 * kSW * KEYS) : -1;
+    }
+    const bool draft = key0 + KEYS > s.ctx;
+    float sum[2 * M];  // keys g, g + 8, ...
+#pragma unroll
+    for (int r = 0; r < 2 * M; ++r) sum[r] = 0.f;
     for (int i0 = 0; i0 < pairs; i0 += 8) {
-      const bool real = i0 + g < pairs;
-      const int i = real ? i0 + g : 0;
-      const uint8_t* qrow = p.q + (int64_t)(s.row0 + i / group) * p.q_row + (int64_t)(h * group + i % group) * p.q_head;
-      float x[2][4];
-      key_products<T, D>(kt, qrow, real, x);
+      QueryTile<D> qn;
+      if (M == 2 && pairs > 8) qn.load(p, s, h, i0 + 8 < pairs ? i0 + 8 : 0, pairs);
+      float x[M][4];
+      key_products<T, D, M>(kt, qt, x);
+      if (M == 1 && pairs > 8) qt.load(p, s, h, i0 + 8 < pairs ? i0 + 8 : 0, pairs);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int ci = i0 + 2 * t + e;  // this column's (row, head) pair
         if (ci >= pairs) continue;
-        const int j = ci / group, row = s.row0 + j;
-        const float z = __ldg(&p.lse[(int64_t)row * p.lse_row + h * group + ci % group]);
+        const int j = (int)fdiv((uint32_t)ci, p.sq.group_div), row = s.row0 + j;
+        const float z = __ldg(&p.lse[(int64_t)row * p.lse_row + h * group + ci - j * group]);
         if (z == DARIC_NEG_INF) continue;  // a row that sees nothing
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 2 * M; ++r) {
           const float w = exp2f(__fmaf_rn(x[r >> 1][(r & 1) * 2 + e], p.scale, -z) * kLog2e);
           bool ok = true;
           if (draft) {
@@ -133,9 +163,10 @@ __global__ void __launch_bounds__(kSW * 32) weight_kernel(const __grid_constant_
           if (ok) sum[r] += w;
         }
       }
+      if (M == 2 && pairs > 8) qt = qn;
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 2 * M; ++r) {
       sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
       sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
       const int pos = key0 + g + 8 * r;
@@ -145,85 +176,84 @@ __global__ void __launch_bounds__(kSW * 32) weight_kernel(const __grid_constant_
         *dst = p.accumulate ? *dst + add : add;
       }
     }
+    if (M == 1) kt = nx;
+    else if (it + 1 < iters) {
+      kt.load(p, off);
+      off = it + 2 < iters ? key_offset<M>(p, s, b, h, key0 + 2 * kSW * KEYS) : -1;
+    }
   }
 }
 
-// Maximum and sum of each query row over this CTA's keys.
+// Maximum and sum of each query row over the kLseKeys keys of a CTA (a split).
 template <class T, int D>
 __global__ void __launch_bounds__(kSW * 32) lse_kernel(const __grid_constant__ ScoresLaunch p) {
+  constexpr int M = 2, KEYS = 16 * M, COLS = 32;  // pairs between two meetings of the warps
+  static_assert(kSW * KEYS == kLseKeys, "one tile per warp");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group, split = blockIdx.y;
-  __shared__ float2 s_ml[kSW][8];
+  __shared__ float2 s_ml[2][kSW][COLS];
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int pairs = s.rows * group;
   const float cexp = p.scale * kLog2e;
-  constexpr int IT = kScoreKeys / (kSW * kKeysWarp);
-  for (int i0 = 0; i0 < pairs; i0 += 8) {
-    const bool real = i0 + g < pairs;
-    const int i = real ? i0 + g : 0;
-    const uint8_t* qrow = p.q + (int64_t)(s.row0 + i / group) * p.q_row + (int64_t)(h * group + i % group) * p.q_head;
-    float m[2] = {DARIC_NEG_INF, DARIC_NEG_INF}, l[2] = {0.f, 0.f};
-    for (int base = split * kScoreKeys; base < s.len; base += p.splits * kScoreKeys) {
-#pragma unroll 1
-      for (int it = 0; it < IT; ++it) {
-        const int key0 = base + (it * kSW + warp) * kKeysWarp;
-        if (key0 >= s.len) break;
-        KeyTile<D> kt;
-        load_keys<D>(p, s, b, h, key0, kt);
-        float x[2][4];
-        key_products<T, D>(kt, qrow, real, x);
-        const bool draft = key0 + kKeysWarp > s.ctx;
+  const int heads = p.kv.heads * group;
+  auto at = [&](int i) {  // part of pair i
+    const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
+    return ((int64_t)(s.row0 + j) * heads + h * group + i - j * group) * p.splits + split;
+  };
+  if (split * kLseKeys >= s.len) {  // behind the end: empty parts
+    for (int i = threadIdx.x; i < pairs; i += kSW * 32) p.part[at(i)] = make_float2(DARIC_NEG_INF, 0.f);
+    return;
+  }
+  const int key0 = split * kLseKeys + warp * KEYS;
+  KeyTile<D, M> kt;
+  kt.load(p, key_offset<M>(p, s, b, h, key0));
+  const bool draft = key0 + KEYS > s.ctx;
+  QueryTile<D> qt;
+  qt.load(p, s, h, 0, pairs);
+  for (int c0 = 0, par = 0; c0 < pairs; c0 += COLS, par ^= 1) {
+    for (int i0 = c0; i0 < c0 + COLS && i0 < pairs; i0 += 8) {
+      QueryTile<D> qn;
+      if (i0 + 8 < pairs) qn.load(p, s, h, i0 + 8, pairs);
+      float x[M][4];
+      key_products<T, D, M>(kt, qt, x);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int ci = i0 + 2 * t + e;
-          const int j = ci / group;
-          float y[4];
-          float mx = m[e];
+      for (int e = 0; e < 2; ++e) {
+        const int ci = i0 + 2 * t + e;
+        const int j = (int)fdiv((uint32_t)ci, p.sq.group_div);
+        float y[2 * M], mx = DARIC_NEG_INF, l = 0.f;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            y[r] = x[r >> 1][(r & 1) * 2 + e];
-            bool ok = ((kt.valid >> r) & 1u) && ci < pairs;
-            if (ok && draft) {
-              const int d = key0 + g + 8 * r - s.ctx;
-              ok = d < 0 || sees_draft(p.sq, s.row0 + j, j, d);
-            }
-            if (!ok) y[r] = DARIC_NEG_INF;
-            mx = fmaxf(mx, y[r]);
+        for (int r = 0; r < 2 * M; ++r) {
+          y[r] = x[r >> 1][(r & 1) * 2 + e];
+          bool ok = ((kt.valid >> r) & 1u) && ci < pairs;
+          if (ok && draft) {
+            const int d = key0 + g + 8 * r - s.ctx;
+            ok = d < 0 || sees_draft(p.sq, s.row0 + j, j, d);
           }
-          const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
-          l[e] *= exp2f((m[e] - bs) * cexp);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) l[e] += exp2f((y[r] - bs) * cexp);
-          m[e] = mx;
+          if (!ok) y[r] = DARIC_NEG_INF;
+          mx = fmaxf(mx, y[r]);
         }
-      }
-    }
-    // over the eight threads of a column, then the warps
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m[e], o), ol = __shfl_xor_sync(0xffffffffu, l[e], o);
-        const float mx = fmaxf(m[e], om), bs = mx == DARIC_NEG_INF ? 0.f : mx;
-        l[e] = l[e] * exp2f((m[e] - bs) * cexp) + ol * exp2f((om - bs) * cexp);
-        m[e] = mx;
+        for (int r = 0; r < 2 * M; ++r) l += exp2f((y[r] - bs) * cexp);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (g == 0) s_ml[par][warp][i0 - c0 + 2 * t + e] = make_float2(mx, l);
       }
-    __syncthreads();
-    if (g == 0) {
-      s_ml[warp][2 * t] = make_float2(m[0], l[0]);
-      s_ml[warp][2 * t + 1] = make_float2(m[1], l[1]);
+      if (i0 + 8 < pairs) qt = qn;
     }
-    __syncthreads();
-    if (threadIdx.x < 8 && i0 + (int)threadIdx.x < pairs) {
-      const int ci = i0 + threadIdx.x;
-      float mx = DARIC_NEG_INF;
-      for (int w = 0; w < kSW; ++w) mx = fmaxf(mx, s_ml[w][threadIdx.x].x);
+    __syncthreads();  // the other half of s_ml is free until the meeting after this one
+    const int i = c0 + (int)threadIdx.x;
+    if (threadIdx.x < COLS && i < pairs) {
+      float mx = DARIC_NEG_INF, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSW; ++w) mx = fmaxf(mx, s_ml[par][w][threadIdx.x].x);
       const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
-      float ll = 0.f;
-      for (int w = 0; w < kSW; ++w) ll += s_ml[w][threadIdx.x].y * exp2f((s_ml[w][threadIdx.x].x - bs) * cexp);
-      const int64_t at = (int64_t)(s.row0 + ci / group) * (p.kv.heads * group) + h * group + ci % group;
-      p.part[at * p.splits + split] = make_float2(mx, ll);
+#pragma unroll
+      for (int w = 0; w < kSW; ++w) l += s_ml[par][w][threadIdx.x].y * exp2f((s_ml[par][w][threadIdx.x].x - bs) * cexp);
+      p.part[at(i)] = make_float2(mx, l);
     }
   }
 }
@@ -253,41 +283,122 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ S
 
 // ------------------------------------------------------------ compact --
 constexpr int kMoveThreads = 256;
-constexpr int kMoveTokens = 256;  // tokens whose places a CTA keeps at a time
+constexpr int kMoveTokens = 1024;  // tokens whose places a CTA keeps at a time
+constexpr int kMoveStages = 3;     // batches of loads under way
+constexpr int kMoveVecs = 8;       // vectors of a thread in a batch
+constexpr int kMoveRing = kMoveStages * kMoveVecs * kMoveThreads * 16;
+constexpr int kMoveSmem = kMoveRing + kMoveTokens * 12;
 
-// E: cache element, TE: rotary table element. A thread moves one 16-byte
-// vector of a V row, or of a K row that is not turned; of a turned K row one
-// task: the two vectors that pair up (NeoX), one vector (GPT-J).
-template <class E, class TE>
-__global__ void __launch_bounds__(kMoveThreads) compact_kernel(const __grid_constant__ CompactLaunch p) {
-  constexpr int EPV = E::kPerVec;
-  __shared__ int64_t s_src[kMoveTokens], s_dst[kMoveTokens];
-  __shared__ int2 s_pos[kMoveTokens];
-  const int slice = blockIdx.x % p.slices;
-  const int x = blockIdx.x / p.slices;
-  const int plane = x & 1, h = x >> 1;
+constexpr uint32_t kStays = 0xffffffffu;  // source of a token that is not moved
+
+// Table entries of NF frequencies from d0 on at the old and the new position,
+// and the factors of the turn between them, in fp32.
+template <class TE, int NF>
+struct TurnEntries {
+  float oc[NF], os[NF], nc[NF], ns[NF];
+  __device__ __forceinline__ void load(const uint8_t* table, int64_t row, int half, int from, int to, int d0) {
+    constexpr int TS = (int)sizeof(typename TE::raw);
+    const uint8_t* orow = table + (int64_t)from * row + d0 * TS;
+    const uint8_t* nrow = table + (int64_t)to * row + d0 * TS;
+    dev::load_entries<TE, NF>(orow, oc);
+    dev::load_entries<TE, NF>(orow + half * TS, os);
+    dev::load_entries<TE, NF>(nrow, nc);
+    dev::load_entries<TE, NF>(nrow + half * TS, ns);
+  }
+  __device__ __forceinline__ void factors(float (&C)[NF], float (&S)[NF]) const {
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      C[f] = nc[f] * oc[f] + ns[f] * os[f];
+      S[f] = ns[f] * oc[f] - nc[f] * os[f];
+    }
+  }
+};
+
+template <class E, int NF>
+__device__ __forceinline__ void turn_neox(const float (&C)[NF], const float (&S)[NF], uint4& lo, uint4& hi) {
+  float x[NF], y[NF], o1[NF], o2[NF];
+  dev::unpack<E>(lo, x);
+  dev::unpack<E>(hi, y);
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    o1[f] = x[f] * C[f] - y[f] * S[f];
+    o2[f] = y[f] * C[f] + x[f] * S[f];
+  }
+  lo = dev::pack_vec<E>(o1);
+  hi = dev::pack_vec<E>(o2);
+}
+
+template <class E, int NF>
+__device__ __forceinline__ void turn_gptj(const float (&C)[NF], const float (&S)[NF], uint4& v) {
+  float x[2 * NF];
+  dev::unpack<E>(v, x);
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    const float a = x[2 * f], b = x[2 * f + 1];
+    x[2 * f] = a * C[f] - b * S[f];
+    x[2 * f + 1] = b * C[f] + a * S[f];
+  }
+  v = dev::pack_vec<E>(x);
+}
+
+// One CTA: the tokens of one segment of one layer, in order, for one piece of
+// their rows. blockIdx.x counts the pieces: first (rotate) the turning
+// columns of K as turn_slices column slices x head groups, then the columns
+// that only move: (plane, head, slice). A thread of a turning piece holds one
+// column task (NeoX: the two vectors that pair up) of four heads of a token,
+// so the factors are made once for them; with lists per head it holds four
+// tokens (GPT-J: the same with one vector a task). A moving piece: eight
+// tokens. Loads go to the thread's own slots of a shared-memory ring three
+// batches ahead of the stores.
+template <class E, class TE, bool NEOX, bool BYHEAD>
+__global__ void __launch_bounds__(kMoveThreads, 2) compact_kernel(const __grid_constant__ CompactLaunch p) {
+  constexpr int EPV = E::kPerVec, NF = NEOX ? EPV : EPV / 2, U = kMoveVecs / 2, ST = kMoveStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;  // [stage][vector][thread]
+  uint2* s_at = reinterpret_cast<uint2*>(smem + kMoveRing);    // source and destination, 16-byte units of the layer
+  int* s_from = reinterpret_cast<int*>(smem + kMoveRing + kMoveTokens * 8);
   const CompactSeg sg = p.segs[blockIdx.y];
   const int l = blockIdx.z;
   const CompactLayer L = p.layers[l];
-  const int64_t list = p.shared ? (p.per_head ? h : 0)
-                                : (int64_t)(p.layer0 + l) * (p.per_head ? p.heads : 1) + (p.per_head ? h : 0);
+  int x = blockIdx.x;
+  const bool turn = x < p.turn_pieces;
+  int h, heads = 1, c0, c1;
+  uint8_t* base = L.base;
+  if (turn) {
+    const int slice = x % p.turn_slices;
+    h = x / p.turn_slices * p.turn_heads;
+    heads = BYHEAD ? min(p.turn_heads, p.heads - h) : U;
+    c0 = p.rot_vecs * slice / p.turn_slices;
+    c1 = p.rot_vecs * (slice + 1) / p.turn_slices;
+  } else {
+    x -= p.turn_pieces;
+    const int slice = x % p.slices;
+    x /= p.slices;
+    h = x % p.heads;
+    const bool v_plane = x / p.heads == 0;  // V first; then K, or its columns that do not turn
+    if (v_plane) base += L.v_off;
+    const int first = v_plane ? 0 : p.tail0;
+    c0 = first + (p.vecs - first) * slice / p.slices;
+    c1 = first + (p.vecs - first) * (slice + 1) / p.slices;
+  }
+  const int64_t list = (p.shared ? 0 : (int64_t)(p.layer0 + l) * (p.per_head ? p.heads : 1)) + (p.per_head ? h : 0);
   const int count = min(max(__ldg(&p.count[list * p.count_row + sg.seg]), 0), sg.cap);
   const int32_t* idx = p.idx + list * p.idx_row + sg.out_off;
-  uint8_t* base = L.base + (int64_t)h * L.head_stride + (plane ? L.v_off : 0);
-  const int vecs = p.head_dim / EPV;
-  const bool turn = p.rotate && plane == 0;
-  const int rot_vecs = turn ? (p.neox ? p.half_rot / EPV : 2 * p.half_rot / EPV) : 0;  // turning tasks of a row
-  const int tail0 = turn ? 2 * p.half_rot / EPV : 0;                                   // first vector that only moves
-  const int tasks = rot_vecs + vecs - tail0;
-  const int c0 = tasks * slice / p.slices, c1 = tasks * (slice + 1) / p.slices;
   const int per = c1 - c0;
   if (per <= 0) return;
+  const int rows = kMoveThreads / per;  // tokens the CTA's threads cover at once
+  const int i0 = (int)threadIdx.x / per, c = c0 + (int)threadIdx.x % per;
+  const bool idle = i0 >= rows;         // per does not divide the threads
+  uint8_t* col = base + (int64_t)h * L.head_stride + c * 16;
+  const int pair_off = p.rot_vecs * 16;  // NeoX: to the other half
+  const int batch = turn ? (BYHEAD ? rows : rows * U) : rows * kMoveVecs;  // tokens of a batch
+
   for (int n0 = 0; n0 < count; n0 += kMoveTokens) {
     const int nt = min(kMoveTokens, count - n0);
     __syncthreads();
     for (int i = threadIdx.x; i < nt; i += kMoveThreads) {
       const int from = __ldg(&idx[n0 + i]), to = sg.dst + n0 + i;
-      int64_t so = -1, dof = -1;
+      uint2 pl = make_uint2(kStays, 0);
       // a list that does not ascend, or would move a token up, is not moved in place
       if (from < to || (n0 + i > 0 && __ldg(&idx[n0 + i - 1]) >= from)) {
         atomicOr(p.err, DEV_ERR_INDEX_RANGE);
@@ -296,8 +407,8 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int pos = e ? to : from;
-          const int pg = pos < 0 ? -1 : (int)fdiv((uint32_t)pos, p.page_div);
-          if (pg < 0 || sg.blk_off + pg >= p.table_numel) {
+          const int pg = (int)fdiv((uint32_t)pos, p.page_div);
+          if (sg.blk_off + pg >= p.table_numel) {
             atomicOr(p.err, DEV_ERR_INDEX_RANGE);
             continue;
           }
@@ -308,99 +419,116 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const __grid_cons
           }
           off[e] = (int64_t)blk * L.page_stride + (int64_t)(pos - pg * p.page_size) * L.tok_stride;
         }
-        const bool in = !turn || (from < p.max_pos && to < p.max_pos);
+        const bool in = !p.rotate || (from < p.max_pos && to < p.max_pos);
         if (!in) atomicOr(p.err, DEV_ERR_TABLE_RANGE);
-        if (off[0] >= 0 && off[1] >= 0 && in) {
-          so = off[0];
-          dof = off[1];
-        }
+        if (off[0] >= 0 && off[1] >= 0 && in)  // both planes or neither
+          pl = make_uint2((uint32_t)(off[0] >> 4), (uint32_t)(off[1] >> 4));
       }
-      s_src[i] = so;
-      s_dst[i] = dof;
-      s_pos[i] = make_int2(from, to);
+      s_at[i] = pl;
+      s_from[i] = from;
     }
     __syncthreads();
-    constexpr int U = 4;
-    for (int w0 = 0; w0 < nt * per; w0 += U * kMoveThreads) {
-      uint4 a[U], b[U];
-      int tok[U], c[U];
+    // token of vector u in batch w, and whether this thread moves it
+    auto token = [&](int w, int u) { return w + i0 + (turn && BYHEAD ? 0 : u * rows); };
+    auto moves = [&](int i, uint2& at) {
+      at = make_uint2(kStays, 0);
+      if (i < nt && !idle) at = s_at[i];
+      return at.x != kStays;
+    };
+    auto load = [&](int w, int stage) {
+      uint4* slot = ring + stage * (kMoveVecs * kMoveThreads);
+      if (w < nt) {
+        if (turn) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int w = w0 + u * kMoveThreads + threadIdx.x;
-        tok[u] = -1;
-        if (w < nt * per) {
-          const int i = w / per;
-          c[u] = c0 + w % per;
-          if (s_src[i] >= 0) {
-            tok[u] = i;
-            const uint8_t* src = base + s_src[i];
-            if (c[u] >= rot_vecs) {
-              a[u] = dev::ld_vec(src + (int64_t)(tail0 + c[u] - rot_vecs) * 16);
-            } else {
-              a[u] = dev::ld_vec(src + (int64_t)c[u] * 16);
-              if (p.neox) b[u] = dev::ld_vec(src + (int64_t)(c[u] + rot_vecs) * 16);
-            }
+          for (int u = 0; u < U; ++u) {
+            uint2 at;
+            if (u >= heads || !moves(token(w, u), at)) continue;
+            const uint8_t* src = col + (int64_t)at.x * 16 + (BYHEAD ? u * L.head_stride : 0);
+            cp16(smem_u32(slot + u * kMoveThreads), src, true);
+            if (NEOX) cp16(smem_u32(slot + (u + U) * kMoveThreads), src + pair_off, true);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kMoveVecs; ++u) {
+            uint2 at;
+            if (moves(token(w, u), at)) cp16(smem_u32(slot + u * kMoveThreads), col + (int64_t)at.x * 16, true);
           }
         }
       }
+      cp_commit();
+    };
+    TurnEntries<TE, NF> te;
+    auto entries = [&](int w) {  // of the batch's tokens, ahead of their use
+      uint2 at;
+      const int i = token(w, 0);
+      if (turn && BYHEAD && moves(i, at))
+        te.load(L.table, p.table_row, p.half_rot, s_from[i], sg.dst + n0 + i, c * NF);
+    };
+#pragma unroll
+    for (int k = 0; k < ST - 1; ++k) load(k * batch, k);
+    entries(0);
+    int stage = 0;
+    for (int w = 0; w < nt; w += batch) {
+      load(w + (ST - 1) * batch, stage == 0 ? ST - 1 : stage - 1);
+      cp_wait<ST - 1>();
+      // Every load of this batch is done before its stores; the sources of
+      // the batches under way are behind all its destinations.
+      __syncthreads();
+      const uint4* slot = ring + stage * (kMoveVecs * kMoveThreads);
       if (turn) {
+        float C[NF], S[NF];
+        if (BYHEAD) {
+          te.factors(C, S);
+          entries(w + batch);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (tok[u] < 0 || c[u] >= rot_vecs) continue;
-          const int2 ps = s_pos[tok[u]];
-          constexpr int TS = (int)sizeof(typename TE::raw);
-          const uint8_t* orow = L.table + (int64_t)ps.x * p.table_row;
-          const uint8_t* nrow = L.table + (int64_t)ps.y * p.table_row;
-          const int nf = p.neox ? EPV : EPV / 2;  // frequencies of a task
-          float v[EPV], y[EPV];
-          dev::unpack<E>(a[u], v);
-          if (p.neox) dev::unpack<E>(b[u], y);
-#pragma unroll
-          for (int f = 0; f < EPV; ++f) {
-            if (f >= nf) break;
-            const int d = c[u] * nf + f;
-            const float oc = TE::to_f(*reinterpret_cast<const typename TE::raw*>(orow + d * TS));
-            const float os = TE::to_f(*reinterpret_cast<const typename TE::raw*>(orow + (p.half_rot + d) * TS));
-            const float nc = TE::to_f(*reinterpret_cast<const typename TE::raw*>(nrow + d * TS));
-            const float ns = TE::to_f(*reinterpret_cast<const typename TE::raw*>(nrow + (p.half_rot + d) * TS));
-            const float C = nc * oc + ns * os, S = ns * oc - nc * os;
-            if (p.neox) {
-              const float x1 = v[f], x2 = y[f];
-              v[f] = x1 * C - x2 * S;
-              y[f] = x2 * C + x1 * S;
-            } else if (2 * f + 1 < EPV) {
-              const float x1 = v[2 * f], x2 = v[2 * f + 1];
-              v[2 * f] = x1 * C - x2 * S;
-              v[2 * f + 1] = x2 * C + x1 * S;
-            }
+          uint2 at;
+          const int i = token(w, u);
+          if (u >= heads || !moves(i, at)) continue;
+          if (!BYHEAD) {
+            te.load(L.table, p.table_row, p.half_rot, s_from[i], sg.dst + n0 + i, c * NF);
+            te.factors(C, S);
           }
-          a[u] = dev::pack_vec<E>(v);
-          if (p.neox) b[u] = dev::pack_vec<E>(y);
+          uint4 a = slot[u * kMoveThreads];
+          uint8_t* dst = col + (int64_t)at.y * 16 + (BYHEAD ? u * L.head_stride : 0);
+          if constexpr (NEOX) {
+            uint4 b = slot[(u + U) * kMoveThreads];
+            turn_neox<E, NF>(C, S, a, b);
+            dev::st_vec(dst + pair_off, b);
+          } else {
+            turn_gptj<E, NF>(C, S, a);
+          }
+          dev::st_vec(dst, a);
         }
-      }
-      __syncthreads();  // every load of the batch is done before its stores
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (tok[u] < 0) continue;
-        uint8_t* dst = base + s_dst[tok[u]];
-        if (c[u] >= rot_vecs) {
-          dev::st_vec(dst + (int64_t)(tail0 + c[u] - rot_vecs) * 16, a[u]);
-        } else {
-          dev::st_vec(dst + (int64_t)c[u] * 16, a[u]);
-          if (p.neox) dev::st_vec(dst + (int64_t)(c[u] + rot_vecs) * 16, b[u]);
+        for (int u = 0; u < kMoveVecs; ++u) {
+          uint2 at;
+          if (moves(token(w, u), at)) dev::st_vec(col + (int64_t)at.y * 16, slot[u * kMoveThreads]);
         }
       }
-      // the next batch's loads may start before these stores have landed: its
-      // sources are behind every destination of this batch
+      stage = stage + 1 == ST ? 0 : stage + 1;
     }
+    cp_wait<0>();
   }
+}
+
+template <class T, int D, int M>
+void weights_m(const ScoresLaunch& p, cudaStream_t s) {
+  const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
+  // eight rounds of keys per CTA where that still leaves several CTAs per SM
+  int iters = 8;
+  auto ctas = [&](int n) { return (cap + 16 * M * kSW * n - 1) / (16 * M * kSW * n) * p.sq.num_seqs * p.kv.heads; };
+  while (iters > 1 && ctas(iters) < 8 * (int64_t)p.sm_count) iters /= 2;
+  const unsigned tiles = (unsigned)((cap + 16 * M * kSW * iters - 1) / (16 * M * kSW * iters));
+  weight_kernel<T, D, M><<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kSW * 32, 0, s>>>(p, iters);
+  DARIC_CUDA(cudaGetLastError());
 }
 
 template <class T, int D>
 void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
   ScoresLaunch p = p0;
-  const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
-  const unsigned tiles = (unsigned)((cap + kScoreKeys - 1) / kScoreKeys);
   if (!p.lse) {
     const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
     lse_kernel<T, D><<<dim3((unsigned)p.sq.num_seqs, (unsigned)p.splits, (unsigned)p.kv.heads), kSW * 32, 0, s>>>(p);
@@ -410,17 +538,33 @@ void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
     p.lse = p.lse_work;
     p.lse_row = (int64_t)p.kv.heads * p.sq.group;
   }
-  weight_kernel<T, D><<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kSW * 32, 0, s>>>(p);
+  // few query rows: small tiles, all of them key bytes in flight; many: twice
+  // the keys per pass over the rows
+  const int64_t pairs = (int64_t)(p.sq.num_rows + p.sq.num_seqs - 1) / p.sq.num_seqs * p.sq.group;
+  if (pairs <= 16) weights_m<T, D, 1>(p, s);
+  else weights_m<T, D, 2>(p, s);
+}
+
+template <class E, class TE, bool NEOX, bool BYHEAD>
+void compact_one(const CompactLaunch& p, dim3 grid, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  allow_smem(compact_kernel<E, TE, NEOX, BYHEAD>, kMoveSmem, done);
+  compact_kernel<E, TE, NEOX, BYHEAD><<<grid, kMoveThreads, kMoveSmem, s>>>(p);
   DARIC_CUDA(cudaGetLastError());
+}
+
+template <class E, class TE>
+void compact_et(const CompactLaunch& p, dim3 grid, cudaStream_t s) {
+  if (p.neox) return p.per_head ? compact_one<E, TE, true, false>(p, grid, s) : compact_one<E, TE, true, true>(p, grid, s);
+  p.per_head ? compact_one<E, TE, false, false>(p, grid, s) : compact_one<E, TE, false, true>(p, grid, s);
 }
 
 template <class E>
 void compact_e(const CompactLaunch& p, int tab, dim3 grid, cudaStream_t s) {
   using namespace dev;
-  if (!p.rotate || tab == DARIC_DTYPE_F32) compact_kernel<E, Elem<DARIC_DTYPE_F32>><<<grid, kMoveThreads, 0, s>>>(p);
-  else if (tab == DARIC_DTYPE_BF16) compact_kernel<E, Elem<DARIC_DTYPE_BF16>><<<grid, kMoveThreads, 0, s>>>(p);
-  else compact_kernel<E, Elem<DARIC_DTYPE_F16>><<<grid, kMoveThreads, 0, s>>>(p);
-  DARIC_CUDA(cudaGetLastError());
+  if (tab == DARIC_DTYPE_F32) return compact_et<E, Elem<DARIC_DTYPE_F32>>(p, grid, s);
+  if (tab == DARIC_DTYPE_BF16) return compact_et<E, Elem<DARIC_DTYPE_BF16>>(p, grid, s);
+  compact_et<E, Elem<DARIC_DTYPE_F16>>(p, grid, s);
 }
 
 }  // namespace
@@ -437,8 +581,31 @@ void launch_scores(const ScoresLaunch& p, int dtype, cudaStream_t s) {
   throw Error(DARIC_ERR_INVALID, "attention_scores: bfloat16 or float16 keys of 64, 128 or 256");
 }
 
-void launch_compact(const CompactLaunch& p, int kv_dtype, int tab_dtype, cudaStream_t s) {
-  const dim3 grid((unsigned)(p.heads * 2 * p.slices), (unsigned)p.num_segs, (unsigned)p.num_layers);
+void launch_compact(CompactLaunch& p, int kv_dtype, int tab_dtype, int elem, int sm_count, cudaStream_t s) {
+  // Pieces of the rows: whole heads first, then column slices of 64 bytes or
+  // more (whole sectors) while the launch has few CTAs.
+  const int64_t lists = (int64_t)p.num_segs * p.num_layers, want = 3 * (int64_t)sm_count;
+  const int row = p.head_dim * elem, half = p.half_rot * elem;
+  p.turn_pieces = 0;
+  p.turn_heads = p.per_head ? 1 : 4;
+  p.turn_slices = 1;
+  const bool tail = p.rotate && 2 * p.half_rot < p.head_dim;
+  const int planes = p.rotate ? (tail ? 2 : 1) : 2;
+  p.slices = 1;
+  while (p.slices < 4 && row / (p.slices * 2) >= 64 && lists * planes * p.heads * p.slices < want) p.slices *= 2;
+  if (p.rotate) {
+    auto pieces = [&] { return (p.heads + p.turn_heads - 1) / p.turn_heads * p.turn_slices; };
+    while (p.turn_slices < 4 && half / (p.turn_slices * 2) >= 64 && lists * pieces() < want) p.turn_slices *= 2;
+    while (p.turn_heads > 1 && lists * pieces() < want / 2) p.turn_heads /= 2;
+    p.turn_pieces = pieces();
+  }
+  p.vecs = row / 16;
+  p.rot_vecs = p.rotate ? half / 16 * (p.neox ? 1 : 2) : 0;
+  p.tail0 = p.rotate ? 2 * half / 16 : 0;
+  const dim3 grid((unsigned)(p.turn_pieces + planes * p.heads * p.slices), (unsigned)p.num_segs, (unsigned)p.num_layers);
+  if (!p.rotate) {  // bytes only: one kernel for every dtype
+    return compact_one<dev::Elem<DARIC_DTYPE_BF16>, dev::Elem<DARIC_DTYPE_F32>, true, true>(p, grid, s);
+  }
   switch (kv_dtype) {
     case DARIC_DTYPE_BF16: return compact_e<dev::Elem<DARIC_DTYPE_BF16>>(p, tab_dtype, grid, s);
     case DARIC_DTYPE_F16: return compact_e<dev::Elem<DARIC_DTYPE_F16>>(p, tab_dtype, grid, s);

@@ -67,7 +67,7 @@ def attention_scores(copier: CacheCopier, layer_name: str, q: torch.Tensor, bloc
         ws = None
         if lse is None and rows:
             block = kv.shape[2]
-            splits = min((cols * block + 511) // 512, 64)
+            splits = (cols * block + 255) // 256
             ws = torch.empty(rows * heads * (splits * 2 + 1) + 4, dtype=torch.float32, device=dev)
         check(_lib.load().daric_copier_attention_scores(
             copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
