@@ -154,7 +154,7 @@ struct CompactLaunch {
   int32_t rotate, neox, half_rot;
   int64_t table_row, max_pos;
   // pieces of the rows (launch_compact): turning columns, then those that move
-  int32_t turn_pieces, turn_heads, turn_slices, slices;
+  int32_t turn_pieces, turn_heads, turn_slices, move_heads, slices;
   int32_t vecs, rot_vecs, tail0;  // 16-byte vectors of a row, turning tasks, first K vector that only moves
   CompactSeg segs[kCompactSegs];
   CompactLayer layers[kCompactLayers];

@@ -22,8 +22,8 @@
 // and loads each batch before it stores it moves them in place; the
 // parallelism is over layers, segments, heads, the K and V planes and slices
 // of the row. Keys turn by (new - old): C = nc oc + ns os, S = ns oc - nc os
-// from the table rows of both positions, in fp32 without rounding between,
-// and the turned key is rounded once.
+// from the table rows of both positions, in fp32 (a product and a fused
+// multiply-add each), and the turned key is rounded once to the cache's type.
 // Bound: the bytes of the tokens that move, read and written once.
 #include "attend_common.cuh"
 #include "device_common.cuh"
@@ -282,12 +282,17 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ S
 }
 
 // ------------------------------------------------------------ compact --
-constexpr int kMoveThreads = 256;
-constexpr int kMoveTokens = 1024;  // tokens whose places a CTA keeps at a time
+constexpr int kMoveThreads = 512;
+constexpr int kMoveTokens = 2048;  // tokens whose places a CTA keeps: two chunks
+constexpr int kMoveBatch = 256;    // most tokens of a batch
 constexpr int kMoveStages = 3;     // batches of loads under way
 constexpr int kMoveVecs = 8;       // vectors of a thread in a batch
 constexpr int kMoveRing = kMoveStages * kMoveVecs * kMoveThreads * 16;
 constexpr int kMoveSmem = kMoveRing + kMoveTokens * 12;
+
+// The places of a batch that is being stored (or was, one barrier ago) and of
+// the batches ahead of it fit beside the chunk that is being written.
+static_assert((kMoveStages + 1) * kMoveBatch <= kMoveTokens / 2, "places stay until their batch is stored");
 
 constexpr uint32_t kStays = 0xffffffffu;  // source of a token that is not moved
 
@@ -308,8 +313,8 @@ struct TurnEntries {
   __device__ __forceinline__ void factors(float (&C)[NF], float (&S)[NF]) const {
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-      C[f] = nc[f] * oc[f] + ns[f] * os[f];
-      S[f] = ns[f] * oc[f] - nc[f] * os[f];
+      C[f] = __fmaf_rn(nc[f], oc[f], ns[f] * os[f]);
+      S[f] = __fmaf_rn(ns[f], oc[f], -(nc[f] * os[f]));
     }
   }
 };
@@ -321,8 +326,8 @@ __device__ __forceinline__ void turn_neox(const float (&C)[NF], const float (&S)
   dev::unpack<E>(hi, y);
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
-    o1[f] = x[f] * C[f] - y[f] * S[f];
-    o2[f] = y[f] * C[f] + x[f] * S[f];
+    o1[f] = __fmaf_rn(x[f], C[f], -(y[f] * S[f]));
+    o2[f] = __fmaf_rn(y[f], C[f], x[f] * S[f]);
   }
   lo = dev::pack_vec<E>(o1);
   hi = dev::pack_vec<E>(o2);
@@ -335,8 +340,8 @@ __device__ __forceinline__ void turn_gptj(const float (&C)[NF], const float (&S)
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     const float a = x[2 * f], b = x[2 * f + 1];
-    x[2 * f] = a * C[f] - b * S[f];
-    x[2 * f + 1] = b * C[f] + a * S[f];
+    x[2 * f] = __fmaf_rn(a, C[f], -(b * S[f]));
+    x[2 * f + 1] = __fmaf_rn(b, C[f], a * S[f]);
   }
   v = dev::pack_vec<E>(x);
 }
@@ -351,7 +356,7 @@ __device__ __forceinline__ void turn_gptj(const float (&C)[NF], const float (&S)
 // tokens. Loads go to the thread's own slots of a shared-memory ring three
 // batches ahead of the stores.
 template <class E, class TE, bool NEOX, bool BYHEAD>
-__global__ void __launch_bounds__(kMoveThreads, 2) compact_kernel(const __grid_constant__ CompactLaunch p) {
+__global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_constant__ CompactLaunch p) {
   constexpr int EPV = E::kPerVec, NF = NEOX ? EPV : EPV / 2, U = kMoveVecs / 2, ST = kMoveStages;
   extern __shared__ __align__(128) uint8_t smem[];
   uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;  // [stage][vector][thread]
@@ -372,10 +377,11 @@ __global__ void __launch_bounds__(kMoveThreads, 2) compact_kernel(const __grid_c
     c1 = p.rot_vecs * (slice + 1) / p.turn_slices;
   } else {
     x -= p.turn_pieces;
-    const int slice = x % p.slices;
+    const int slice = x % p.slices, groups = (p.heads + p.move_heads - 1) / p.move_heads;
     x /= p.slices;
-    h = x % p.heads;
-    const bool v_plane = x / p.heads == 0;  // V first; then K, or its columns that do not turn
+    h = x % groups * p.move_heads;
+    heads = min(p.move_heads, p.heads - h);
+    const bool v_plane = x / groups == 0;  // V first; then K, or its columns that do not turn
     if (v_plane) base += L.v_off;
     const int first = v_plane ? 0 : p.tail0;
     c0 = first + (p.vecs - first) * slice / p.slices;
@@ -384,23 +390,25 @@ __global__ void __launch_bounds__(kMoveThreads, 2) compact_kernel(const __grid_c
   const int64_t list = (p.shared ? 0 : (int64_t)(p.layer0 + l) * (p.per_head ? p.heads : 1)) + (p.per_head ? h : 0);
   const int count = min(max(__ldg(&p.count[list * p.count_row + sg.seg]), 0), sg.cap);
   const int32_t* idx = p.idx + list * p.idx_row + sg.out_off;
-  const int per = c1 - c0;
-  if (per <= 0) return;
-  const int rows = kMoveThreads / per;  // tokens the CTA's threads cover at once
-  const int i0 = (int)threadIdx.x / per, c = c0 + (int)threadIdx.x % per;
-  const bool idle = i0 >= rows;         // per does not divide the threads
-  uint8_t* col = base + (int64_t)h * L.head_stride + c * 16;
-  const int pair_off = p.rot_vecs * 16;  // NeoX: to the other half
-  const int batch = turn ? (BYHEAD ? rows : rows * U) : rows * kMoveVecs;  // tokens of a batch
+  if (c1 <= c0) return;
+  const int per = turn ? c1 - c0 : (c1 - c0) * heads;  // threads of a token
+  const int rows = min(kMoveThreads / per, kMoveBatch);  // tokens the CTA's threads cover at once
+  const int i0 = (int)threadIdx.x / per, e0 = (int)threadIdx.x % per;
+  const int c = c0 + e0 % (c1 - c0);
+  const bool idle = i0 >= rows;                          // per does not divide the threads
+  uint8_t* col = base + (int64_t)(h + (turn ? 0 : e0 / (c1 - c0))) * L.head_stride + c * 16;
+  const int pair_off = p.rot_vecs * 16;                  // NeoX: to the other half
+  const int reps = turn && BYHEAD ? 1 : min(turn ? U : kMoveVecs, kMoveBatch / rows);  // tokens of a thread
+  const int batch = rows * reps;                         // tokens of a batch
 
-  for (int n0 = 0; n0 < count; n0 += kMoveTokens) {
-    const int nt = min(kMoveTokens, count - n0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < nt; i += kMoveThreads) {
-      const int from = __ldg(&idx[n0 + i]), to = sg.dst + n0 + i;
+  // Places of the next chunk of tokens, [ready, ready + kMoveTokens / 2).
+  int ready = 0;
+  auto places = [&]() {
+    for (int i = ready + (int)threadIdx.x; i < min(ready + kMoveTokens / 2, count); i += kMoveThreads) {
+      const int from = __ldg(&idx[i]), to = sg.dst + i;
       uint2 pl = make_uint2(kStays, 0);
       // a list that does not ascend, or would move a token up, is not moved in place
-      if (from < to || (n0 + i > 0 && __ldg(&idx[n0 + i - 1]) >= from)) {
+      if (from < to || (i > 0 && __ldg(&idx[i - 1]) >= from)) {
         atomicOr(p.err, DEV_ERR_INDEX_RANGE);
       } else if (from != to) {
         int64_t off[2] = {-1, -1};
@@ -424,94 +432,122 @@ __global__ void __launch_bounds__(kMoveThreads, 2) compact_kernel(const __grid_c
         if (off[0] >= 0 && off[1] >= 0 && in)  // both planes or neither
           pl = make_uint2((uint32_t)(off[0] >> 4), (uint32_t)(off[1] >> 4));
       }
-      s_at[i] = pl;
-      s_from[i] = from;
+      s_at[i % kMoveTokens] = pl;
+      s_from[i % kMoveTokens] = from;
     }
+    ready += kMoveTokens / 2;
     __syncthreads();
-    // token of vector u in batch w, and whether this thread moves it
-    auto token = [&](int w, int u) { return w + i0 + (turn && BYHEAD ? 0 : u * rows); };
-    auto moves = [&](int i, uint2& at) {
-      at = make_uint2(kStays, 0);
-      if (i < nt && !idle) at = s_at[i];
-      return at.x != kStays;
-    };
-    auto load = [&](int w, int stage) {
-      uint4* slot = ring + stage * (kMoveVecs * kMoveThreads);
-      if (w < nt) {
-        if (turn) {
+  };
+  // place of the token of vector u in batch w
+  auto place = [&](int w, int u) {
+    const int i = w + i0 + u * rows;
+    return i < count && u < reps && !idle ? s_at[i % kMoveTokens] : make_uint2(kStays, 0);
+  };
+  auto load = [&](int w, int stage) {
+    uint4* slot = ring + stage * (kMoveVecs * kMoveThreads);
+    if (turn && BYHEAD) {
+      const uint2 at = place(w, 0);
+      if (at.x != kStays) {
+        const uint8_t* src = col + (int64_t)at.x * 16;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            uint2 at;
-            if (u >= heads || !moves(token(w, u), at)) continue;
-            const uint8_t* src = col + (int64_t)at.x * 16 + (BYHEAD ? u * L.head_stride : 0);
+        for (int u = 0; u < U; ++u, src += L.head_stride) {
+          if (u < heads) {
             cp16(smem_u32(slot + u * kMoveThreads), src, true);
             if (NEOX) cp16(smem_u32(slot + (u + U) * kMoveThreads), src + pair_off, true);
           }
-        } else {
-#pragma unroll
-          for (int u = 0; u < kMoveVecs; ++u) {
-            uint2 at;
-            if (moves(token(w, u), at)) cp16(smem_u32(slot + u * kMoveThreads), col + (int64_t)at.x * 16, true);
-          }
         }
       }
-      cp_commit();
-    };
-    TurnEntries<TE, NF> te;
-    auto entries = [&](int w) {  // of the batch's tokens, ahead of their use
-      uint2 at;
-      const int i = token(w, 0);
-      if (turn && BYHEAD && moves(i, at))
-        te.load(L.table, p.table_row, p.half_rot, s_from[i], sg.dst + n0 + i, c * NF);
-    };
+    } else {
+      constexpr int N = kMoveVecs;
+      uint2 at[N];
 #pragma unroll
-    for (int k = 0; k < ST - 1; ++k) load(k * batch, k);
-    entries(0);
-    int stage = 0;
-    for (int w = 0; w < nt; w += batch) {
-      load(w + (ST - 1) * batch, stage == 0 ? ST - 1 : stage - 1);
-      cp_wait<ST - 1>();
-      // Every load of this batch is done before its stores; the sources of
-      // the batches under way are behind all its destinations.
-      __syncthreads();
-      const uint4* slot = ring + stage * (kMoveVecs * kMoveThreads);
-      if (turn) {
-        float C[NF], S[NF];
-        if (BYHEAD) {
-          te.factors(C, S);
-          entries(w + batch);
-        }
+      for (int u = 0; u < N; ++u) at[u] = turn && u >= U ? make_uint2(kStays, 0) : place(w, u);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          uint2 at;
-          const int i = token(w, u);
-          if (u >= heads || !moves(i, at)) continue;
-          if (!BYHEAD) {
-            te.load(L.table, p.table_row, p.half_rot, s_from[i], sg.dst + n0 + i, c * NF);
-            te.factors(C, S);
-          }
-          uint4 a = slot[u * kMoveThreads];
-          uint8_t* dst = col + (int64_t)at.y * 16 + (BYHEAD ? u * L.head_stride : 0);
-          if constexpr (NEOX) {
-            uint4 b = slot[(u + U) * kMoveThreads];
-            turn_neox<E, NF>(C, S, a, b);
-            dev::st_vec(dst + pair_off, b);
-          } else {
-            turn_gptj<E, NF>(C, S, a);
-          }
-          dev::st_vec(dst, a);
+      for (int u = 0; u < N; ++u)
+        if (at[u].x != kStays) {
+          const uint8_t* src = col + (int64_t)at[u].x * 16;
+          cp16(smem_u32(slot + u * kMoveThreads), src, true);
+          if (NEOX && u < U && turn) cp16(smem_u32(slot + (u + U) % N * kMoveThreads), src + pair_off, true);
         }
-      } else {
-#pragma unroll
-        for (int u = 0; u < kMoveVecs; ++u) {
-          uint2 at;
-          if (moves(token(w, u), at)) dev::st_vec(col + (int64_t)at.y * 16, slot[u * kMoveThreads]);
-        }
-      }
-      stage = stage + 1 == ST ? 0 : stage + 1;
     }
-    cp_wait<0>();
+    cp_commit();
+  };
+  TurnEntries<TE, NF> te;
+  auto entries = [&](int w) {  // of the batch's token, ahead of their use
+    const int i = w + i0;
+    if (turn && BYHEAD && place(w, 0).x != kStays)
+      te.load(L.table, p.table_row, p.half_rot, s_from[i % kMoveTokens], sg.dst + i, c * NF);
+  };
+  places();
+#pragma unroll
+  for (int k = 0; k < ST - 1; ++k) load(k * batch, k);
+  entries(0);
+  int stage = 0;
+  for (int w = 0; w < count; w += batch) {
+    if (w + ST * batch > ready && ready < count) places();
+    load(w + (ST - 1) * batch, stage == 0 ? ST - 1 : stage - 1);
+    cp_wait<ST - 1>();
+    // Every load of this batch is done before its stores; the sources of
+    // the batches under way are behind all its destinations.
+    __syncthreads();
+    const uint4* slot = ring + stage * (kMoveVecs * kMoveThreads);
+    if (turn && BYHEAD) {
+      const uint2 at = place(w, 0);
+      float C[NF], S[NF];
+      te.factors(C, S);
+      entries(w + batch);
+      if (at.x != kStays) {
+        uint8_t* dst = col + (int64_t)at.y * 16;
+#pragma unroll
+        for (int u = 0; u < U; ++u, dst += L.head_stride) {
+          if (u < heads) {
+            uint4 a = slot[u * kMoveThreads];
+            if constexpr (NEOX) {
+              uint4 b = slot[(u + U) * kMoveThreads];
+              turn_neox<E, NF>(C, S, a, b);
+              dev::st_vec(dst + pair_off, b);
+            } else {
+              turn_gptj<E, NF>(C, S, a);
+            }
+            dev::st_vec(dst, a);
+          }
+        }
+      }
+    } else if (turn) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint2 at = place(w, u);
+        if (at.x == kStays) continue;
+        const int i = w + i0 + u * rows;
+        float C[NF], S[NF];
+        te.load(L.table, p.table_row, p.half_rot, s_from[i % kMoveTokens], sg.dst + i, c * NF);
+        te.factors(C, S);
+        uint8_t* dst = col + (int64_t)at.y * 16;
+        uint4 a = slot[u * kMoveThreads];
+        if constexpr (NEOX) {
+          uint4 b = slot[(u + U) * kMoveThreads];
+          turn_neox<E, NF>(C, S, a, b);
+          dev::st_vec(dst + pair_off, b);
+        } else {
+          turn_gptj<E, NF>(C, S, a);
+        }
+        dev::st_vec(dst, a);
+      }
+    } else {
+      uint2 at[kMoveVecs];
+      uint4 a[kMoveVecs];
+#pragma unroll
+      for (int u = 0; u < kMoveVecs; ++u) {
+        at[u] = place(w, u);
+        a[u] = slot[u * kMoveThreads];
+      }
+#pragma unroll
+      for (int u = 0; u < kMoveVecs; ++u)
+        if (at[u].x != kStays) dev::st_vec(col + (int64_t)at[u].y * 16, a[u]);
+    }
+    stage = stage + 1 == ST ? 0 : stage + 1;
   }
+  cp_wait<0>();
 }
 
 template <class T, int D, int M>
@@ -582,27 +618,36 @@ void launch_scores(const ScoresLaunch& p, int dtype, cudaStream_t s) {
 }
 
 void launch_compact(CompactLaunch& p, int kv_dtype, int tab_dtype, int elem, int sm_count, cudaStream_t s) {
-  // Pieces of the rows: whole heads first, then column slices of 64 bytes or
-  // more (whole sectors) while the launch has few CTAs.
-  const int64_t lists = (int64_t)p.num_segs * p.num_layers, want = 3 * (int64_t)sm_count;
+  // Pieces of the rows. A CTA (one to an SM) keeps one piece, up to four whole
+  // heads. What counts first is (waves of CTAs) x (size of a piece), then that
+  // pieces are large: the rows of a token's heads lie together, and their
+  // DRAM pages are opened once. Column slices of 64 bytes or more (whole
+  // sectors) are for launches of few lists.
+  const int64_t lists = (int64_t)p.num_segs * p.num_layers;
   const int row = p.head_dim * elem, half = p.half_rot * elem;
-  p.turn_pieces = 0;
-  p.turn_heads = p.per_head ? 1 : 4;
-  p.turn_slices = 1;
   const bool tail = p.rotate && 2 * p.half_rot < p.head_dim;
   const int planes = p.rotate ? (tail ? 2 : 1) : 2;
-  p.slices = 1;
-  while (p.slices < 4 && row / (p.slices * 2) >= 64 && lists * planes * p.heads * p.slices < want) p.slices *= 2;
-  if (p.rotate) {
-    auto pieces = [&] { return (p.heads + p.turn_heads - 1) / p.turn_heads * p.turn_slices; };
-    while (p.turn_slices < 4 && half / (p.turn_slices * 2) >= 64 && lists * pieces() < want) p.turn_slices *= 2;
-    while (p.turn_heads > 1 && lists * pieces() < want / 2) p.turn_heads /= 2;
-    p.turn_pieces = pieces();
-  }
+  double best = 1e30;
+  for (int heads = p.per_head ? 1 : 4; heads >= 1; heads /= 2)
+    for (int slices = 1; slices <= 4; slices *= 2) {
+      if (slices > 1 && row / slices < 64) break;
+      if (row / 16 / slices * heads > kMoveThreads) continue;
+      const int groups = (p.heads + heads - 1) / heads;
+      const int turn = p.rotate ? groups * slices : 0;
+      const int64_t ctas = (turn + (int64_t)planes * groups * slices) * lists;
+      const double cost = (double)((ctas + sm_count - 1) / sm_count) * heads / slices;
+      if (cost < 0.8 * best) {
+        best = cost;
+        p.turn_heads = p.move_heads = heads;
+        p.turn_slices = p.slices = slices;
+        p.turn_pieces = turn;
+      }
+    }
+  const int groups = (p.heads + p.move_heads - 1) / p.move_heads;
   p.vecs = row / 16;
   p.rot_vecs = p.rotate ? half / 16 * (p.neox ? 1 : 2) : 0;
   p.tail0 = p.rotate ? 2 * half / 16 : 0;
-  const dim3 grid((unsigned)(p.turn_pieces + planes * p.heads * p.slices), (unsigned)p.num_segs, (unsigned)p.num_layers);
+  const dim3 grid((unsigned)(p.turn_pieces + planes * groups * p.slices), (unsigned)p.num_segs, (unsigned)p.num_layers);
   if (!p.rotate) {  // bytes only: one kernel for every dtype
     return compact_one<dev::Elem<DARIC_DTYPE_BF16>, dev::Elem<DARIC_DTYPE_F32>, true, true>(p, grid, s);
   }
