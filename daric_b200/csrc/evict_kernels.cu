@@ -1,29 +1,14 @@
-// Eviction from the paged KV cache: the attention weight each cached token
-// received, and the move of the kept tokens to the front of their blocks.
+// Eviction from the paged KV cache: the move of the kept tokens to the front of
+// their blocks.
 //
-// weight_kernel: scores[h, p] (+)= sum over the sequence's query rows j and the
-// group's heads e of  exp(scale q_je . k_p - lse_je)  where j sees p. Keys are
-// the rows of the matrix fragments and query rows their columns, so a key's
-// sum stays in the four threads that hold its row: no atomics, one fixed order
-// of additions. A warp holds 32 keys in registers (16 bytes a thread straight
-// from the cache: both operands take the head dimension in the same permuted
-// order, which leaves the products alone) and passes all query rows by them
-// (16 keys where the rows are few).
-// Bound: the K bytes for a few rows, the matrix and exp2 rates for many.
-//
-// Without an lse, lse_kernel first runs the same products and keeps the
-// maximum and the sum of each query row over the 256 keys of a CTA;
-// lse_join_kernel joins them. K is read twice then (the second time from the
-// L2 cache for prompts up to about 100 MB of keys).
-//
-// compact_kernel: kept token n of a list, position i_n (ascending), moves to
-// position dst + n. Since i_n >= dst + n, a destination is never behind the
-// source of a later token, so one CTA that goes through the tokens in order
-// and loads each batch before it stores it moves them in place; the
-// parallelism is over layers, segments, heads, the K and V planes and slices
-// of the row. Keys turn by (new - old): C = nc oc + ns os, S = ns oc - nc os
-// from the table rows of both positions, in fp32 (a product and a fused
-// multiply-add each), and the turned key is rounded once to the cache's type.
+// Kept token n of a list, position i_n (ascending), moves to position dst + n.
+// Since i_n >= dst + n, a destination is never behind the source of a later
+// token, so one CTA that goes through the tokens in order and loads each batch
+// before it stores it moves them in place; the parallelism is over layers,
+// segments, heads, the K and V planes and slices of the row. Keys turn by
+// (new - old): C = nc oc + ns os, S = ns oc - nc os from the table rows of both
+// positions, in fp32 (a product and a fused multiply-add each), and the turned
+// key is rounded once to the cache's type.
 // Bound: the bytes of the tokens that move, read and written once.
 #include "attend_common.cuh"
 #include "device_common.cuh"
@@ -34,252 +19,6 @@
 namespace daric {
 namespace {
 using namespace att;
-
-constexpr int kSW = 8;  // warps of a score CTA
-
-// Address of the keys of a tile: M * 16 keys of a warp, lane i looks key i up.
-template <int M>
-__device__ __forceinline__ int64_t key_offset(const ScoresLaunch& p, const Seq& s, int b, int h, int key0) {
-  const int pos = key0 + (int)(threadIdx.x & (16 * M - 1));
-  if (pos >= s.len) return -1;
-  const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
-  const int blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
-  if (blk < 0 || blk >= p.kv.num_pages) {
-    atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
-    return -1;
-  }
-  return (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
-         (int64_t)h * p.kv.head_stride;
-}
-
-// M * 16 keys in fragment order: rows g, g + 8 (, g + 16, g + 24).
-template <int D, int M>
-struct KeyTile {
-  static constexpr int KB = D / 32;  // 64-byte pieces of a row
-  uint4 a[2 * M][KB];
-  unsigned valid;                    // bit r: this thread's row g + 8 r exists
-
-  __device__ __forceinline__ void load(const ScoresLaunch& p, int64_t off) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    valid = 0;
-#pragma unroll
-    for (int r = 0; r < 2 * M; ++r) {
-      const int64_t o = __shfl_sync(0xffffffffu, off, g + 8 * r);
-      if (o >= 0) valid |= 1u << r;
-#pragma unroll
-      for (int k = 0; k < KB; ++k)
-        a[r][k] = o >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.kv.base + o) + 4 * k + t) : make_uint4(0, 0, 0, 0);
-    }
-  }
-};
-
-// Eight query rows in fragment order: pair i0 + g of the sequence.
-template <int D>
-struct QueryTile {
-  static constexpr int KB = D / 32;
-  uint4 w[KB];
-  __device__ __forceinline__ void load(const ScoresLaunch& p, const Seq& s, int h, int i0, int pairs) {
-    const int lane = threadIdx.x & 31, i = i0 + (lane >> 2), t = lane & 3;
-    const bool real = i < pairs;
-    const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
-    const uint4* q = reinterpret_cast<const uint4*>(p.q + (int64_t)(s.row0 + j) * p.q_row +
-                                                    (int64_t)(h * p.sq.group + i - j * p.sq.group) * p.q_head) + t;
-#pragma unroll
-    for (int k = 0; k < KB; ++k) w[k] = real ? __ldg(q + 4 * k) : make_uint4(0, 0, 0, 0);
-  }
-};
-
-template <class T, int D, int M>
-__device__ __forceinline__ void key_products(const KeyTile<D, M>& kt, const QueryTile<D>& qt, float (&x)[M][4]) {
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[m][e] = 0.f;
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) {
-    const uint4 w = qt.w[k];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const uint4 u = kt.a[2 * m][k], v = kt.a[2 * m + 1][k];
-      { uint32_t f[4] = {u.x, v.x, u.y, v.y}; Mma<T>::run(x[m], f, w.x, w.y); }
-      { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x[m], f, w.z, w.w); }
-    }
-  }
-}
-
-// A CTA takes `iters` rounds of kSW tiles of M * 16 keys. With M = 1 (few
-// query rows) the next round's keys are on their way while a round is worked
-// on; with M = 2 (many) the next eight query rows are.
-template <class T, int D, int M>
-__global__ void __launch_bounds__(kSW * 32, D > 128 ? 1 : (M == 1 ? 2 : 1)) weight_kernel(const __grid_constant__ ScoresLaunch p, int iters) {
-  constexpr int KEYS = 16 * M;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group;
-  Seq s = load_seq(p.sq, b);
-  clamp_len(p.sq, p.kv.page_size, s);
-  const int64_t col = __ldg(&p.col_off[b]);
-  if (col < 0 || col + s.len > p.scores_cols) {
-    if (threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
-    return;
-  }
-  const int pairs = s.rows * group;
-  int key0 = (int)blockIdx.y * iters * kSW * KEYS + warp * KEYS;
-  if (key0 >= s.len) return;
-  KeyTile<D, M> kt, nx;
-  kt.load(p, key_offset<M>(p, s, b, h, key0));
-  int64_t off = iters > 1 ? key_offset<M>(p, s, b, h, key0 + kSW * KEYS) : -1;
-  QueryTile<D> qt;
-  qt.load(p, s, h, 0, pairs);
-  for (int it = 0; it < iters && key0 < s.len; ++it, key0 += kSW * KEYS) {
-    if (M == 1 && it + 1 < iters) {
-      nx.load(p, off);
-      off = it + 2 < iters ? key_offset<M>(p, s, b, h, key0 + 2 * kSW * KEYS) : -1;
-    }
-    const bool draft = key0 + KEYS > s.ctx;
-    float sum[2 * M];  // keys g, g + 8, ...
-#pragma unroll
-    for (int r = 0; r < 2 * M; ++r) sum[r] = 0.f;
-    for (int i0 = 0; i0 < pairs; i0 += 8) {
-      QueryTile<D> qn;
-      if (M == 2 && pairs > 8) qn.load(p, s, h, i0 + 8 < pairs ? i0 + 8 : 0, pairs);
-      float x[M][4];
-      key_products<T, D, M>(kt, qt, x);
-      if (M == 1 && pairs > 8) qt.load(p, s, h, i0 + 8 < pairs ? i0 + 8 : 0, pairs);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int ci = i0 + 2 * t + e;  // this column's (row, head) pair
-        if (ci >= pairs) continue;
-        const int j = (int)fdiv((uint32_t)ci, p.sq.group_div), row = s.row0 + j;
-        const float z = __ldg(&p.lse[(int64_t)row * p.lse_row + h * group + ci - j * group]);
-        if (z == DARIC_NEG_INF) continue;  // a row that sees nothing
-#pragma unroll
-        for (int r = 0; r < 2 * M; ++r) {
-          const float w = exp2f(__fmaf_rn(x[r >> 1][(r & 1) * 2 + e], p.scale, -z) * kLog2e);
-          bool ok = true;
-          if (draft) {
-            const int d = key0 + g + 8 * r - s.ctx;
-            ok = d < 0 || sees_draft(p.sq, row, j, d);
-          }
-          if (ok) sum[r] += w;
-        }
-      }
-      if (M == 2 && pairs > 8) qt = qn;
-    }
-#pragma unroll
-    for (int r = 0; r < 2 * M; ++r) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-      const int pos = key0 + g + 8 * r;
-      if (t == 0 && pos < s.len) {
-        float* dst = p.scores + (int64_t)h * p.scores_row + col + pos;
-        const float add = (kt.valid >> r) & 1u ? sum[r] : 0.f;
-        *dst = p.accumulate ? *dst + add : add;
-      }
-    }
-    if (M == 1) kt = nx;
-    else if (it + 1 < iters) {
-      kt.load(p, off);
-      off = it + 2 < iters ? key_offset<M>(p, s, b, h, key0 + 2 * kSW * KEYS) : -1;
-    }
-  }
-}
-
-// Maximum and sum of each query row over the kLseKeys keys of a CTA (a split).
-template <class T, int D>
-__global__ void __launch_bounds__(kSW * 32) lse_kernel(const __grid_constant__ ScoresLaunch p) {
-  constexpr int M = 2, KEYS = 16 * M, COLS = 32;  // pairs between two meetings of the warps
-  static_assert(kSW * KEYS == kLseKeys, "one tile per warp");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group, split = blockIdx.y;
-  __shared__ float2 s_ml[2][kSW][COLS];
-  Seq s = load_seq(p.sq, b);
-  clamp_len(p.sq, p.kv.page_size, s);
-  const int pairs = s.rows * group;
-  const float cexp = p.scale * kLog2e;
-  const int heads = p.kv.heads * group;
-  auto at = [&](int i) {  // part of pair i
-    const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
-    return ((int64_t)(s.row0 + j) * heads + h * group + i - j * group) * p.splits + split;
-  };
-  if (split * kLseKeys >= s.len) {  // behind the end: empty parts
-    for (int i = threadIdx.x; i < pairs; i += kSW * 32) p.part[at(i)] = make_float2(DARIC_NEG_INF, 0.f);
-    return;
-  }
-  const int key0 = split * kLseKeys + warp * KEYS;
-  KeyTile<D, M> kt;
-  kt.load(p, key_offset<M>(p, s, b, h, key0));
-  const bool draft = key0 + KEYS > s.ctx;
-  QueryTile<D> qt;
-  qt.load(p, s, h, 0, pairs);
-  for (int c0 = 0, par = 0; c0 < pairs; c0 += COLS, par ^= 1) {
-    for (int i0 = c0; i0 < c0 + COLS && i0 < pairs; i0 += 8) {
-      QueryTile<D> qn;
-      if (i0 + 8 < pairs) qn.load(p, s, h, i0 + 8, pairs);
-      float x[M][4];
-      key_products<T, D, M>(kt, qt, x);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int ci = i0 + 2 * t + e;
-        const int j = (int)fdiv((uint32_t)ci, p.sq.group_div);
-        float y[2 * M], mx = DARIC_NEG_INF, l = 0.f;
-#pragma unroll
-        for (int r = 0; r < 2 * M; ++r) {
-          y[r] = x[r >> 1][(r & 1) * 2 + e];
-          bool ok = ((kt.valid >> r) & 1u) && ci < pairs;
-          if (ok && draft) {
-            const int d = key0 + g + 8 * r - s.ctx;
-            ok = d < 0 || sees_draft(p.sq, s.row0 + j, j, d);
-          }
-          if (!ok) y[r] = DARIC_NEG_INF;
-          mx = fmaxf(mx, y[r]);
-        }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
-#pragma unroll
-        for (int r = 0; r < 2 * M; ++r) l += exp2f((y[r] - bs) * cexp);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (g == 0) s_ml[par][warp][i0 - c0 + 2 * t + e] = make_float2(mx, l);
-      }
-      if (i0 + 8 < pairs) qt = qn;
-    }
-    __syncthreads();  // the other half of s_ml is free until the meeting after this one
-    const int i = c0 + (int)threadIdx.x;
-    if (threadIdx.x < COLS && i < pairs) {
-      float mx = DARIC_NEG_INF, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kSW; ++w) mx = fmaxf(mx, s_ml[par][w][threadIdx.x].x);
-      const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
-#pragma unroll
-      for (int w = 0; w < kSW; ++w) l += s_ml[par][w][threadIdx.x].y * exp2f((s_ml[par][w][threadIdx.x].x - bs) * cexp);
-      p.part[at(i)] = make_float2(mx, l);
-    }
-  }
-}
-
-// lse of each query row and head from its parts (one warp each).
-__global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ ScoresLaunch p, int64_t items) {
-  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (at >= items) return;
-  const float cexp = p.scale * kLog2e;
-  float m = DARIC_NEG_INF, l = 0.f;
-  for (int i = lane; i < p.splits; i += 32) {
-    const float2 v = p.part[at * p.splits + i];
-    const float mx = fmaxf(m, v.x), bs = mx == DARIC_NEG_INF ? 0.f : mx;
-    l = l * exp2f((m - bs) * cexp) + v.y * exp2f((v.x - bs) * cexp);
-    m = mx;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o);
-    const float mx = fmaxf(m, om), bs = mx == DARIC_NEG_INF ? 0.f : mx;
-    l = l * exp2f((m - bs) * cexp) + ol * exp2f((om - bs) * cexp);
-    m = mx;
-  }
-  if (lane == 0) p.lse_work[at] = l == 0.f ? DARIC_NEG_INF : __fmaf_rn(m, p.scale, logf(l));
-}
 
 // ------------------------------------------------------------ compact --
 constexpr int kMoveThreads = 512;
@@ -550,37 +289,6 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
   cp_wait<0>();
 }
 
-template <class T, int D, int M>
-void weights_m(const ScoresLaunch& p, cudaStream_t s) {
-  const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
-  // eight rounds of keys per CTA where that still leaves several CTAs per SM
-  int iters = 8;
-  auto ctas = [&](int n) { return (cap + 16 * M * kSW * n - 1) / (16 * M * kSW * n) * p.sq.num_seqs * p.kv.heads; };
-  while (iters > 1 && ctas(iters) < 8 * (int64_t)p.sm_count) iters /= 2;
-  const unsigned tiles = (unsigned)((cap + 16 * M * kSW * iters - 1) / (16 * M * kSW * iters));
-  weight_kernel<T, D, M><<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kSW * 32, 0, s>>>(p, iters);
-  DARIC_CUDA(cudaGetLastError());
-}
-
-template <class T, int D>
-void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
-  ScoresLaunch p = p0;
-  if (!p.lse) {
-    const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
-    lse_kernel<T, D><<<dim3((unsigned)p.sq.num_seqs, (unsigned)p.splits, (unsigned)p.kv.heads), kSW * 32, 0, s>>>(p);
-    DARIC_CUDA(cudaGetLastError());
-    lse_join_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(p, items);
-    DARIC_CUDA(cudaGetLastError());
-    p.lse = p.lse_work;
-    p.lse_row = (int64_t)p.kv.heads * p.sq.group;
-  }
-  // few query rows: small tiles, all of them key bytes in flight; many: twice
-  // the keys per pass over the rows
-  const int64_t pairs = (int64_t)(p.sq.num_rows + p.sq.num_seqs - 1) / p.sq.num_seqs * p.sq.group;
-  if (pairs <= 16) weights_m<T, D, 1>(p, s);
-  else weights_m<T, D, 2>(p, s);
-}
-
 template <class E, class TE, bool NEOX, bool BYHEAD>
 void compact_one(const CompactLaunch& p, dim3 grid, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
@@ -604,18 +312,6 @@ void compact_e(const CompactLaunch& p, int tab, dim3 grid, cudaStream_t s) {
 }
 
 }  // namespace
-
-void launch_scores(const ScoresLaunch& p, int dtype, cudaStream_t s) {
-  switch (dtype == DARIC_DTYPE_BF16 ? p.kv.head_dim : (dtype == DARIC_DTYPE_F16 ? -p.kv.head_dim : 0)) {
-    case 64: return scores_d<__nv_bfloat16, 64>(p, s);
-    case 128: return scores_d<__nv_bfloat16, 128>(p, s);
-    case 256: return scores_d<__nv_bfloat16, 256>(p, s);
-    case -64: return scores_d<__half, 64>(p, s);
-    case -128: return scores_d<__half, 128>(p, s);
-    case -256: return scores_d<__half, 256>(p, s);
-  }
-  throw Error(DARIC_ERR_INVALID, "attention_scores: bfloat16 or float16 keys of 64, 128 or 256");
-}
 
 void launch_compact(CompactLaunch& p, int kv_dtype, int tab_dtype, int elem, int sm_count, cudaStream_t s) {
   // Pieces of the rows. A CTA (one to an SM) keeps one piece, up to four whole

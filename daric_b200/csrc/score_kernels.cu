@@ -1,0 +1,485 @@
+// Attention weight that each cached token receives, for eviction:
+// scores[h, p] (+)= sum over the sequence's query rows j and the heads e of
+// h's group of  exp(scale q_je . k_p - lse_je)  where j sees p.
+//
+// Keys are the rows of the matrix fragments and query rows their columns, so a
+// key's sum stays in the four threads that hold its row: no atomics, one fixed
+// order of additions. Both operands take the head dimension in the same
+// permuted order (16 bytes of a row per thread and step), which leaves the
+// products alone and lets a thread hold exactly the bytes it loads: nothing is
+// shared between threads, no ldmatrix, no barrier.
+//
+// Few rows (16 (row, head) pairs or fewer): weight_stream_kernel. Bound: the K
+// bytes. Every thread copies its own fragment pieces, and the scores it will
+// add to, into its own slots of a ring of six stages.
+// Many rows: weight_block_kernel. A warp keeps 32 keys in registers and all
+// query rows pass by them from shared memory. Bound: the latency of a warp's
+// chain at prompt sizes, the matrix and exp2 rates for long ones.
+// Without an lse, lse_kernel first runs the same products and keeps the
+// maximum and the sum of each query row over the 256 keys of a CTA, and
+// lse_join_kernel joins them; K is read twice then (the second time from the
+// L2 cache for prompts up to about 100 MB of keys).
+#include "attend_common.cuh"
+
+#include <algorithm>
+
+namespace daric {
+namespace {
+using namespace att;
+
+// Byte offset of a key's row in the layer, -1 where there is none.
+__device__ __forceinline__ int64_t key_offset(const ScoresLaunch& p, const Seq& s, int b, int h, int pos) {
+  if (pos >= s.len) return -1;
+  const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
+  const int blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
+  if (blk < 0 || blk >= p.kv.num_pages) {
+    atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+    return -1;
+  }
+  return (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
+         (int64_t)h * p.kv.head_stride;
+}
+
+// Products of 16 keys (u: row g, v: row g + 8) and 8 query rows (w) over 32
+// elements of the head dimension.
+template <class T>
+__device__ __forceinline__ void products(float (&x)[4], uint4 u, uint4 v, uint4 w) {
+  { uint32_t f[4] = {u.x, v.x, u.y, v.y}; Mma<T>::run(x, f, w.x, w.y); }
+  { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x, f, w.z, w.w); }
+}
+
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// exp(x * scale - z): weights are at most about 1
+__device__ __forceinline__ float weight_of(float x, float scale, float z) {
+  return exp2_fast(__fmaf_rn(x, scale, -z) * kLog2e);
+}
+
+// ------------------------------------------------------------- stream --
+constexpr int kStreamWarps = 4;
+
+template <int D>
+struct StreamGeom {
+  static constexpr int KB = D / 32;                      // 64-byte pieces of a row
+  static constexpr int THREADS = kStreamWarps * 32;
+  static constexpr int STAGE = THREADS * (2 * KB * 16 + 8);  // fragment pieces and two old scores
+  static constexpr int S = D > 128 ? 3 : 6;
+  static constexpr int SMEM = S * STAGE;
+};
+
+// NT: eights of (row, head) pairs. A CTA takes `iters` rounds of 64 keys.
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kStreamWarps * 32, 2) weight_stream_kernel(const __grid_constant__ ScoresLaunch p, int iters) {
+  using G = StreamGeom<D>;
+  constexpr int KB = G::KB, S = G::S, TH = G::THREADS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group;
+  Seq s = load_seq(p.sq, b);
+  clamp_len(p.sq, p.kv.page_size, s);
+  const int64_t col = __ldg(&p.col_off[b]);
+  if (col < 0 || col + s.len > p.scores_cols) {
+    if (threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
+    return;
+  }
+  const int first = (int)blockIdx.y * iters * kStreamWarps * 16 + warp * 16;
+  if (first >= s.len) return;
+  const int n = min(iters, (s.len - first + kStreamWarps * 16 - 1) / (kStreamWarps * 16));
+  const int pairs = s.rows * group;
+  float* out = p.scores + (int64_t)h * p.scores_row + col;
+  uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;                          // [stage][vector][thread]
+  float* old = reinterpret_cast<float*>(smem + S * 2 * KB * TH * 16) + threadIdx.x;  // [stage][2][thread]
+
+  unsigned valid = 0;  // bits 2 * stage + r: the thread's row g + 8 r of the stage exists
+  int64_t nxt[2];      // rows g and g + 8 of the round that is copied next
+  auto lookup = [&](int it) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      nxt[r] = it < n ? key_offset(p, s, b, h, first + it * kStreamWarps * 16 + g + 8 * r) : -1;
+  };
+  auto issue = [&](int it, int st) {
+    if (it < n) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const bool in = nxt[r] >= 0;
+        valid = (valid & ~(1u << (2 * st + r))) | ((unsigned)in << (2 * st + r));
+        const uint8_t* src = p.kv.base + (in ? nxt[r] + t * 16 : 0);
+#pragma unroll
+        for (int k = 0; k < KB; ++k) cp16(smem_u32(ring + (st * 2 * KB + r * KB + k) * TH), in ? src + k * 64 : src, in);
+        const int pos = first + it * kStreamWarps * 16 + g + 8 * r;
+        if (p.accumulate && t == 0 && pos < s.len) cp4(smem_u32(old + (st * 2 + r) * TH), out + pos);
+      }
+    }
+    cp_commit();
+  };
+  lookup(0);
+#pragma unroll
+  for (int k = 0; k < S - 1; ++k) {
+    issue(k, k);
+    lookup(k + 1);
+  }
+  // query rows and their lse: of the first 8 NT pairs for the whole round, of
+  // the others (a sequence of more rows than the mean) in every iteration
+  struct Eight {
+    uint4 w[KB];
+    float z[2];
+    int row[2];
+  };
+  auto eight = [&](int q0, Eight& a) {
+    const int i = q0 + g, j = (int)fdiv((uint32_t)i, p.sq.group_div);
+    const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(s.row0 + j) * p.q_row +
+                                                      (int64_t)(h * group + i - j * group) * p.q_head) + t;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) a.w[k] = i < pairs ? __ldg(src + 4 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int ci = q0 + 2 * t + e, cj = (int)fdiv((uint32_t)ci, p.sq.group_div);
+      a.row[e] = s.row0 + cj;
+      a.z[e] = ci < pairs ? __ldg(&p.lse[(int64_t)a.row[e] * p.lse_row + h * group + ci - cj * group]) : DARIC_NEG_INF;
+    }
+  };
+  Eight qs[NT];
+#pragma unroll
+  for (int q = 0; q < NT; ++q) eight(q * 8, qs[q]);
+  int st = 0;
+  for (int it = 0; it < n; ++it) {
+    issue(it + S - 1, st == 0 ? S - 1 : st - 1);
+    lookup(it + S);
+    cp_wait<S - 1>();
+    const int key0 = first + it * kStreamWarps * 16;
+    const bool draft = key0 + 16 > s.ctx;
+    float sum[2] = {0.f, 0.f};
+    auto add_weights = [&](const float (&x)[4], const Eight& a) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (a.z[e] == DARIC_NEG_INF) continue;  // no such pair, or a row that sees nothing
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float y = weight_of(x[2 * r + e], p.scale, a.z[e]);
+          const int d = key0 + g + 8 * r - s.ctx;
+          if (!draft || d < 0 || sees_draft(p.sq, a.row[e], a.row[e] - s.row0, d)) sum[r] += y;
+        }
+      }
+    };
+    const uint4* u = ring + st * 2 * KB * TH;
+    {
+      float x[NT][4];
+#pragma unroll
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[q][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const uint4 lo = u[k * TH], hi = u[(KB + k) * TH];
+#pragma unroll
+        for (int q = 0; q < NT; ++q) products<T>(x[q], lo, hi, qs[q].w[k]);
+      }
+#pragma unroll
+      for (int q = 0; q < NT; ++q) add_weights(x[q], qs[q]);
+    }
+    for (int q0 = 8 * NT; q0 < pairs; q0 += 8) {
+      Eight a;
+      eight(q0, a);
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KB; ++k) products<T>(x, u[k * TH], u[(KB + k) * TH], a.w[k]);
+      add_weights(x, a);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+      const int pos = key0 + g + 8 * r;
+      if (t == 0 && pos < s.len) {
+        const float add = (valid >> (2 * st + r)) & 1u ? sum[r] : 0.f;
+        out[pos] = p.accumulate ? old[(st * 2 + r) * TH] + add : add;
+      }
+    }
+    st = st + 1 == S ? 0 : st + 1;
+  }
+  cp_wait<0>();
+}
+
+// -------------------------------------------------------------- block --
+constexpr int kBlockWarps = 8;
+constexpr int kBlockRows = 64;  // pairs in shared memory at a time
+
+// 16 M keys of a warp in fragment order: rows g, g + 8 (, g + 16, g + 24).
+template <int D, int M>
+struct KeyTile {
+  static constexpr int KB = D / 32;
+  uint4 a[2 * M][KB];
+  unsigned valid;  // bit r: this thread's row g + 8 r exists
+
+  __device__ __forceinline__ void load(const ScoresLaunch& p, const Seq& s, int b, int h, int key0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    valid = 0;
+#pragma unroll
+    for (int r = 0; r < 2 * M; ++r) {
+      const int64_t o = key_offset(p, s, b, h, key0 + g + 8 * r);
+      if (o >= 0) valid |= 1u << r;
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+        a[r][k] = o >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.kv.base + o) + 4 * k + t) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+// kBlockRows query rows in shared memory; rows 64 bytes longer than they are,
+// so that eight rows of a fragment read fall into different banks.
+template <int D>
+struct QueryBlock {
+  static constexpr int CH = D / 8, PITCH = D * 2 + 64;
+  uint8_t rows[kBlockRows * PITCH];
+  float z[kBlockRows];
+  int row[kBlockRows];
+
+  // pairs [i0, i0 + kBlockRows) of the sequence; the CTA's threads meet around it
+  __device__ __forceinline__ void load(const ScoresLaunch& p, const Seq& s, int h, int i0, int pairs) {
+    const int group = p.sq.group;
+    __syncthreads();
+    for (int v = threadIdx.x; v < kBlockRows * CH; v += kBlockWarps * 32) {
+      const int i = v / CH, c = v % CH, pi = i0 + i, j = (int)fdiv((uint32_t)pi, p.sq.group_div);
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (pi < pairs)
+        w = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)(s.row0 + j) * p.q_row +
+                                                 (int64_t)(h * group + pi - j * group) * p.q_head) + c);
+      *reinterpret_cast<uint4*>(rows + i * PITCH + c * 16) = w;
+    }
+    if (threadIdx.x < kBlockRows) {
+      const int pi = i0 + threadIdx.x, j = (int)fdiv((uint32_t)pi, p.sq.group_div);
+      row[threadIdx.x] = s.row0 + j;
+      z[threadIdx.x] = pi < pairs && p.lse ? __ldg(&p.lse[(int64_t)(s.row0 + j) * p.lse_row + h * group + pi - j * group])
+                                           : DARIC_NEG_INF;
+    }
+    __syncthreads();
+  }
+};
+
+// Products of a key tile with the eight query rows from `i` of the block on.
+template <class T, int D, int M>
+__device__ __forceinline__ void block_products(const KeyTile<D, M>& kt, const QueryBlock<D>& qb, int i, float (&x)[M][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[m][e] = 0.f;
+  const uint8_t* q = qb.rows + (i + g) * QueryBlock<D>::PITCH + t * 16;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) {
+    const uint4 w = *reinterpret_cast<const uint4*>(q + k * 64);
+#pragma unroll
+    for (int m = 0; m < M; ++m) products<T>(x[m], kt.a[2 * m][k], kt.a[2 * m + 1][k], w);
+  }
+}
+
+template <class T, int D, int M>
+__global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) weight_block_kernel(const __grid_constant__ ScoresLaunch p) {
+  constexpr int KEYS = 16 * M;
+  __shared__ __align__(16) QueryBlock<D> qb;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int b = blockIdx.x, h = blockIdx.z;
+  Seq s = load_seq(p.sq, b);
+  clamp_len(p.sq, p.kv.page_size, s);
+  const int64_t col = __ldg(&p.col_off[b]);
+  if (col < 0 || col + s.len > p.scores_cols) {
+    if (threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
+    return;
+  }
+  const int pairs = s.rows * p.sq.group;
+  const int key0 = ((int)blockIdx.y * kBlockWarps + warp) * KEYS;
+  if ((int)blockIdx.y * kBlockWarps * KEYS >= s.len) return;
+  KeyTile<D, M> kt;
+  kt.load(p, s, b, h, key0);
+  const bool draft = key0 + KEYS > s.ctx;
+  float sum[2 * M];  // keys g, g + 8, ...
+#pragma unroll
+  for (int r = 0; r < 2 * M; ++r) sum[r] = 0.f;
+  for (int i0 = 0; i0 < pairs; i0 += kBlockRows) {
+    qb.load(p, s, h, i0, pairs);
+    const int n = min(kBlockRows, pairs - i0);
+#pragma unroll 2
+    for (int i = 0; i < n; i += 8) {
+      float x[M][4];
+      block_products<T, D, M>(kt, qb, i, x);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float z = qb.z[i + 2 * t + e];
+        const int row = qb.row[i + 2 * t + e];
+#pragma unroll
+        for (int r = 0; r < 2 * M; ++r) {
+          const float a = weight_of(x[r >> 1][(r & 1) * 2 + e], p.scale, z);
+          const int d = key0 + g + 8 * r - s.ctx;
+          // z = -inf: no such pair, or a row that sees nothing
+          if (z != DARIC_NEG_INF && (!draft || d < 0 || sees_draft(p.sq, row, row - s.row0, d))) sum[r] += a;
+        }
+      }
+    }
+  }
+  float* out = p.scores + (int64_t)h * p.scores_row + col;
+#pragma unroll
+  for (int r = 0; r < 2 * M; ++r) {
+    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    const int pos = key0 + g + 8 * r;
+    if (t == 0 && pos < s.len) {
+      const float add = (kt.valid >> r) & 1u ? sum[r] : 0.f;
+      out[pos] = p.accumulate ? out[pos] + add : add;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- lse --
+// Maximum and sum of each query row over the kLseKeys keys of a CTA (a split).
+template <class T, int D>
+__global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) lse_kernel(const __grid_constant__ ScoresLaunch p) {
+  constexpr int M = 2, KEYS = 16 * M;
+  static_assert(kBlockWarps * KEYS == kLseKeys, "one tile per warp");
+  __shared__ __align__(16) QueryBlock<D> qb;
+  __shared__ float2 s_ml[kBlockWarps][kBlockRows / 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group, split = blockIdx.y;
+  Seq s = load_seq(p.sq, b);
+  clamp_len(p.sq, p.kv.page_size, s);
+  const int pairs = s.rows * group;
+  const float cexp = p.scale * kLog2e;
+  auto at = [&](int i) {  // part of pair i
+    const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
+    return ((int64_t)(s.row0 + j) * (p.kv.heads * group) + h * group + i - j * group) * p.splits + split;
+  };
+  if (split * kLseKeys >= s.len) {  // behind the end: empty parts
+    for (int i = threadIdx.x; i < pairs; i += kBlockWarps * 32) p.part[at(i)] = make_float2(DARIC_NEG_INF, 0.f);
+    return;
+  }
+  const int key0 = split * kLseKeys + warp * KEYS;
+  KeyTile<D, M> kt;
+  kt.load(p, s, b, h, key0);
+  const bool draft = key0 + KEYS > s.ctx;
+  for (int i0 = 0; i0 < pairs; i0 += kBlockRows) {
+    qb.load(p, s, h, i0, pairs);
+    // the warps meet twice a block, over half of its rows each
+    for (int c0 = 0; c0 < kBlockRows && i0 + c0 < pairs; c0 += kBlockRows / 2) {
+      if (c0) __syncthreads();
+#pragma unroll 2
+      for (int i = c0; i < c0 + kBlockRows / 2 && i0 + i < pairs; i += 8) {
+        float x[M][4];
+        block_products<T, D, M>(kt, qb, i, x);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = qb.row[i + 2 * t + e];
+          float y[2 * M], mx = DARIC_NEG_INF, l = 0.f;
+#pragma unroll
+          for (int r = 0; r < 2 * M; ++r) {
+            y[r] = x[r >> 1][(r & 1) * 2 + e];
+            bool ok = (kt.valid >> r) & 1u;
+            if (ok && draft) {
+              const int d = key0 + g + 8 * r - s.ctx;
+              ok = d < 0 || (i0 + i + 2 * t + e < pairs && sees_draft(p.sq, row, row - s.row0, d));
+            }
+            if (!ok) y[r] = DARIC_NEG_INF;
+            mx = fmaxf(mx, y[r]);
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
+#pragma unroll
+          for (int r = 0; r < 2 * M; ++r) l += exp2_fast((y[r] - bs) * cexp);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          if (g == 0) s_ml[warp][i - c0 + 2 * t + e] = make_float2(mx, l);
+        }
+      }
+      __syncthreads();
+      const int i = i0 + c0 + (int)threadIdx.x;
+      if (threadIdx.x < kBlockRows / 2 && i < pairs) {
+        float mx = DARIC_NEG_INF, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kBlockWarps; ++w) mx = fmaxf(mx, s_ml[w][threadIdx.x].x);
+        const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
+#pragma unroll
+        for (int w = 0; w < kBlockWarps; ++w) l += s_ml[w][threadIdx.x].y * exp2_fast((s_ml[w][threadIdx.x].x - bs) * cexp);
+        p.part[at(i)] = make_float2(mx, l);
+      }
+    }
+  }
+}
+
+// lse of each query row and head from its parts (one warp each).
+__global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ ScoresLaunch p, int64_t items) {
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (at >= items) return;
+  const float cexp = p.scale * kLog2e;
+  float m = DARIC_NEG_INF, l = 0.f;
+  for (int i = lane; i < p.splits; i += 32) {
+    const float2 v = p.part[at * p.splits + i];
+    const float mx = fmaxf(m, v.x), bs = mx == DARIC_NEG_INF ? 0.f : mx;
+    l = l * exp2_fast((m - bs) * cexp) + v.y * exp2_fast((v.x - bs) * cexp);
+    m = mx;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o);
+    const float mx = fmaxf(m, om), bs = mx == DARIC_NEG_INF ? 0.f : mx;
+    l = l * exp2_fast((m - bs) * cexp) + ol * exp2_fast((om - bs) * cexp);
+    m = mx;
+  }
+  if (lane == 0) p.lse_work[at] = l == 0.f ? DARIC_NEG_INF : __fmaf_rn(m, p.scale, logf(l));
+}
+
+template <class T, int D, int NT>
+void stream_n(const ScoresLaunch& p, cudaStream_t s) {
+  const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
+  // long rounds (the ring fills once) that still leave the SMs several CTAs
+  int iters = 64;
+  auto ctas = [&](int n) { return (cap + 16 * kStreamWarps * n - 1) / (16 * kStreamWarps * n) * p.sq.num_seqs * p.kv.heads; };
+  while (iters > 1 && ctas(iters) < 6 * (int64_t)p.sm_count) iters /= 2;
+  const unsigned tiles = (unsigned)((cap + 16 * kStreamWarps * iters - 1) / (16 * kStreamWarps * iters));
+  static std::atomic<uint64_t> done{0};
+  allow_smem(weight_stream_kernel<T, D, NT>, StreamGeom<D>::SMEM, done);
+  weight_stream_kernel<T, D, NT>
+      <<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kStreamWarps * 32, StreamGeom<D>::SMEM, s>>>(p, iters);
+  DARIC_CUDA(cudaGetLastError());
+}
+
+template <class T, int D>
+void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
+  ScoresLaunch p = p0;
+  const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
+  if (!p.lse) {
+    const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
+    lse_kernel<T, D><<<dim3((unsigned)p.sq.num_seqs, (unsigned)p.splits, (unsigned)p.kv.heads), kBlockWarps * 32, 0, s>>>(p);
+    DARIC_CUDA(cudaGetLastError());
+    lse_join_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(p, items);
+    DARIC_CUDA(cudaGetLastError());
+    p.lse = p.lse_work;
+    p.lse_row = (int64_t)p.kv.heads * p.sq.group;
+  }
+  // by the mean rows of a sequence (the real ones are on the device); a
+  // sequence of more rows is right in either form
+  const int64_t pairs = (int64_t)(p.sq.num_rows + p.sq.num_seqs - 1) / p.sq.num_seqs * p.sq.group;
+  if (pairs <= 8) return stream_n<T, D, 1>(p, s);
+  if (pairs <= 16) return stream_n<T, D, 2>(p, s);
+  constexpr int M = D > 128 ? 1 : 2;
+  const unsigned tiles = (unsigned)((cap + kBlockWarps * 16 * M - 1) / (kBlockWarps * 16 * M));
+  weight_block_kernel<T, D, M><<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kBlockWarps * 32, 0, s>>>(p);
+  DARIC_CUDA(cudaGetLastError());
+}
+
+}  // namespace
+
+void launch_scores(const ScoresLaunch& p, int dtype, cudaStream_t s) {
+  switch (dtype == DARIC_DTYPE_BF16 ? p.kv.head_dim : (dtype == DARIC_DTYPE_F16 ? -p.kv.head_dim : 0)) {
+    case 64: return scores_d<__nv_bfloat16, 64>(p, s);
+    case 128: return scores_d<__nv_bfloat16, 128>(p, s);
+    case 256: return scores_d<__nv_bfloat16, 256>(p, s);
+    case -64: return scores_d<__half, 64>(p, s);
+    case -128: return scores_d<__half, 128>(p, s);
+    case -256: return scores_d<__half, 256>(p, s);
+  }
+  throw Error(DARIC_ERR_INVALID, "attention_scores: bfloat16 or float16 keys of 64, 128 or 256");
+}
+
+}  // namespace daric
