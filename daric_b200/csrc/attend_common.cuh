@@ -35,6 +35,12 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
   const int n = ok ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+// The same with constant offsets from both addresses.
+template <int DST, int SRC>
+__device__ __forceinline__ void cp16_at(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(DST), "n"(SRC)
+               : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {

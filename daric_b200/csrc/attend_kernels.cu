@@ -236,13 +236,17 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) attend_kernel(const
       if (one) {
         const int rows = ok ? nxt_n : 0;
         if (lane == 0) s_valid[kg][stage][rg] = (uint32_t)((1ull << rows) - 1);
-        const uint8_t* src = p.kv.base + off + r0 * p.kv.tok_stride + c16;
+        // rows past the valid ones are in the page all the same: nothing of
+        // them is read, and zeros are written
+        const uint8_t* k = p.kv.base + off + r0 * p.kv.tok_stride + c16;
+        const int64_t step = RPI * p.kv.tok_stride;
+        int left = rows - r0;
 #pragma unroll
         for (int i = 0; i < G::KPW / RPI; ++i) {
-          const bool in = r0 + i * RPI < rows;
-          const uint8_t* k = in ? src + i * RPI * p.kv.tok_stride : p.kv.base;
-          cp16(d0 + i * RPI * G::PITCH, k, in);
-          cp16(d0 + (G::KT + i * RPI) * G::PITCH, in ? k + p.kv.v_off : k, in);
+          cp16(d0 + i * RPI * G::PITCH, k, left > 0);
+          cp16(d0 + (G::KT + i * RPI) * G::PITCH, k + p.kv.v_off, left > 0);
+          k += step;
+          left -= RPI;
         }
       } else {
         const unsigned valid = __ballot_sync(0xffffffffu, ok);

@@ -9,9 +9,12 @@
 // products alone and lets a thread hold exactly the bytes it loads: nothing is
 // shared between threads, no ldmatrix, no barrier.
 //
+// The heads of a token lie together in the cache, so the CTAs of its heads are
+// neighbours in the grid and open its DRAM pages once.
+//
 // Few rows (16 (row, head) pairs or fewer): weight_stream_kernel. Bound: the K
 // bytes. Every thread copies its own fragment pieces, and the scores it will
-// add to, into its own slots of a ring of six stages.
+// add to, into its own slots of a ring of three stages.
 // Many rows: weight_block_kernel. A warp keeps 32 keys in registers and all
 // query rows pass by them from shared memory. Bound: the latency of a warp's
 // chain at prompt sizes, the matrix and exp2 rates for long ones.
@@ -48,6 +51,15 @@ __device__ __forceinline__ void products(float (&x)[4], uint4 u, uint4 v, uint4 
   { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x, f, w.z, w.w); }
 }
 
+// N pieces of 16 bytes, 64 bytes apart in the row, to slots STEP bytes apart.
+template <int N, int STEP, int I>
+__device__ __forceinline__ void copy_pieces(uint32_t dst, const uint8_t* src, int n) {
+  if constexpr (I < N) {
+    cp16_at<I * STEP, I * 64>(dst, src, n);
+    copy_pieces<N, STEP, I + 1>(dst, src, n);
+  }
+}
+
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -65,18 +77,18 @@ struct StreamGeom {
   static constexpr int KB = D / 32;                      // 64-byte pieces of a row
   static constexpr int THREADS = kStreamWarps * 32;
   static constexpr int STAGE = THREADS * (2 * KB * 16 + 8);  // fragment pieces and two old scores
-  static constexpr int S = D > 128 ? 3 : 6;
+  static constexpr int S = 3;
   static constexpr int SMEM = S * STAGE;
 };
 
 // NT: eights of (row, head) pairs. A CTA takes `iters` rounds of 64 keys.
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(kStreamWarps * 32, 2) weight_stream_kernel(const __grid_constant__ ScoresLaunch p, int iters) {
+__global__ void __launch_bounds__(kStreamWarps * 32, D > 128 ? 2 : 4) weight_stream_kernel(const __grid_constant__ ScoresLaunch p, int iters) {
   using G = StreamGeom<D>;
   constexpr int KB = G::KB, S = G::S, TH = G::THREADS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group;
+  const int b = blockIdx.z, h = blockIdx.x, group = p.sq.group;
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int64_t col = __ldg(&p.col_off[b]);
@@ -92,24 +104,57 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2) weight_stream_kernel(con
   uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;                          // [stage][vector][thread]
   float* old = reinterpret_cast<float*>(smem + S * 2 * KB * TH * 16) + threadIdx.x;  // [stage][2][thread]
 
+  // A round's 16 keys lie in one page when 16 divides the page size: one
+  // lookup serves the warp and a thread's rows are at fixed distances. Else
+  // every thread looks its two rows up.
+  const bool one = p.kv.page_size % 16 == 0;
   unsigned valid = 0;  // bits 2 * stage + r: the thread's row g + 8 r of the stage exists
+  const uint8_t* const keys = p.kv.base + (int64_t)h * p.kv.head_stride + t * 16;
+  const int64_t row0 = g * p.kv.tok_stride, row1 = (g + 8) * p.kv.tok_stride;
   int64_t nxt[2];      // rows g and g + 8 of the round that is copied next
+  int blk = -1;        // one: its block and first token
+  int tok = 0;
   auto lookup = [&](int it) {
+    const int key0 = first + it * kStreamWarps * 16;
+    if (one) {
+      blk = -1;
+      if (it < n) {
+        const int pg = (int)fdiv((uint32_t)key0, p.kv.page_div);
+        tok = key0 - pg * p.kv.page_size;
+        blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
+      }
+    } else {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-      nxt[r] = it < n ? key_offset(p, s, b, h, first + it * kStreamWarps * 16 + g + 8 * r) : -1;
+      for (int r = 0; r < 2; ++r) nxt[r] = it < n ? key_offset(p, s, b, 0, key0 + g + 8 * r) : -1;
+    }
   };
   auto issue = [&](int it, int st) {
     if (it < n) {
+      const int pos = first + it * kStreamWarps * 16 + g;
+      bool in[2];
+      const uint8_t* src[2];
+      if (one) {
+        const bool ok = (unsigned)blk < (unsigned)p.kv.num_pages;
+        if (!ok) atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+        const uint8_t* page = keys + (ok ? blk : 0) * p.kv.page_stride + tok * p.kv.tok_stride;
+        src[0] = page + row0;
+        src[1] = page + row1;
+        in[0] = ok && pos < s.len;
+        in[1] = ok && pos + 8 < s.len;
+      } else {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const bool in = nxt[r] >= 0;
-        valid = (valid & ~(1u << (2 * st + r))) | ((unsigned)in << (2 * st + r));
-        const uint8_t* src = p.kv.base + (in ? nxt[r] + t * 16 : 0);
-#pragma unroll
-        for (int k = 0; k < KB; ++k) cp16(smem_u32(ring + (st * 2 * KB + r * KB + k) * TH), in ? src + k * 64 : src, in);
-        const int pos = first + it * kStreamWarps * 16 + g + 8 * r;
-        if (p.accumulate && t == 0 && pos < s.len) cp4(smem_u32(old + (st * 2 + r) * TH), out + pos);
+        for (int r = 0; r < 2; ++r) {
+          in[r] = nxt[r] >= 0;
+          src[r] = keys + (in[r] ? nxt[r] : 0);
+        }
+      }
+      valid = (valid & ~(3u << (2 * st))) | ((unsigned)in[0] << (2 * st)) | ((unsigned)in[1] << (2 * st + 1));
+      const uint32_t dst = smem_u32(ring + st * 2 * KB * TH);
+      copy_pieces<KB, TH * 16, 0>(dst, src[0], in[0] ? 16 : 0);
+      copy_pieces<KB, TH * 16, 0>(dst + KB * TH * 16, src[1], in[1] ? 16 : 0);
+      if (p.accumulate && t == 0) {
+        if (pos < s.len) cp4(smem_u32(old + (st * 2) * TH), out + pos);
+        if (pos + 8 < s.len) cp4(smem_u32(old + (st * 2 + 1) * TH), out + pos + 8);
       }
     }
     cp_commit();
@@ -280,7 +325,7 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) weight_bloc
   constexpr int KEYS = 16 * M;
   __shared__ __align__(16) QueryBlock<D> qb;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.x, h = blockIdx.z;
+  const int b = blockIdx.z, h = blockIdx.x;
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int64_t col = __ldg(&p.col_off[b]);
@@ -340,7 +385,7 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) lse_kernel(
   __shared__ __align__(16) QueryBlock<D> qb;
   __shared__ float2 s_ml[kBlockWarps][kBlockRows / 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.x, h = blockIdx.z, group = p.sq.group, split = blockIdx.y;
+  const int b = blockIdx.z, h = blockIdx.x, group = p.sq.group, split = blockIdx.y;
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int pairs = s.rows * group;
@@ -440,7 +485,7 @@ void stream_n(const ScoresLaunch& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   allow_smem(weight_stream_kernel<T, D, NT>, StreamGeom<D>::SMEM, done);
   weight_stream_kernel<T, D, NT>
-      <<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kStreamWarps * 32, StreamGeom<D>::SMEM, s>>>(p, iters);
+      <<<dim3((unsigned)p.kv.heads, tiles, (unsigned)p.sq.num_seqs), kStreamWarps * 32, StreamGeom<D>::SMEM, s>>>(p, iters);
   DARIC_CUDA(cudaGetLastError());
 }
 
@@ -450,7 +495,7 @@ void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
   const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
   if (!p.lse) {
     const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
-    lse_kernel<T, D><<<dim3((unsigned)p.sq.num_seqs, (unsigned)p.splits, (unsigned)p.kv.heads), kBlockWarps * 32, 0, s>>>(p);
+    lse_kernel<T, D><<<dim3((unsigned)p.kv.heads, (unsigned)p.splits, (unsigned)p.sq.num_seqs), kBlockWarps * 32, 0, s>>>(p);
     DARIC_CUDA(cudaGetLastError());
     lse_join_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(p, items);
     DARIC_CUDA(cudaGetLastError());
@@ -464,7 +509,7 @@ void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
   if (pairs <= 16) return stream_n<T, D, 2>(p, s);
   constexpr int M = D > 128 ? 1 : 2;
   const unsigned tiles = (unsigned)((cap + kBlockWarps * 16 * M - 1) / (kBlockWarps * 16 * M));
-  weight_block_kernel<T, D, M><<<dim3((unsigned)p.sq.num_seqs, tiles, (unsigned)p.kv.heads), kBlockWarps * 32, 0, s>>>(p);
+  weight_block_kernel<T, D, M><<<dim3((unsigned)p.kv.heads, tiles, (unsigned)p.sq.num_seqs), kBlockWarps * 32, 0, s>>>(p);
   DARIC_CUDA(cudaGetLastError());
 }
 
