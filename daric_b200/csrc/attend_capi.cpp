@@ -90,10 +90,6 @@ void check_scale(float scale) {
   DARIC_CHECK(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
 }
 
-// Resident CTAs per SM of the attention: two rings of 104 KB, or one of 203 KB
-// with 256-wide heads.
-int attend_ctas(int64_t head_dim) { return head_dim > 128 ? 1 : 2; }
-
 // Row-tile variant: the query heads of one KV head times the rows of a
 // sequence (their mean: the lengths are on the device) in 16s.
 int attend_variant(const SeqBatch& b, bool sparse) {
@@ -102,6 +98,10 @@ int attend_variant(const SeqBatch& b, bool sparse) {
   if (rows <= 32 || sparse) return 2;
   return 4;
 }
+
+// Resident CTAs per SM: rings of 70 KB (one row group), 104 KB or less (more
+// of them), or one of up to 203 KB with 256-wide heads.
+int attend_ctas(int64_t head_dim, int rg) { return head_dim > 128 ? 1 : (rg == 1 ? 3 : 2); }
 
 size_t attend_bytes(int grid, int rows, int head_dim) {
   return (size_t)grid * (2 * (size_t)rows * head_dim * 4 + 2 * (size_t)rows * 8 + 16);
@@ -125,7 +125,10 @@ int daric_attend_workspace(int device, int64_t head_dim, int64_t* out_bytes) {
   return guard([&] {
     DARIC_CHECK(out_bytes, "out_bytes is NULL");
     DARIC_CHECK(head_dim > 0 && head_dim <= 256, "head dimension must be at most 256");
-    *out_bytes = (int64_t)attend_bytes(device_info(device).sm_count * attend_ctas(head_dim), attend_rows(4), (int)head_dim);
+    const int sms = device_info(device).sm_count;
+    size_t most = 0;
+    for (int rg : {1, 2, 4}) most = std::max(most, attend_bytes(sms * attend_ctas(head_dim, rg), attend_rows(rg), (int)head_dim));
+    *out_bytes = (int64_t)most;
   });
 }
 
@@ -168,7 +171,7 @@ int daric_copier_tree_attention(daric_copier* copier, const char* layer_name, in
                          ((double)table_cols * L.kv.page_size / 16.0 + 1.0);
     DARIC_CHECK(tiles < 4.0e9, "tree_attention: the batch has too many tiles for one call");
     DARIC_CHECK((int64_t)num_rows * p.sq.group / rows < (1 << 18), "tree_attention: too many query rows");
-    const int grid = di.sm_count * attend_ctas(head_dim);
+    const int grid = di.sm_count * attend_ctas(head_dim, rg);
     attend_workspace(p, grid, rows, workspace, workspace_bytes);
     OnDevice on(device);
     launch_attend(p, kv_dtype, rg, grid, (cudaStream_t)stream);
@@ -214,7 +217,7 @@ int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, 
     const double tiles = (double)L.kv.heads * (double)num_rows * ((double)p.sq.group / rows + 1.0) *
                          ((double)k * L.kv.page_size / 16.0 + 1.0);
     DARIC_CHECK(tiles < 4.0e9, "sparse_attention: the batch has too many tiles for one call");
-    const int grid = di.sm_count * attend_ctas(head_dim);
+    const int grid = di.sm_count * attend_ctas(head_dim, rg);
     attend_workspace(p, grid, rows, workspace, workspace_bytes);
     OnDevice on(device);
     launch_attend(p, kv_dtype, rg, grid, (cudaStream_t)stream);

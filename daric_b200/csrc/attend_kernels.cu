@@ -41,7 +41,9 @@ struct Geom {
   static constexpr int TILE = KT * KG;                                  // keys of a tile
   static constexpr int PITCH = D * 2 + 16;
   static constexpr int STAGE = 2 * KT * PITCH;
-  static constexpr int S = D > 128 && RG == 4 ? 4 : 3;                  // stages of a ring
+  // stages of a ring: where four warps can be three CTAs on an SM, more warps
+  // count for more than more stages (64 ragged decodes: 98 us against 105)
+  static constexpr int S = RG == 1 && D <= 128 ? 2 : (D > 128 && RG == 4 ? 4 : 3);
   static constexpr int ROWS = 16 * RG;
   static constexpr int RING = KG * S * STAGE;
   static constexpr int QB = ROWS * PITCH;
@@ -65,7 +67,7 @@ __device__ __forceinline__ int tiles_of(const AttendLaunch& p, const Seq& s) {
 }
 
 template <class T, int D, int RG, bool SPARSE>
-__global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) attend_kernel(const __grid_constant__ AttendLaunch p) {
+__global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) attend_kernel(const __grid_constant__ AttendLaunch p) {
   using G = Geom<D, RG>;
   constexpr int CH = D / 8;  // 16-byte vectors of a row
   extern __shared__ __align__(128) uint8_t smem[];
