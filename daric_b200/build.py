@@ -22,7 +22,7 @@ BUILD = ROOT / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["capi.cpp", "page_kernels.cu", "bulk_kernels.cu", "inplace_kernels.cu", "select_kernels.cu",
-           "attend_capi.cpp", "attend_kernels.cu", "blocks_kernels.cu", "score_kernels.cu",
+           "attend_capi.cpp", "attend_kernels.cu", "wide_kernels.cu", "blocks_kernels.cu", "score_kernels.cu",
            "evict_kernels.cu"]
 
 

@@ -77,6 +77,8 @@ struct AttendLaunch {
 constexpr int attend_rows(int rg) { return 16 * rg; }
 
 void launch_attend(const AttendLaunch& p, int dtype, int rg, int grid, cudaStream_t s);
+// Many rows: tiles of 128 * mt pairs, head_dim 64 or 128 (wide_kernels.cu).
+void launch_wide(const AttendLaunch& p, int dtype, int mt, int grid, cudaStream_t s);
 
 // Smallest and largest key value of each dimension over the tokens of a page,
 // per KV head: bounds[block][head][0 = min, 1 = max][dim], contiguous.

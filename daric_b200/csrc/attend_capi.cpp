@@ -90,18 +90,29 @@ void check_scale(float scale) {
   DARIC_CHECK(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
 }
 
-// Row-tile variant: the query heads of one KV head times the rows of a
-// sequence (their mean: the lengths are on the device) in 16s.
-int attend_variant(const SeqBatch& b, bool sparse) {
-  const int64_t rows = sparse ? b.group : (int64_t)((b.num_rows + b.num_seqs - 1) / b.num_seqs) * b.group;
-  if (rows <= 16) return 1;
-  if (rows <= 32 || sparse) return 2;
-  return 4;
-}
+// How the query heads of one KV head times the rows of a sequence (their
+// mean: the lengths are on the device) are tiled: up to 16 and 32 pairs as row
+// groups of 16 (attend_kernels.cu, memory-bound there); from 33 on as 128 or
+// 256 rows on the tensor cores (wide_kernels.cu). 256-wide heads do not fit
+// those and take four row groups.
+struct Variant {
+  int rg;    // row groups of 16, or 0
+  int mt;    // tiles of 128 rows, or 0
+  int rows;  // of a CTA
+  int ctas;  // resident per SM: rings of 70 KB with one row group, 104 KB or less with more, else all of it
+};
+Variant variant_rg(int rg, int64_t dim) { return {rg, 0, attend_rows(rg), dim > 128 ? 1 : (rg == 1 ? 3 : 2)}; }
+Variant variant_mt(int mt) { return {0, mt, 128 * mt, 1}; }
 
-// Resident CTAs per SM: rings of 70 KB (one row group), 104 KB or less (more
-// of them), or one of up to 203 KB with 256-wide heads.
-int attend_ctas(int64_t head_dim, int rg) { return head_dim > 128 ? 1 : (rg == 1 ? 3 : 2); }
+Variant attend_variant(const SeqBatch& b, const KvView& kv, bool sparse) {
+  const int64_t rows = sparse ? b.group : (int64_t)((b.num_rows + b.num_seqs - 1) / b.num_seqs) * b.group;
+  if (rows <= 16) return variant_rg(1, kv.head_dim);
+  if (rows <= 32 || sparse) return variant_rg(2, kv.head_dim);
+  // the wide form keeps offsets in 32 bits of 16 bytes
+  if (kv.head_dim > 128 || (double)kv.num_pages * (double)kv.page_stride >= 60.0 * (1ll << 30))
+    return variant_rg(4, kv.head_dim);
+  return variant_mt(rows <= 128 ? 1 : 2);
+}
 
 size_t attend_bytes(int grid, int rows, int head_dim) {
   return (size_t)grid * (2 * (size_t)rows * head_dim * 4 + 2 * (size_t)rows * 8 + 16);
@@ -127,7 +138,8 @@ int daric_attend_workspace(int device, int64_t head_dim, int64_t* out_bytes) {
     DARIC_CHECK(head_dim > 0 && head_dim <= 256, "head dimension must be at most 256");
     const int sms = device_info(device).sm_count;
     size_t most = 0;
-    for (int rg : {1, 2, 4}) most = std::max(most, attend_bytes(sms * attend_ctas(head_dim, rg), attend_rows(rg), (int)head_dim));
+    for (const Variant& v : {variant_rg(1, head_dim), variant_rg(2, head_dim), variant_rg(4, head_dim), variant_mt(2)})
+      if (v.mt == 0 || head_dim <= 128) most = std::max(most, attend_bytes(sms * v.ctas, v.rows, (int)head_dim));
     *out_bytes = (int64_t)most;
   });
 }
@@ -166,15 +178,17 @@ int daric_copier_tree_attention(daric_copier* copier, const char* layer_name, in
     p.lse_row = lse_row;
     p.scale = scale;
     // tiles of the whole batch are counted in 32 bits
-    const int rg = attend_variant(p.sq, false), rows = attend_rows(rg);
+    const Variant var = attend_variant(p.sq, L.kv, false);
+    const int rows = var.rows;
     const double tiles = (double)L.kv.heads * ((double)num_rows * p.sq.group / rows + (double)num_seqs) *
                          ((double)table_cols * L.kv.page_size / 16.0 + 1.0);
     DARIC_CHECK(tiles < 4.0e9, "tree_attention: the batch has too many tiles for one call");
     DARIC_CHECK((int64_t)num_rows * p.sq.group / rows < (1 << 18), "tree_attention: too many query rows");
-    const int grid = di.sm_count * attend_ctas(head_dim, rg);
+    const int grid = di.sm_count * var.ctas;
     attend_workspace(p, grid, rows, workspace, workspace_bytes);
     OnDevice on(device);
-    launch_attend(p, kv_dtype, rg, grid, (cudaStream_t)stream);
+    if (var.mt) launch_wide(p, kv_dtype, var.mt, grid, (cudaStream_t)stream);
+    else launch_attend(p, kv_dtype, var.rg, grid, (cudaStream_t)stream);
   });
 }
 
@@ -213,14 +227,15 @@ int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, 
     p.pages_head = pages_head;
     p.k = (int32_t)k;
     p.scale = scale;
-    const int rg = attend_variant(p.sq, true), rows = attend_rows(rg);
+    const Variant var = attend_variant(p.sq, L.kv, true);
+    const int rows = var.rows;
     const double tiles = (double)L.kv.heads * (double)num_rows * ((double)p.sq.group / rows + 1.0) *
                          ((double)k * L.kv.page_size / 16.0 + 1.0);
     DARIC_CHECK(tiles < 4.0e9, "sparse_attention: the batch has too many tiles for one call");
-    const int grid = di.sm_count * attend_ctas(head_dim, rg);
+    const int grid = di.sm_count * var.ctas;
     attend_workspace(p, grid, rows, workspace, workspace_bytes);
     OnDevice on(device);
-    launch_attend(p, kv_dtype, rg, grid, (cudaStream_t)stream);
+    launch_attend(p, kv_dtype, var.rg, grid, (cudaStream_t)stream);
   });
 }
 

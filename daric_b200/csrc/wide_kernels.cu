@@ -1,0 +1,695 @@
+// Attention of many query rows over the paged KV cache on the tensor cores.
+//
+// The mathematics and the split of the work are those of attend_kernels.cu;
+// here a CTA holds MT = 1 or 2 tiles of 128 (query row, query head) pairs of
+// one KV head and passes tiles of 128 keys by them:
+//   S = Q K^T   tcgen05.mma, Q and K from shared memory, S in tensor memory
+//   P = 2^((S - m) c) by one thread per row, rounded to the cache's type and
+//       written over S in tensor memory (relative 2^-9 bf16, 2^-12 fp16 per
+//       weight; l sums the unrounded values)
+//   O += P V    tcgen05.mma, P from tensor memory, V from shared memory in the
+//       layout it was copied in (its rows are the summed dimension)
+// m is the maximum when it was last moved: it moves, and O and l are rescaled,
+// only when the running maximum is over 2^8 times ahead, so that O is rarely
+// read back. m, l, S and O are fp32.
+//
+// Warps: 4 MT of softmax, one thread each for a row; one that issues the
+// matrix instructions; four that copy. A copy slot is a K or a V tile (16-byte
+// cp.async, a page table lookup per key, into the 128-byte swizzle); each
+// copying thread reports a slot when its own copies of it have landed, two
+// slots behind the newest. With MT = 2 the two tiles take turns, so one is
+// multiplied while the other is exponentiated; with MT = 1 the key tiles do,
+// through two S areas.
+//
+// Bound: the K and V bytes up to about 256 pairs; above, exp2 (16 a clock and
+// SM) and the matrix rate together. Why tcgen05 and not the warp matrix
+// instructions here: from 33 pairs on those need more time per key than its
+// bytes do.
+#include "attend_common.cuh"
+#include "tensor_common.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace daric {
+namespace {
+using namespace att;
+using bulk::fence_proxy_async;
+using bulk::mbar_arrive;
+using bulk::mbar_init;
+using bulk::mbar_init_fence;
+using bulk::mbar_try_wait;
+using bulk::mbar_wait;
+
+constexpr int kKeys = 128;      // keys of a tile
+constexpr int kMaskRing = 8;    // tiles whose key masks are kept
+constexpr int kCopyThreads = 128;
+
+template <int D, int MT>
+struct Wide {
+  static constexpr int ROWS = 128 * MT;
+  static constexpr int SLOT = kKeys * D * 2;
+  static constexpr int QB = ROWS * D * 2;
+  static constexpr int NS = D == 64 ? 10 : (MT == 2 ? 5 : 6);
+  static constexpr int THREADS = 128 * MT + 32 + kCopyThreads;
+  static constexpr int MMA_WARP = 4 * MT;
+  static constexpr int COPY_WARP = 4 * MT + 1;
+  static constexpr int TILES = QB + NS * SLOT;
+};
+
+struct WideShared {
+  uint64_t full[10], empty[10];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_empty[2];
+  uint64_t q_full, q_empty;
+  uint32_t vmask[kMaskRing][4];
+  uint32_t off[2][kKeys];  // row offsets of two key tiles, 16-byte units of the layer
+  uint32_t tmem;
+  int abort;               // a wait gave up: everyone leaves
+  int poison[4];           // by count modulo 4: the segment if its drafted V rows hold infinities or NaN
+};
+template <int D, int MT>
+constexpr int wide_smem() {
+  return Wide<D, MT>::TILES + 1024 + (int)sizeof(WideShared);
+}
+
+// The part of a segment that a CTA works on.
+struct Part {
+  int b, h, rt, tile0, n, ntiles;
+  Seq s;
+  int row_base, my_rows;  // first pair of the row tile, and pairs that exist
+};
+
+template <class T, int D, int MT>
+__global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __grid_constant__ AttendLaunch p) {
+  using W = Wide<D, MT>;
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int HB = D / 64;          // 64-element halves of a row
+  constexpr int HALF = kKeys * 128;   // bytes of such a half of a tile
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  WideShared& sh = *reinterpret_cast<WideShared*>(base + W::TILES);
+  uint8_t* q_tile = base;
+  uint8_t* slots = base + W::QB;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = p.sq.group;
+
+  // ---- the line of tiles and this CTA's part of it (as in attend_kernels.cu)
+  uint32_t* sums = reinterpret_cast<uint32_t*>(slots);  // before any copy
+  const int per = (p.sq.num_seqs + W::THREADS - 1) / W::THREADS;
+  auto tiles_of = [&](const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); };
+  auto tiles_seq = [&](const Seq& s) {
+    return ((uint32_t)(s.rows * group) + W::ROWS - 1) / W::ROWS * (uint32_t)p.kv.heads * (uint32_t)tiles_of(s);
+  };
+  {
+    uint32_t mine = 0;
+    for (int i = tid * per; i < min((tid + 1) * per, p.sq.num_seqs); ++i) {
+      Seq s = load_seq(p.sq, i);
+      clamp_len(p.sq, p.kv.page_size, s);
+      mine += tiles_seq(s);
+    }
+    sums[tid] = mine;
+    __syncthreads();
+    for (int o = 1; o < W::THREADS; o <<= 1) {
+      const uint32_t v = tid >= o ? sums[tid - o] : 0;
+      __syncthreads();
+      sums[tid] += v;
+      __syncthreads();
+    }
+  }
+  const uint32_t total = sums[W::THREADS - 1];
+  uint32_t t0, t1;
+  split_range(total, gridDim.x, blockIdx.x, t0, t1);
+  int b = 0;
+  uint32_t seg_at = 0;
+  if (t0 < t1) {
+    int lo = 0, hi = W::THREADS - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] > t0) hi = mid; else lo = mid + 1;
+    }
+    b = lo * per;
+    seg_at = lo ? sums[lo - 1] : 0;
+  }
+  if (tid == 0) {
+    p.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    for (int i = 0; i < W::NS; ++i) {
+      mbar_init(&sh.full[i], kCopyThreads);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.pv_done[i], 1);
+      mbar_init(&sh.o_empty[i], 128);
+    }
+    mbar_init(&sh.q_full, kCopyThreads);
+    mbar_init(&sh.q_empty, 1);
+    mbar_init_fence();
+    sh.abort = 0;
+    for (int i = 0; i < 4; ++i) sh.poison[i] = -1;
+  }
+  __syncthreads();  // sums are read, barriers are ready
+  if (t0 >= t1) return;
+  if (warp == W::MMA_WARP) tc::alloc512(&sh.tmem);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  volatile int* abort = &sh.abort;
+  // A wait that is out of time ends the kernel: its error bit is set and every role leaves its loop.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (mbar_wait(bar, parity)) return true;
+    *abort = 1;
+    atomicOr(p.sq.err, DEV_ERR_TIMEOUT);
+    return false;
+  };
+  // Part of the line at tile t; false: none (lengths changed while the kernel ran).
+  auto part_at = [&](uint32_t t, Part& g) {
+    for (;; ++b) {
+      if (b >= p.sq.num_seqs) return false;
+      g.s = load_seq(p.sq, b);
+      clamp_len(p.sq, p.kv.page_size, g.s);
+      const uint32_t n = tiles_seq(g.s);
+      if (t < seg_at + n) break;
+      seg_at += n;
+    }
+    uint32_t x = t - seg_at;
+    g.ntiles = tiles_of(g.s);
+    g.tile0 = (int)(x % (uint32_t)g.ntiles);
+    x /= (uint32_t)g.ntiles;
+    const int rts = (g.s.rows * group + W::ROWS - 1) / W::ROWS;
+    g.rt = (int)(x % (uint32_t)rts);
+    g.h = (int)(x / (uint32_t)rts);
+    g.b = b;
+    g.n = (int)min((uint32_t)(g.ntiles - g.tile0), t1 - t);
+    g.row_base = g.rt * W::ROWS;
+    g.my_rows = min(W::ROWS, g.s.rows * group - g.row_base);
+    return true;
+  };
+  // First position of the drafted part that some row of the tile does not
+  // see: tiles that end at or before it need no mask but that of their keys.
+  auto all_see = [&](const Part& g) {
+    if (p.sq.mask) return g.s.ctx;
+    return g.s.ctx + (int)fdiv((uint32_t)g.row_base, p.sq.group_div) + 1;
+  };
+  // order in which the slots of a part are filled: MT = 2: K0 V0 K1 V1 ...;
+  // MT = 1: K0 K1 V0 K2 V1 ... (the next scores are under way while a tile is
+  // exponentiated)
+  auto k_slot = [&](int i) { return MT == 2 ? 2 * i : (i == 0 ? 0 : 2 * i - 1); };
+  auto v_slot = [&](int i, int n) { return MT == 2 ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
+
+  if (warp >= W::COPY_WARP) {
+    // ------------------------------------------------------------ copies --
+    const int ct = tid - W::COPY_WARP * 32;
+    uint32_t n_slot = 0, n_seg = 0, n_tile = 0;  // slots, segments, key tiles so far
+    uint64_t* pend[2] = {nullptr, nullptr};      // groups not reported yet, older first
+    auto report = [&](uint64_t* bar) {
+      if (!bar) return;
+      fence_proxy_async();
+      mbar_arrive(bar);
+    };
+    auto flush = [&]() {
+      cp_wait<0>();
+      report(pend[0]);
+      report(pend[1]);
+      pend[0] = pend[1] = nullptr;
+    };
+    auto push = [&](uint64_t* bar) {  // a group was issued: reports the one two before it
+      cp_commit();
+      cp_wait<2>();
+      report(pend[0]);
+      pend[0] = pend[1];
+      pend[1] = bar;
+    };
+    auto take = [&](uint64_t* bar, uint32_t parity) {  // what is reported late must not be waited for
+      if (mbar_try_wait(bar, parity)) return true;
+      flush();
+      return wait(bar, parity);
+    };
+    // The copying threads go on or stop together: what each found, for all.
+    auto together = [&](bool mine) {
+      uint32_t all;
+      __syncwarp();
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
+          : "=r"(all)
+          : "r"((uint32_t)mine), "n"(kCopyThreads)
+          : "memory");
+      return all != 0;
+    };
+    uint32_t t = t0;
+    bool ok = true;
+    while (ok && t < t1) {
+      Part g;
+      if (!together(part_at(t, g))) break;
+      const int32_t* trow = p.sq.table + (int64_t)g.b * p.sq.table_ld;
+      const uint8_t* kv = p.kv.base + (int64_t)g.h * p.kv.head_stride;
+      const int see = all_see(g);
+      // query rows
+      if (n_seg) ok = together(take(&sh.q_empty, (n_seg - 1) & 1));
+      if (!ok) break;
+      {
+        constexpr int CH = D / 8;
+        for (int v = ct; v < W::ROWS * CH; v += kCopyThreads) {
+          const int r = v / CH, c = v % CH, i = g.row_base + r;
+          const bool in = r < g.my_rows;
+          const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
+          const uint8_t* src = in ? p.q + (int64_t)(g.s.row0 + j) * p.q_row +
+                                        (int64_t)(g.h * group + i - j * group) * p.q_head + c * 16
+                                  : p.q;
+          const uint32_t dst = smem_u32(q_tile) + (r >> 7) * (HB * HALF) + (c >> 3) * HALF + (r & 127) * 128 +
+                               (((c & 7) ^ (r & 7)) << 4);
+          cp16(dst, src, in);
+        }
+        push(&sh.q_full);
+      }
+      auto lookup = [&](int i) {  // block of this thread's key of tile i, -1: none
+        const int pos = (g.tile0 + i) * kKeys + ct;
+        if (i >= g.n || pos >= g.s.len) return -1;
+        return __ldg(&trow[fdiv((uint32_t)pos, p.kv.page_div)]);
+      };
+      int blk = lookup(0);
+      auto place = [&](int i) {  // offsets and mask of tile i; looks the next one up
+        const int pos = (g.tile0 + i) * kKeys + ct;
+        bool in = pos < g.s.len;
+        if (in && (blk < 0 || blk >= p.kv.num_pages)) {
+          atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+          in = false;
+        }
+        int64_t off = 0;
+        if (in) {
+          const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
+          off = (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride;
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, in);
+        // the copies that read these offsets before are issued
+        asm volatile("bar.sync 1, %0;" ::"n"(kCopyThreads) : "memory");
+        if (lane == 0) sh.vmask[(n_tile + i) % kMaskRing][ct >> 5] = m;
+        sh.off[i & 1][ct] = in ? (uint32_t)(off >> 4) : 0xffffffffu;
+        blk = lookup(i + 1);
+        __syncwarp();
+        asm volatile("bar.sync 1, %0;" ::"n"(kCopyThreads) : "memory");
+      };
+      auto copy = [&](int i, bool v_tile) {
+        const uint32_t st = n_slot % W::NS, use = n_slot / W::NS;
+        if (!ok) return;
+        if (use) ok = together(take(&sh.empty[st], (use - 1) & 1));
+        if (!ok) return;
+        constexpr int CH = D / 8, RPI = kCopyThreads / CH;  // rows at a time
+        const int c = ct % CH;
+        const uint8_t* src = kv + (v_tile ? p.kv.v_off : 0) + c * 16;
+        const uint32_t dst = smem_u32(slots) + st * W::SLOT + (c >> 3) * HALF;
+#pragma unroll 8
+        for (int r = ct / CH; r < kKeys; r += RPI) {
+          const uint32_t o = sh.off[i & 1][r];
+          const bool in = o != 0xffffffffu;
+          cp16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? (int64_t)o * 16 : 0), in);
+        }
+        if (v_tile && (g.tile0 + i + 1) * kKeys > see) {
+          // drafted V rows that some rows must not see: values without a
+          // finite size would reach them through 0 * inf. They are taken out
+          // here and added where they are seen, at the end of the segment.
+          cp_commit();
+          cp_wait<0>();
+          uint8_t* tile = slots + st * W::SLOT + (c >> 3) * HALF;
+          bool bad = false;
+          for (int r = ct / CH; r < kKeys; r += RPI) {
+            uint4* w = reinterpret_cast<uint4*>(tile + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            uint4 x = *w;
+            uint16_t* u = reinterpret_cast<uint16_t*>(&x);
+            bool here = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if ((u[e] & Mma<T>::kExpMask) == Mma<T>::kExpMask) {
+                u[e] = 0;
+                here = true;
+              }
+            if (here) *w = x;
+            bad = bad || here;
+          }
+          if (bad) *(volatile int*)&sh.poison[n_seg & 3] = (int)n_seg;
+        }
+        push(&sh.full[st]);
+        ++n_slot;
+      };
+      if (MT == 2) {
+        for (int i = 0; ok && i < g.n; ++i) {
+          place(i);
+          copy(i, false);
+          copy(i, true);
+        }
+      } else {
+        place(0);
+        copy(0, false);
+        for (int i = 1; ok && i < g.n; ++i) {
+          place(i);
+          copy(i, false);
+          copy(i - 1, true);
+        }
+        copy(g.n - 1, true);
+      }
+      n_tile += (uint32_t)g.n;
+      ++n_seg;
+      t += (uint32_t)g.n;
+    }
+    flush();
+    cp_wait<0>();
+  } else if (warp == W::MMA_WARP) {
+    // ---------------------------------------------------------- products --
+    if (lane == 0) {
+      constexpr uint32_t id_qk = tc::instr_desc(BF, false, 128, kKeys), id_pv = tc::instr_desc(BF, true, 128, D);
+      uint32_t n_slot = 0, n_seg = 0, n_item = 0;
+      uint32_t t = t0;
+      bool ok = true;
+      while (ok && t < t1) {
+        Part g;
+        if (!part_at(t, g)) break;
+        ok = wait(&sh.q_full, n_seg & 1);
+        if (!ok) break;
+        const int items = MT * g.n;
+        auto slot_of = [&](int s) { return (n_slot + (uint32_t)s) % W::NS; };
+        auto full = [&](int s) { return wait(&sh.full[slot_of(s)], ((n_slot + (uint32_t)s) / W::NS) & 1); };
+        auto scores = [&](int j) {  // S of item j
+          const int i = MT == 2 ? j >> 1 : j, tile = MT == 2 ? j & 1 : 0;
+          const int ks = k_slot(i);
+          if (!full(ks)) return false;
+          tc::fence_after();
+          const uint32_t s = (n_item + (uint32_t)j) & 1;
+          const uint32_t qa = smem_u32(q_tile) + tile * (HB * HALF), ka = smem_u32(slots) + slot_of(ks) * W::SLOT;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t o = (k >> 2) * HALF + (k & 3) * 32;
+            tc::mma_ss(tmem + s * kKeys, tc::smem_desc(qa + o, 16), tc::smem_desc(ka + o, 16), id_qk, k > 0);
+          }
+          tc::commit(&sh.s_full[s]);
+          if (MT == 1 || tile == 1) tc::commit(&sh.empty[slot_of(ks)]);
+          if (j == items - 1) tc::commit(&sh.q_empty);
+          return true;
+        };
+        ok = scores(0) && (items < 2 || scores(1));
+        for (int j = 0; ok && j < items; ++j) {
+          const int i = MT == 2 ? j >> 1 : j, tile = MT == 2 ? j & 1 : 0;
+          const uint32_t c = n_item + (uint32_t)j, s = c & 1;
+          if (j < MT && n_seg) ok = wait(&sh.o_empty[tile], (n_seg - 1) & 1);
+          const int vs = v_slot(i, g.n);
+          ok = ok && wait(&sh.p_full[s], (c >> 1) & 1) && full(vs);
+          if (!ok) break;
+          tc::fence_after();
+          const uint32_t va = smem_u32(slots) + slot_of(vs) * W::SLOT;
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            tc::mma_ts(tmem + 2 * kKeys + tile * D, tmem + s * kKeys + k * 8, tc::smem_desc(va + k * 2048, HALF), id_pv,
+                       i > 0 || k > 0);
+          tc::commit(&sh.pv_done[s]);
+          if (MT == 1 || tile == 1) tc::commit(&sh.empty[slot_of(vs)]);
+          if (j + 2 < items) ok = scores(j + 2);
+        }
+        n_slot += 2 * (uint32_t)g.n;
+        n_item += (uint32_t)items;
+        ++n_seg;
+        t += (uint32_t)g.n;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- softmax --
+    const int tile = warp >> 2;                            // row tile of the CTA
+    const int r = (warp & 3) * 32 + lane;                  // row of it
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_col = tmem + lanes + 2 * kKeys + tile * D;
+    const float cexp = p.scale * kLog2e;
+    uint32_t n_item = 0, n_seg = 0, n_tile = 0;            // items of this tile so far
+    uint32_t t = t0;
+    bool ok = true;
+    while (ok && t < t1) {
+      Part g;
+      if (!part_at(t, g)) break;
+      const int i_pair = tile * 128 + r;
+      const bool real = i_pair < g.my_rows;
+      const int pi = g.row_base + i_pair;
+      const int j = real ? (int)fdiv((uint32_t)pi, p.sq.group_div) : 0;  // row of the sequence
+      const int row = g.s.row0 + j, head = g.h * group + pi - j * group;
+      const int see = all_see(g);
+      float m = DARIC_NEG_INF, l0 = 0.f, l1 = 0.f;
+      for (int i = 0; i < g.n; ++i) {
+        const uint32_t c = n_item + (uint32_t)i;
+        // MT = 2: the tile's own S area; MT = 1: the two in turn
+        const uint32_t s = MT == 2 ? (uint32_t)tile : c & 1, ph = MT == 2 ? c & 1 : (c >> 1) & 1;
+        ok = wait(&sh.s_full[s], ph);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc::fence_after();
+        const uint32_t s_col = tmem + lanes + s * kKeys;
+        const int key0 = (g.tile0 + i) * kKeys;
+        const uint32_t* vm = sh.vmask[(n_tile + (uint32_t)i) % kMaskRing];
+        uint32_t vis[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) vis[w] = vm[w];
+        bool masked = (vis[0] & vis[1] & vis[2] & vis[3]) != 0xffffffffu;
+        if (key0 + kKeys > see) {
+          masked = true;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int d0 = key0 + 32 * w - g.s.ctx;  // drafted token of bit 0
+            uint32_t bits;
+            if (d0 <= -32) {
+              bits = 0xffffffffu;
+            } else if (!real) {
+              bits = 0;
+            } else if (!p.sq.mask) {
+              const int up = j - d0 + 1;  // bits [0, up)
+              bits = up <= 0 ? 0u : (up >= 32 ? 0xffffffffu : (1u << up) - 1u);
+            } else {
+              const int at = max(d0, 0), word = at >> 6, sft = at & 63;
+              const uint64_t* mr = p.sq.mask + (int64_t)row * p.sq.mask_words;
+              uint64_t x = word < p.sq.mask_words ? __ldg(&mr[word]) >> sft : 0;
+              if (sft > 32 && word + 1 < p.sq.mask_words) x |= __ldg(&mr[word + 1]) << (64 - sft);
+              bits = (uint32_t)x;
+              if (d0 < 0) bits = (bits << -d0) | ((1u << -d0) - 1u);
+            }
+            vis[w] &= bits;
+          }
+        }
+        __syncwarp();
+        // running maximum
+        float mx = DARIC_NEG_INF;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[32];
+          tc::ld32(s_col + w * 32, x);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (vis[w] >> e) & 1u ? __uint_as_float(x[e]) : DARIC_NEG_INF);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+          }
+        }
+        // the maximum moves when it is over 2^8 ahead (or was none)
+        const bool move = mx > m && (m == DARIC_NEG_INF || (mx - m) * cexp > 8.f);
+        const bool scale_o = move && m != DARIC_NEG_INF;
+        if (__any_sync(0xffffffffu, scale_o)) {
+          const uint32_t pc = c - 1, ps = MT == 2 ? (uint32_t)tile : pc & 1, pp = MT == 2 ? pc & 1 : (pc >> 1) & 1;
+          ok = wait(&sh.pv_done[ps], pp);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc::fence_after();
+          const float a = scale_o ? exp2_fast((m - mx) * cexp) : 1.f;
+          l0 *= a;
+          l1 *= a;
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) {
+            uint32_t x[32];
+            tc::ld32(o_col + w * 32, x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * a);
+            tc::st32(o_col + w * 32, x);
+          }
+          tc::wait_st();
+        }
+        if (move) m = mx;
+        const float mb = m == DARIC_NEG_INF ? 0.f : m * cexp;
+        // weights, over the scores they came from (64 scores become 32 columns)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[32], y[16];
+          tc::ld32(s_col + w * 32, x);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((vis[w] >> e) & 1u)) x[e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float a = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e]), cexp, -mb));
+            const float d = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e + 1]), cexp, -mb));
+            l0 += a;
+            l1 += d;
+            y[e] = Mma<T>::pack(a, d);
+          }
+          tc::st16(s_col + w * 16, y);
+        }
+        tc::wait_st();
+        tc::fence_before();
+        mbar_arrive(&sh.p_full[s]);
+      }
+      if (!ok) break;
+      // ---- the segment's rows
+      {
+        const uint32_t pc = n_item + (uint32_t)g.n - 1;
+        const uint32_t ps = MT == 2 ? (uint32_t)tile : pc & 1, pp = MT == 2 ? pc & 1 : (pc >> 1) & 1;
+        ok = wait(&sh.pv_done[ps], pp);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc::fence_after();
+      }
+      const bool starts = g.tile0 == 0, ends = g.tile0 + g.n == g.ntiles;
+      const float l = l0 + l1;
+      const float inv = starts && ends ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+      const int slot = blockIdx.x * 2 + (starts ? 1 : 0);
+      const bool poison = *(volatile int*)&sh.poison[n_seg & 3] == (int)n_seg;
+      uint8_t* out = p.out + (int64_t)row * p.out_row + (int64_t)head * p.out_head;
+      // partial outputs lie [4 columns][row]: neighbouring rows are neighbours
+      float4* part = reinterpret_cast<float4*>(p.part) + (int64_t)slot * (D / 4) * W::ROWS + i_pair;
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) {
+        uint32_t x[32];
+        __syncwarp();
+        tc::ld32(o_col + w * 32, x);
+        if (poison && real) {
+          const int d0 = max((g.tile0 * kKeys) - g.s.ctx, 0);
+          const int d1 = min((g.tile0 + g.n) * kKeys, g.s.len) - g.s.ctx;
+          for (int d = d0; d < d1; ++d) {
+            const int pos = g.s.ctx + d;
+            if (pos < 0 || !sees_draft(p.sq, row, j, d)) continue;
+            const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
+            const int blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
+            if (blk < 0 || blk >= p.kv.num_pages) continue;
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(
+                p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
+                (int64_t)g.h * p.kv.head_stride + p.kv.v_off) + w * 32;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const uint16_t u = v[e];
+              if ((u & Mma<T>::kExpMask) == Mma<T>::kExpMask)
+                x[e] = __float_as_uint(__uint_as_float(x[e]) + Mma<T>::widen(u));
+            }
+          }
+        }
+        if (real && starts && ends) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              y[k] = Mma<T>::pack(__uint_as_float(x[8 * e + 2 * k]) * inv, __uint_as_float(x[8 * e + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(out + w * 64 + e * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            part[(int64_t)(w * 8 + e) * W::ROWS] =
+                make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
+                            __uint_as_float(x[4 * e + 3]));
+        }
+      }
+      __syncwarp();
+      tc::fence_before();
+      mbar_arrive(&sh.o_empty[tile]);
+      if (real) {
+        if (starts && ends) {
+          if (p.lse) p.lse[(int64_t)row * p.lse_row + head] = l == 0.f ? DARIC_NEG_INF : __fmaf_rn(m, p.scale, logf(l));
+        } else {
+          p.part_ml[(int64_t)slot * W::ROWS + i_pair] = make_float2(m, l);
+        }
+      }
+      if (tid == 0 && starts && !ends)
+        p.desc[blockIdx.x] = make_int4(g.s.row0, g.h | g.rt << 12, g.my_rows,
+                                       (int)split_owner(total, gridDim.x, t + (uint32_t)(g.ntiles - g.tile0) - 1));
+      n_item += (uint32_t)g.n;
+      n_tile += (uint32_t)g.n;
+      ++n_seg;
+      t += (uint32_t)g.n;
+    }
+  }
+  // Nothing of this CTA is under way any more: every product was waited for
+  // by the softmax, every copy by its thread.
+  __syncthreads();
+  if (warp == W::MMA_WARP) {
+    __syncwarp();
+    tc::dealloc512(tmem);
+  }
+}
+
+// Joins the parts of the segment that starts in CTA blockIdx.x and ends in a
+// later one, in the order of the CTAs. A lane is a row, a warp a column group.
+template <class T, int D, int MT>
+__global__ void __launch_bounds__(256) wide_join_kernel(const __grid_constant__ AttendLaunch p) {
+  constexpr int ROWS = 128 * MT;
+  const int4 ds = p.desc[blockIdx.x];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int i = blockIdx.y * 32 + lane;
+  if (ds.x < 0 || blockIdx.y * 32 >= ds.z) return;
+  const int c0 = blockIdx.x, c1 = ds.w;
+  const float cexp = p.scale * kLog2e;
+  float mm = DARIC_NEG_INF;
+  for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, p.part_ml[(int64_t)(c * 2 + (c == c0)) * ROWS + i].x);
+  const float base = mm == DARIC_NEG_INF ? 0.f : mm;
+  float ll = 0.f;
+  constexpr int V = D / 32;  // groups of four columns of a warp
+  float4 o[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0; c <= c1; ++c) {
+    const int64_t s = c * 2 + (c == c0);
+    const float2 ml = p.part_ml[s * ROWS + i];
+    const float w = exp2_fast((ml.x - base) * cexp);
+    ll += ml.y * w;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float4 x = reinterpret_cast<const float4*>(p.part)[(s * (D / 4) + warp * V + v) * ROWS + i];
+      o[v].x += x.x * w;
+      o[v].y += x.y * w;
+      o[v].z += x.z * w;
+      o[v].w += x.w * w;
+    }
+  }
+  if (i >= ds.z) return;
+  const int rt = ds.y >> 12, h = ds.y & 4095;
+  const int pi = rt * ROWS + i;
+  const int64_t row = ds.x + pi / p.sq.group;
+  const int head = h * p.sq.group + pi % p.sq.group;
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  uint8_t* out = p.out + row * p.out_row + (int64_t)head * p.out_head + warp * V * 8;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    *reinterpret_cast<uint2*>(out + v * 8) =
+        make_uint2(Mma<T>::pack(o[v].x * inv, o[v].y * inv), Mma<T>::pack(o[v].z * inv, o[v].w * inv));
+  if (warp == 0 && p.lse) p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : __fmaf_rn(mm, p.scale, logf(ll));
+}
+
+template <class T, int D, int MT>
+void wide_one(const AttendLaunch& p, int grid, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  static_assert(wide_smem<D, MT>() <= 227 * 1024, "shared memory of a CTA");
+  allow_smem(wide_kernel<T, D, MT>, wide_smem<D, MT>(), done);
+  wide_kernel<T, D, MT><<<grid, Wide<D, MT>::THREADS, wide_smem<D, MT>(), s>>>(p);
+  DARIC_CUDA(cudaGetLastError());
+  wide_join_kernel<T, D, MT><<<dim3((unsigned)grid, 4 * MT), 256, 0, s>>>(p);
+  DARIC_CUDA(cudaGetLastError());
+}
+
+template <class T>
+void wide_t(const AttendLaunch& p, int mt, int grid, cudaStream_t s) {
+  if (p.kv.head_dim == 64) return mt == 2 ? wide_one<T, 64, 2>(p, grid, s) : wide_one<T, 64, 1>(p, grid, s);
+  mt == 2 ? wide_one<T, 128, 2>(p, grid, s) : wide_one<T, 128, 1>(p, grid, s);
+}
+
+}  // namespace
+
+void launch_wide(const AttendLaunch& p, int dtype, int mt, int grid, cudaStream_t s) {
+  if (dtype == DARIC_DTYPE_BF16) return wide_t<__nv_bfloat16>(p, mt, grid, s);
+  wide_t<__half>(p, mt, grid, s);
+}
+
+}  // namespace daric

@@ -65,6 +65,31 @@ def test_wide_trees(t, words):
     check_tree(bt, *run_tree(bt, mask), mask)
 
 
+@pytest.mark.parametrize("dtype,layout,d", [("bf16", "5d", 128), ("f16", "4d", 128), ("bf16", "5dpf", 64), ("f16", "5d", 64),
+                                            ("bf16", "4d", 256)])
+@pytest.mark.parametrize("kvh,group,t", [(2, 4, 16), (1, 8, 17), (2, 7, 37), (1, 8, 64)])
+def test_many_rows(dtype, layout, d, kvh, group, t):
+    """64 to 512 (row, head) pairs of a KV head, ragged, trees and chains, one and several CTAs per segment."""
+    bt = Batch([t + 1, 900, 128 + t, 5000], [t, t - 3, 1, t], kvh=kvh, group=group, d=d, dtype=dtype, layout=layout, seed=t)
+    check_tree(bt, *run_tree(bt))
+    mask = tree_masks(bt.rows, 1, torch.Generator().manual_seed(t))
+    check_tree(bt, *run_tree(bt, mask), mask)
+
+
+def test_growing_logits_move_the_maximum():
+    """Keys whose logits rise along the sequence by far more than 2^8 each tile:
+    what was summed up so far is rescaled, often to nothing."""
+    bt = Batch([1500, 700], [16, 16], kvh=1, group=4, seed=41)
+    for b in range(2):
+        pos = torch.arange(bt.lens[b], device="cuda")
+        blk = bt.table[b].long()[pos // bt.bs]
+        bt.k[blk, pos % bt.bs, 0, 0] = (pos.float() / 20).to(bt.cache.dtype)
+    bt.q[..., 0] = bt.q[..., 0].abs() + 1
+    check_tree(bt, *run_tree(bt))
+    bt.q[..., 0] = -bt.q[..., 0]
+    check_tree(bt, *run_tree(bt))
+
+
 def test_appended_prompt_rows():
     """Hundreds of causal rows per sequence: several row tiles."""
     bt = Batch([500, 333], [300, 333], kvh=2, group=3, seed=5)
