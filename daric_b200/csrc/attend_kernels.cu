@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
         nxt_in = i - e * p.kv.page_size;
         int pg = e, left = sg.s.len - i;
         if (SPARSE) {
-          pg = e < p.k && seq_id >= 0 ? __ldg(&prow[e]) : -1;
+          pg = e < p.k && seq_id >= 0 ? ld_ahead(&prow[e]) : -1;
           if (pg >= p.sq.table_cols) {
             atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
             pg = -1;
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
           left = pg < 0 ? 0 : qpos + 1 - pg * p.kv.page_size - nxt_in;
         }
         if (left > 0) {
-          nxt_blk = __ldg(&trow[pg]);
+          nxt_blk = ld_ahead(&trow[pg]);
           nxt_n = one ? min(left, G::KPW) : 1;
         }
       }

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, D > 128 ? 2 : 4) weight_str
       if (it < n) {
         const int pg = (int)fdiv((uint32_t)key0, p.kv.page_div);
         tok = key0 - pg * p.kv.page_size;
-        blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
+        blk = ld_ahead(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
       }
     } else {
 #pragma unroll

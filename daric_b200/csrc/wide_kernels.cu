@@ -13,13 +13,14 @@
 // only when the running maximum is over 2^8 times ahead, so that O is rarely
 // read back. m, l, S and O are fp32.
 //
-// Warps: 4 MT of softmax, one thread each for a row; one that issues the
-// matrix instructions; four that copy. A copy slot is a K or a V tile (16-byte
-// cp.async, a page table lookup per key, into the 128-byte swizzle); each
-// copying thread reports a slot when its own copies of it have landed, two
-// slots behind the newest. With MT = 2 the two tiles take turns, so one is
-// multiplied while the other is exponentiated; with MT = 1 the key tiles do,
-// through two S areas.
+// Two streams of (scores, weights, output) take turns, so that one is
+// multiplied while the other is exponentiated: with MT = 2 the two row tiles,
+// with MT = 1 the even and the odd key tiles, whose two outputs are joined at
+// the end of a segment. Warps: four of softmax per stream, one thread a row;
+// four that copy; one that issues the matrix instructions. A copy slot is a K
+// or a V tile (16-byte cp.async, a page table lookup per key, into the
+// 128-byte swizzle); each copying thread reports a slot when its own copies of
+// it have landed, some slots behind the newest.
 //
 // Bound: the K and V bytes up to about 256 pairs; above, exp2 (16 a clock and
 // SM) and the matrix rate together. Why tcgen05 and not the warp matrix
@@ -51,25 +52,27 @@ struct Wide {
   static constexpr int SLOT = kKeys * D * 2;
   static constexpr int QB = ROWS * D * 2;
   static constexpr int NS = D == 64 ? 10 : (MT == 2 ? 5 : 6);
-  static constexpr int THREADS = 128 * MT + 32 + kCopyThreads;
-  static constexpr int MMA_WARP = 4 * MT;
-  static constexpr int COPY_WARP = 4 * MT + 1;
+  static constexpr int BEHIND = NS > 5 ? 3 : 2;  // slots copied but not reported yet
+  static constexpr int THREADS = 512;  // the last three warps only lend their registers
+  static constexpr int COPY_WARP = 8;
+  static constexpr int MMA_WARP = 12;
   static constexpr int TILES = QB + NS * SLOT;
 };
 
 struct WideShared {
   uint64_t full[10], empty[10];
   uint64_t s_full[2], p_full[2], pv_done[2], o_empty[2];
-  uint64_t q_full, q_empty;
+  uint64_t q_full, q_empty, ml_full;
+  float2 ml[128];          // MT = 1: maximum and sum of the odd key tiles
   uint32_t vmask[kMaskRing][4];
-  uint32_t off[2][kKeys];  // row offsets of two key tiles, 16-byte units of the layer
+  uint32_t off[3][kKeys];  // row offsets of three key tiles, 16-byte units of the layer
   uint32_t tmem;
   int abort;               // a wait gave up: everyone leaves
   int poison[4];           // by count modulo 4: the segment if its drafted V rows hold infinities or NaN
 };
 template <int D, int MT>
 constexpr int wide_smem() {
-  return Wide<D, MT>::TILES + 1024 + (int)sizeof(WideShared);
+  return Wide<D, MT>::TILES + (int)sizeof(WideShared);
 }
 
 // The part of a segment that a CTA works on.
@@ -85,8 +88,7 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int HB = D / 64;          // 64-element halves of a row
   constexpr int HALF = kKeys * 128;   // bytes of such a half of a tile
-  extern __shared__ uint8_t raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t base[];  // the only shared memory: it starts on 1024 bytes
   WideShared& sh = *reinterpret_cast<WideShared*>(base + W::TILES);
   uint8_t* q_tile = base;
   uint8_t* slots = base + W::QB;
@@ -132,6 +134,7 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
   }
   if (tid == 0) {
     p.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (smem_u32(base) & 1023) atomicOr(p.sq.err, DEV_ERR_TIMEOUT);
     for (int i = 0; i < W::NS; ++i) {
       mbar_init(&sh.full[i], kCopyThreads);
       mbar_init(&sh.empty[i], 1);
@@ -144,12 +147,13 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
     }
     mbar_init(&sh.q_full, kCopyThreads);
     mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.ml_full, 128);
     mbar_init_fence();
     sh.abort = 0;
     for (int i = 0; i < 4; ++i) sh.poison[i] = -1;
   }
   __syncthreads();  // sums are read, barriers are ready
-  if (t0 >= t1) return;
+  if (t0 >= t1 || (smem_u32(base) & 1023)) return;
   if (warp == W::MMA_WARP) tc::alloc512(&sh.tmem);
   tc::fence_before();
   __syncthreads();
@@ -201,11 +205,20 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
   auto k_slot = [&](int i) { return MT == 2 ? 2 * i : (i == 0 ? 0 : 2 * i - 1); };
   auto v_slot = [&](int i, int n) { return MT == 2 ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
 
-  if (warp >= W::COPY_WARP) {
+  // items of stream s in a part of n key tiles, and the key tile of its local item
+  auto items_of = [&](int s, int n) { return MT == 2 ? n : (n + 1 - s) / 2; };
+
+  if (warp >= W::COPY_WARP && warp < W::MMA_WARP) {
     // ------------------------------------------------------------ copies --
+    // Registers: 512 threads start with 128 each, 65536 in all; 256 x 184 of
+    // softmax + 128 x 80 here + 128 x 64 = 65536.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int ct = tid - W::COPY_WARP * 32;
     uint32_t n_slot = 0, n_seg = 0, n_tile = 0;  // slots, segments, key tiles so far
-    uint64_t* pend[2] = {nullptr, nullptr};      // groups not reported yet, older first
+    constexpr int BH = W::BEHIND;
+    uint64_t* pend[BH];                          // groups not reported yet, older first
+#pragma unroll
+    for (int i = 0; i < BH; ++i) pend[i] = nullptr;
     auto report = [&](uint64_t* bar) {
       if (!bar) return;
       fence_proxy_async();
@@ -213,19 +226,22 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
     };
     auto flush = [&]() {
       cp_wait<0>();
-      report(pend[0]);
-      report(pend[1]);
-      pend[0] = pend[1] = nullptr;
+#pragma unroll
+      for (int i = 0; i < BH; ++i) {
+        report(pend[i]);
+        pend[i] = nullptr;
+      }
     };
-    auto push = [&](uint64_t* bar) {  // a group was issued: reports the one two before it
+    auto push = [&](uint64_t* bar) {  // a group was issued: reports the one BH before it
       cp_commit();
-      cp_wait<2>();
+      cp_wait<BH>();
       report(pend[0]);
-      pend[0] = pend[1];
-      pend[1] = bar;
+#pragma unroll
+      for (int i = 0; i + 1 < BH; ++i) pend[i] = pend[i + 1];
+      pend[BH - 1] = bar;
     };
     auto take = [&](uint64_t* bar, uint32_t parity) {  // what is reported late must not be waited for
-      if (mbar_try_wait(bar, parity)) return true;
+      if (tc::mbar_test(bar, parity)) return true;
       flush();
       return wait(bar, parity);
     };
@@ -244,7 +260,7 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
     bool ok = true;
     while (ok && t < t1) {
       Part g;
-      if (!together(part_at(t, g))) break;
+      if (!together(part_at(t, g))) break;  // the same for all: they read the same lengths
       const int32_t* trow = p.sq.table + (int64_t)g.b * p.sq.table_ld;
       const uint8_t* kv = p.kv.base + (int64_t)g.h * p.kv.head_stride;
       const int see = all_see(g);
@@ -269,7 +285,7 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
       auto lookup = [&](int i) {  // block of this thread's key of tile i, -1: none
         const int pos = (g.tile0 + i) * kKeys + ct;
         if (i >= g.n || pos >= g.s.len) return -1;
-        return __ldg(&trow[fdiv((uint32_t)pos, p.kv.page_div)]);
+        return ld_ahead(&trow[fdiv((uint32_t)pos, p.kv.page_div)]);
       };
       int blk = lookup(0);
       auto place = [&](int i) {  // offsets and mask of tile i; looks the next one up
@@ -285,28 +301,32 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
           off = (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride;
         }
         const unsigned m = __ballot_sync(0xffffffffu, in);
-        // the copies that read these offsets before are issued
-        asm volatile("bar.sync 1, %0;" ::"n"(kCopyThreads) : "memory");
         if (lane == 0) sh.vmask[(n_tile + i) % kMaskRing][ct >> 5] = m;
-        sh.off[i & 1][ct] = in ? (uint32_t)(off >> 4) : 0xffffffffu;
+        sh.off[i % 3][ct] = in ? (uint32_t)(off >> 4) : 0xffffffffu;
         blk = lookup(i + 1);
-        __syncwarp();
-        asm volatile("bar.sync 1, %0;" ::"n"(kCopyThreads) : "memory");
+        // The offsets of the tile three before this one are read by now: its
+        // last copies were issued before the meeting of the tile in between.
+        ok = together(ok);
       };
       auto copy = [&](int i, bool v_tile) {
         const uint32_t st = n_slot % W::NS, use = n_slot / W::NS;
         if (!ok) return;
-        if (use) ok = together(take(&sh.empty[st], (use - 1) & 1));
-        if (!ok) return;
+        if (use) ok = take(&sh.empty[st], (use - 1) & 1);
+        if (!ok) return;  // all stop at the next meeting
         constexpr int CH = D / 8, RPI = kCopyThreads / CH;  // rows at a time
         const int c = ct % CH;
         const uint8_t* src = kv + (v_tile ? p.kv.v_off : 0) + c * 16;
         const uint32_t dst = smem_u32(slots) + st * W::SLOT + (c >> 3) * HALF;
-#pragma unroll 8
-        for (int r = ct / CH; r < kKeys; r += RPI) {
-          const uint32_t o = sh.off[i & 1][r];
-          const bool in = o != 0xffffffffu;
-          cp16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? (int64_t)o * 16 : 0), in);
+        const uint32_t* off = sh.off[i % 3];
+        uint32_t o[kKeys / RPI];  // read ahead of the copies, which nothing is moved across
+#pragma unroll
+        for (int k = 0; k < kKeys / RPI; ++k) o[k] = off[ct / CH + k * RPI];
+        const uint32_t d0 = dst + (ct / CH) * 128;
+#pragma unroll
+        for (int k = 0; k < kKeys / RPI; ++k) {
+          const bool in = o[k] != 0xffffffffu;
+          const int r7 = (ct / CH + k * RPI) & 7;
+          cp16(d0 + k * RPI * 128 + (((c & 7) ^ r7) << 4), src + (in ? (int64_t)o[k] * 16 : 0), in);
         }
         if (v_tile && (g.tile0 + i + 1) * kKeys > see) {
           // drafted V rows that some rows must not see: values without a
@@ -336,32 +356,39 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
         ++n_slot;
       };
       if (MT == 2) {
-        for (int i = 0; ok && i < g.n; ++i) {
+        for (int i = 0; i < g.n; ++i) {
           place(i);
+          if (!ok) break;
           copy(i, false);
           copy(i, true);
         }
       } else {
         place(0);
         copy(0, false);
-        for (int i = 1; ok && i < g.n; ++i) {
+        for (int i = 1; i < g.n; ++i) {
           place(i);
+          if (!ok) break;
           copy(i, false);
           copy(i - 1, true);
         }
         copy(g.n - 1, true);
       }
+      ok = together(ok);
       n_tile += (uint32_t)g.n;
       ++n_seg;
       t += (uint32_t)g.n;
     }
     flush();
     cp_wait<0>();
-  } else if (warp == W::MMA_WARP) {
+  } else if (warp >= W::MMA_WARP) {
     // ---------------------------------------------------------- products --
-    if (lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == W::MMA_WARP && lane == 0) {
       constexpr uint32_t id_qk = tc::instr_desc(BF, false, 128, kKeys), id_pv = tc::instr_desc(BF, true, 128, D);
-      uint32_t n_slot = 0, n_seg = 0, n_item = 0;
+      uint32_t n_slot = 0, n_seg = 0;
+      uint32_t done[2] = {0, 0}, seen[2] = {0, 0};  // items of each stream, and segments with items, before this one
+      const uint64_t q_desc = tc::smem_desc(smem_u32(q_tile), 16), k_desc = tc::smem_desc(smem_u32(slots), 16),
+                     v_desc = tc::smem_desc(smem_u32(slots), HALF);
       uint32_t t = t0;
       bool ok = true;
       while (ok && t < t1) {
@@ -372,43 +399,47 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
         const int items = MT * g.n;
         auto slot_of = [&](int s) { return (n_slot + (uint32_t)s) % W::NS; };
         auto full = [&](int s) { return wait(&sh.full[slot_of(s)], ((n_slot + (uint32_t)s) / W::NS) & 1); };
-        auto scores = [&](int j) {  // S of item j
-          const int i = MT == 2 ? j >> 1 : j, tile = MT == 2 ? j & 1 : 0;
-          const int ks = k_slot(i);
+        auto scores = [&](int j) {  // S of item j of stream j & 1
+          const uint32_t s = j & 1;
+          const int ks = k_slot(MT == 2 ? j >> 1 : j);
           if (!full(ks)) return false;
           tc::fence_after();
-          const uint32_t s = (n_item + (uint32_t)j) & 1;
-          const uint32_t qa = smem_u32(q_tile) + tile * (HB * HALF), ka = smem_u32(slots) + slot_of(ks) * W::SLOT;
+          const uint64_t qa = q_desc + (MT == 2 ? s * (uint32_t)(HB * HALF >> 4) : 0u);
+          const uint64_t ka = k_desc + slot_of(ks) * (uint32_t)(W::SLOT >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t o = (k >> 2) * HALF + (k & 3) * 32;
-            tc::mma_ss(tmem + s * kKeys, tc::smem_desc(qa + o, 16), tc::smem_desc(ka + o, 16), id_qk, k > 0);
+            constexpr int STEP = 32 >> 4;
+            const int o = (k >> 2) * (HALF >> 4) + (k & 3) * STEP;
+            tc::mma_ss(tmem + s * kKeys, qa + o, ka + o, id_qk, k > 0);
           }
           tc::commit(&sh.s_full[s]);
-          if (MT == 1 || tile == 1) tc::commit(&sh.empty[slot_of(ks)]);
+          if (MT == 1 || s == 1) tc::commit(&sh.empty[slot_of(ks)]);
           if (j == items - 1) tc::commit(&sh.q_empty);
           return true;
         };
         ok = scores(0) && (items < 2 || scores(1));
         for (int j = 0; ok && j < items; ++j) {
-          const int i = MT == 2 ? j >> 1 : j, tile = MT == 2 ? j & 1 : 0;
-          const uint32_t c = n_item + (uint32_t)j, s = c & 1;
-          if (j < MT && n_seg) ok = wait(&sh.o_empty[tile], (n_seg - 1) & 1);
-          const int vs = v_slot(i, g.n);
-          ok = ok && wait(&sh.p_full[s], (c >> 1) & 1) && full(vs);
+          const uint32_t s = j & 1;
+          const int i = j >> 1;  // local item of the stream
+          const int vs = v_slot(MT == 2 ? i : j, g.n);
+          if (i == 0 && done[s]) ok = wait(&sh.o_empty[s], (seen[s] - 1) & 1);
+          ok = ok && full(vs) && wait(&sh.p_full[s], (done[s] + (uint32_t)i) & 1);
           if (!ok) break;
           tc::fence_after();
-          const uint32_t va = smem_u32(slots) + slot_of(vs) * W::SLOT;
+          const uint64_t va = v_desc + slot_of(vs) * (uint32_t)(W::SLOT >> 4);
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            tc::mma_ts(tmem + 2 * kKeys + tile * D, tmem + s * kKeys + k * 8, tc::smem_desc(va + k * 2048, HALF), id_pv,
-                       i > 0 || k > 0);
+            tc::mma_ts(tmem + 2 * kKeys + s * D, tmem + s * kKeys + k * 8, va + k * (2048 >> 4), id_pv, i > 0 || k > 0);
           tc::commit(&sh.pv_done[s]);
-          if (MT == 1 || tile == 1) tc::commit(&sh.empty[slot_of(vs)]);
+          if (MT == 1 || s == 1) tc::commit(&sh.empty[slot_of(vs)]);
           if (j + 2 < items) ok = scores(j + 2);
         }
         n_slot += 2 * (uint32_t)g.n;
-        n_item += (uint32_t)items;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          done[s] += (uint32_t)items_of(s, g.n);
+          seen[s] += items_of(s, g.n) > 0;
+        }
         ++n_seg;
         t += (uint32_t)g.n;
       }
@@ -416,12 +447,15 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
     __syncwarp();
   } else {
     // ----------------------------------------------------------- softmax --
-    const int tile = warp >> 2;                            // row tile of the CTA
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int st = warp >> 2;                              // stream
+    const int tile = MT == 2 ? st : 0;                     // row tile of the CTA
     const int r = (warp & 3) * 32 + lane;                  // row of it
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t o_col = tmem + lanes + 2 * kKeys + tile * D;
+    const uint32_t s_col = tmem + lanes + st * kKeys, o_col = tmem + lanes + 2 * kKeys + st * D;
     const float cexp = p.scale * kLog2e;
-    uint32_t n_item = 0, n_seg = 0, n_tile = 0;            // items of this tile so far
+    uint32_t done = 0, other = 0;                          // items of this stream, of the other one (MT = 1)
+    uint32_t n_seg = 0, n_tile = 0, n_ml = 0;
     uint32_t t = t0;
     bool ok = true;
     while (ok && t < t1) {
@@ -433,25 +467,53 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
       const int j = real ? (int)fdiv((uint32_t)pi, p.sq.group_div) : 0;  // row of the sequence
       const int row = g.s.row0 + j, head = g.h * group + pi - j * group;
       const int see = all_see(g);
+      const int items = items_of(st, g.n);
       float m = DARIC_NEG_INF, l0 = 0.f, l1 = 0.f;
-      for (int i = 0; i < g.n; ++i) {
-        const uint32_t c = n_item + (uint32_t)i;
-        // MT = 2: the tile's own S area; MT = 1: the two in turn
-        const uint32_t s = MT == 2 ? (uint32_t)tile : c & 1, ph = MT == 2 ? c & 1 : (c >> 1) & 1;
-        ok = wait(&sh.s_full[s], ph);
+      for (int li = 0; li < items; ++li) {
+        const uint32_t c = done + (uint32_t)li;
+        const int i = MT == 2 ? li : 2 * li + st;  // key tile
+        ok = wait(&sh.s_full[st], c & 1);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc::fence_after();
-        const uint32_t s_col = tmem + lanes + s * kKeys;
         const int key0 = (g.tile0 + i) * kKeys;
         const uint32_t* vm = sh.vmask[(n_tile + (uint32_t)i) % kMaskRing];
-        uint32_t vis[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) vis[w] = vm[w];
-        bool masked = (vis[0] & vis[1] & vis[2] & vis[3]) != 0xffffffffu;
-        if (key0 + kKeys > see) {
-          masked = true;
+        const bool draft = key0 + kKeys > see;
+        const bool masked = draft || (vm[0] & vm[1] & vm[2] & vm[3]) != 0xffffffffu;
+        float mb = m * cexp;
+        bool careful = masked || __any_sync(0xffffffffu, m == DARIC_NEG_INF);
+        if (!careful) {
+          // one pass: weights by the maximum so far, kept in registers until
+          // the maximum of this tile is known to be near enough
+          uint32_t y[64];
+          float mx = DARIC_NEG_INF, a0 = 0.f, a1 = 0.f;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
+            uint32_t x[32];
+            tc::ld32(s_col + w * 32, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float u = __uint_as_float(x[2 * e]), v = __uint_as_float(x[2 * e + 1]);
+              mx = fmaxf(mx, fmaxf(u, v));
+              const float a = exp2_fast(__fmaf_rn(u, cexp, -mb)), d = exp2_fast(__fmaf_rn(v, cexp, -mb));
+              a0 += a;
+              a1 += d;
+              y[w * 16 + e] = Mma<T>::pack(a, d);
+            }
+          }
+          careful = __any_sync(0xffffffffu, (mx - m) * cexp > 8.f);
+          if (!careful) {
+            l0 += a0;
+            l1 += a1;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) tc::st32(s_col + w * 32, *reinterpret_cast<const uint32_t(*)[32]>(&y[w * 32]));
+          }
+        }
+        if (careful) {
+          uint32_t vis[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            vis[w] = vm[w];
+            if (!draft) continue;
             const int d0 = key0 + 32 * w - g.s.ctx;  // drafted token of bit 0
             uint32_t bits;
             if (d0 <= -32) {
@@ -471,142 +533,158 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
             }
             vis[w] &= bits;
           }
-        }
-        __syncwarp();
-        // running maximum
-        float mx = DARIC_NEG_INF;
+          __syncwarp();
+          float mx = DARIC_NEG_INF;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t x[32];
-          tc::ld32(s_col + w * 32, x);
-          if (masked) {
+          for (int w = 0; w < 4; ++w) {
+            uint32_t x[32];
+            tc::ld32(s_col + w * 32, x);
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (vis[w] >> e) & 1u ? __uint_as_float(x[e]) : DARIC_NEG_INF);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
           }
-        }
-        // the maximum moves when it is over 2^8 ahead (or was none)
-        const bool move = mx > m && (m == DARIC_NEG_INF || (mx - m) * cexp > 8.f);
-        const bool scale_o = move && m != DARIC_NEG_INF;
-        if (__any_sync(0xffffffffu, scale_o)) {
-          const uint32_t pc = c - 1, ps = MT == 2 ? (uint32_t)tile : pc & 1, pp = MT == 2 ? pc & 1 : (pc >> 1) & 1;
-          ok = wait(&sh.pv_done[ps], pp);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          tc::fence_after();
-          const float a = scale_o ? exp2_fast((m - mx) * cexp) : 1.f;
-          l0 *= a;
-          l1 *= a;
+          // the maximum moves when it is over 2^8 ahead (or was none)
+          const bool move = mx > m && (m == DARIC_NEG_INF || (mx - m) * cexp > 8.f);
+          const bool scale_o = move && m != DARIC_NEG_INF;
+          if (__any_sync(0xffffffffu, scale_o)) {
+            ok = wait(&sh.pv_done[st], (c - 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::fence_after();
+            const float a = scale_o ? exp2_fast((m - mx) * cexp) : 1.f;
+            l0 *= a;
+            l1 *= a;
+#pragma unroll 1
+            for (int w = 0; w < D / 32; ++w) {
+              uint32_t x[32];
+              tc::ld32(o_col + w * 32, x);
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) {
-            uint32_t x[32];
-            tc::ld32(o_col + w * 32, x);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * a);
-            tc::st32(o_col + w * 32, x);
+              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * a);
+              tc::st32(o_col + w * 32, x);
+            }
+            tc::wait_st();
           }
-          tc::wait_st();
-        }
-        if (move) m = mx;
-        const float mb = m == DARIC_NEG_INF ? 0.f : m * cexp;
-        // weights, over the scores they came from (64 scores become 32 columns)
+          if (move) m = mx;
+          mb = m == DARIC_NEG_INF ? 0.f : m * cexp;
+          // weights, over the scores they came from (64 scores become 32 columns)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t x[32], y[16];
-          tc::ld32(s_col + w * 32, x);
-          if (masked) {
+          for (int w = 0; w < 4; ++w) {
+            uint32_t x[32], y[16];
+            tc::ld32(s_col + w * 32, x);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((vis[w] >> e) & 1u)) x[e] = 0xff800000u;
+            for (int e = 0; e < 16; ++e) {
+              const float u = (vis[w] >> (2 * e)) & 1u ? __uint_as_float(x[2 * e]) : DARIC_NEG_INF;
+              const float v = (vis[w] >> (2 * e + 1)) & 1u ? __uint_as_float(x[2 * e + 1]) : DARIC_NEG_INF;
+              const float a = exp2_fast(__fmaf_rn(u, cexp, -mb)), d = exp2_fast(__fmaf_rn(v, cexp, -mb));
+              l0 += a;
+              l1 += d;
+              y[e] = Mma<T>::pack(a, d);
+            }
+            tc::st16(s_col + w * 16, y);
           }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e]), cexp, -mb));
-            const float d = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e + 1]), cexp, -mb));
-            l0 += a;
-            l1 += d;
-            y[e] = Mma<T>::pack(a, d);
-          }
-          tc::st16(s_col + w * 16, y);
         }
         tc::wait_st();
         tc::fence_before();
-        mbar_arrive(&sh.p_full[s]);
+        mbar_arrive(&sh.p_full[st]);
       }
       if (!ok) break;
       // ---- the segment's rows
-      {
-        const uint32_t pc = n_item + (uint32_t)g.n - 1;
-        const uint32_t ps = MT == 2 ? (uint32_t)tile : pc & 1, pp = MT == 2 ? pc & 1 : (pc >> 1) & 1;
-        ok = wait(&sh.pv_done[ps], pp);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        tc::fence_after();
+      if (items > 0) ok = wait(&sh.pv_done[st], (done + (uint32_t)items - 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const bool pair = MT == 1 && g.n > 1;  // the odd key tiles have an output of their own
+      bool writes = true;
+      float a1 = 0.f, l = l0 + l1, a0 = 1.f;
+      if (MT == 1) {
+        writes = st == 0;
+        if (pair && st == 1) {
+          sh.ml[r] = make_float2(m, l);
+          mbar_arrive(&sh.ml_full);
+        }
+        if (pair && st == 0) {
+          ok = wait(&sh.ml_full, n_ml & 1) && wait(&sh.pv_done[1], (other + (uint32_t)items_of(1, g.n) - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          const float2 ml = sh.ml[r];
+          const float mm = fmaxf(m, ml.x), mz = mm == DARIC_NEG_INF ? 0.f : mm;
+          a0 = exp2_fast((m - mz) * cexp);
+          a1 = exp2_fast((ml.x - mz) * cexp);
+          l = l * a0 + ml.y * a1;
+          m = mm;
+        }
+        n_ml += pair;
+        other += (uint32_t)items_of(1 - st, g.n);
       }
-      const bool starts = g.tile0 == 0, ends = g.tile0 + g.n == g.ntiles;
-      const float l = l0 + l1;
-      const float inv = starts && ends ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-      const int slot = blockIdx.x * 2 + (starts ? 1 : 0);
-      const bool poison = *(volatile int*)&sh.poison[n_seg & 3] == (int)n_seg;
-      uint8_t* out = p.out + (int64_t)row * p.out_row + (int64_t)head * p.out_head;
-      // partial outputs lie [4 columns][row]: neighbouring rows are neighbours
-      float4* part = reinterpret_cast<float4*>(p.part) + (int64_t)slot * (D / 4) * W::ROWS + i_pair;
+      if (writes) {
+        tc::fence_after();
+        const bool starts = g.tile0 == 0, ends = g.tile0 + g.n == g.ntiles;
+        const float inv = starts && ends ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const int slot = blockIdx.x * 2 + (starts ? 1 : 0);
+        const bool poison = *(volatile int*)&sh.poison[n_seg & 3] == (int)n_seg;
+        uint8_t* out = p.out + (int64_t)row * p.out_row + (int64_t)head * p.out_head;
+        // partial outputs lie [4 columns][row]: neighbouring rows are neighbours
+        float4* part = reinterpret_cast<float4*>(p.part) + (int64_t)slot * (D / 4) * W::ROWS + i_pair;
+#pragma unroll 1
+        for (int w = 0; w < D / 32; ++w) {
+          uint32_t x[32];
+          __syncwarp();
+          tc::ld32(o_col + w * 32, x);
+          if (pair) {
+            uint32_t z[32];
+            tc::ld32(o_col + D + w * 32, z);
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        uint32_t x[32];
-        __syncwarp();
-        tc::ld32(o_col + w * 32, x);
-        if (poison && real) {
-          const int d0 = max((g.tile0 * kKeys) - g.s.ctx, 0);
-          const int d1 = min((g.tile0 + g.n) * kKeys, g.s.len) - g.s.ctx;
-          for (int d = d0; d < d1; ++d) {
-            const int pos = g.s.ctx + d;
-            if (pos < 0 || !sees_draft(p.sq, row, j, d)) continue;
-            const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
-            const int blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
-            if (blk < 0 || blk >= p.kv.num_pages) continue;
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(
-                p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
-                (int64_t)g.h * p.kv.head_stride + p.kv.v_off) + w * 32;
+            for (int e = 0; e < 32; ++e)
+              x[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), a1, __uint_as_float(x[e]) * a0));
+          }
+          if (poison && real) {
+            const int d0 = max((g.tile0 * kKeys) - g.s.ctx, 0);
+            const int d1 = min((g.tile0 + g.n) * kKeys, g.s.len) - g.s.ctx;
+            for (int d = d0; d < d1; ++d) {
+              const int pos = g.s.ctx + d;
+              if (pos < 0 || !sees_draft(p.sq, row, j, d)) continue;
+              const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
+              const int blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
+              if (blk < 0 || blk >= p.kv.num_pages) continue;
+              const uint16_t* v = reinterpret_cast<const uint16_t*>(
+                  p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
+                  (int64_t)g.h * p.kv.head_stride + p.kv.v_off) + w * 32;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const uint16_t u = v[e];
-              if ((u & Mma<T>::kExpMask) == Mma<T>::kExpMask)
-                x[e] = __float_as_uint(__uint_as_float(x[e]) + Mma<T>::widen(u));
+              for (int e = 0; e < 32; ++e) {
+                const uint16_t u = v[e];
+                if ((u & Mma<T>::kExpMask) == Mma<T>::kExpMask)
+                  x[e] = __float_as_uint(__uint_as_float(x[e]) + Mma<T>::widen(u));
+              }
             }
           }
-        }
-        if (real && starts && ends) {
+          if (real && starts && ends) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t y[4];
+            for (int e = 0; e < 4; ++e) {
+              uint32_t y[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              y[k] = Mma<T>::pack(__uint_as_float(x[8 * e + 2 * k]) * inv, __uint_as_float(x[8 * e + 2 * k + 1]) * inv);
-            *reinterpret_cast<uint4*>(out + w * 64 + e * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+              for (int k = 0; k < 4; ++k)
+                y[k] = Mma<T>::pack(__uint_as_float(x[8 * e + 2 * k]) * inv, __uint_as_float(x[8 * e + 2 * k + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + w * 64 + e * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          } else if (real) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              part[(int64_t)(w * 8 + e) * W::ROWS] =
+                  make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
+                              __uint_as_float(x[4 * e + 3]));
           }
-        } else if (real) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            part[(int64_t)(w * 8 + e) * W::ROWS] =
-                make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
-                            __uint_as_float(x[4 * e + 3]));
         }
-      }
-      __syncwarp();
-      tc::fence_before();
-      mbar_arrive(&sh.o_empty[tile]);
-      if (real) {
-        if (starts && ends) {
-          if (p.lse) p.lse[(int64_t)row * p.lse_row + head] = l == 0.f ? DARIC_NEG_INF : __fmaf_rn(m, p.scale, logf(l));
-        } else {
-          p.part_ml[(int64_t)slot * W::ROWS + i_pair] = make_float2(m, l);
+        __syncwarp();
+        tc::fence_before();
+        mbar_arrive(&sh.o_empty[st]);
+        if (pair) mbar_arrive(&sh.o_empty[1]);
+        if (real) {
+          if (starts && ends) {
+            if (p.lse) p.lse[(int64_t)row * p.lse_row + head] = l == 0.f ? DARIC_NEG_INF : __fmaf_rn(m, p.scale, logf(l));
+          } else {
+            p.part_ml[(int64_t)slot * W::ROWS + i_pair] = make_float2(m, l);
+          }
         }
+        if (tid == 0 && starts && !ends)
+          p.desc[blockIdx.x] = make_int4(g.s.row0, g.h | g.rt << 12, g.my_rows,
+                                         (int)split_owner(total, gridDim.x, t + (uint32_t)(g.ntiles - g.tile0) - 1));
       }
-      if (tid == 0 && starts && !ends)
-        p.desc[blockIdx.x] = make_int4(g.s.row0, g.h | g.rt << 12, g.my_rows,
-                                       (int)split_owner(total, gridDim.x, t + (uint32_t)(g.ntiles - g.tile0) - 1));
-      n_item += (uint32_t)g.n;
+      done += (uint32_t)items;
       n_tile += (uint32_t)g.n;
       ++n_seg;
       t += (uint32_t)g.n;
