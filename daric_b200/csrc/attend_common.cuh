@@ -24,6 +24,25 @@ void allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
   if (dev < 64) done.fetch_or(bit, std::memory_order_release);
 }
 
+// A second kernel that needs the first one's results is launched while the
+// first runs (programmatic dependent launch) and waits on the GPU: its launch
+// costs no time of its own.
+__device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class K, class P>
+void launch_after(K kern, dim3 grid, int threads, cudaStream_t s, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  DARIC_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 #define DARIC_NEG_INF __int_as_float(0xff800000)

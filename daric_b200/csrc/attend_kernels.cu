@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
   uint8_t* ring = smem + kg * G::S * G::STAGE;
   uint8_t* qs = smem + (G::RING > G::MERGE ? G::RING : G::MERGE);
   const int group = p.sq.group;
+  grid_next();
 
   // ---- the line of tiles and this CTA's part of it
   uint32_t total, t0, t1;
@@ -506,6 +507,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
 template <class T, int D, int RG>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AttendLaunch p) {
   constexpr int ROWS = 16 * RG;
+  grid_wait();
   const int4 ds = p.desc[blockIdx.x];
   const int i = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (ds.x < 0 || i >= ds.z) return;
@@ -554,8 +556,7 @@ void launch_one(const AttendLaunch& p, int grid, cudaStream_t s) {
   allow_smem(kern, bytes, done);
   kern<<<grid, kThreads, bytes, s>>>(p);
   DARIC_CUDA(cudaGetLastError());
-  join_kernel<T, D, RG><<<dim3((unsigned)grid, 4 * RG), 128, 0, s>>>(p);
-  DARIC_CUDA(cudaGetLastError());
+  launch_after(join_kernel<T, D, RG>, dim3((unsigned)grid, 4 * RG), 128, s, p);
 }
 
 template <class T, int D>

@@ -23,6 +23,16 @@ __host__ __device__ constexpr uint32_t instr_desc(bool bf16, bool b_mn, int m, i
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// One lane of a warp that is together: the others skip. Matrix instructions
+// take their operands from the warp's uniform registers, so the warp stays
+// together up to here and what they are made of is the same in every lane.
+__device__ __forceinline__ bool elect() {
+  uint32_t mine;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(mine));
+  return mine != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // D[tmem] (+)= A[smem] B[smem]
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(

@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
   uint8_t* slots = base + W::QB;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.sq.group;
+  grid_next();
 
   // ---- the line of tiles and this CTA's part of it (as in attend_kernels.cu)
   uint32_t* sums = reinterpret_cast<uint32_t*>(slots);  // before any copy
@@ -210,8 +211,8 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
 
   if (warp >= W::COPY_WARP && warp < W::MMA_WARP) {
     // ------------------------------------------------------------ copies --
-    // Registers: 512 threads start with 128 each, 65536 in all; 256 x 184 of
-    // softmax + 128 x 80 here + 128 x 64 = 65536.
+    // Registers: 512 threads start with 128 each, 65536 in all; 256 x 176 of
+    // softmax + 128 x 80 here + 128 x 80 = 65536.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int ct = tid - W::COPY_WARP * 32;
     uint32_t n_slot = 0, n_seg = 0, n_tile = 0;  // slots, segments, key tiles so far
@@ -382,72 +383,153 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
     cp_wait<0>();
   } else if (warp >= W::MMA_WARP) {
     // ---------------------------------------------------------- products --
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == W::MMA_WARP && lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == W::MMA_WARP) {
       constexpr uint32_t id_qk = tc::instr_desc(BF, false, 128, kKeys), id_pv = tc::instr_desc(BF, true, 128, D);
-      uint32_t n_slot = 0, n_seg = 0;
-      uint32_t done[2] = {0, 0}, seen[2] = {0, 0};  // items of each stream, and segments with items, before this one
+      // The tensor pipe runs dry while this warp does anything else, so the
+      // loop is kept short: ring places move by addition, a slot is waited
+      // for once.
+      uint32_t at = 0, at_par = 0;  // slot of the segment's first tile and its parity
+      uint32_t n_seg = 0;
+      uint32_t p_par[2] = {0, 0}, o_par[2] = {0, 0}, o_used = 0;
       const uint64_t q_desc = tc::smem_desc(smem_u32(q_tile), 16), k_desc = tc::smem_desc(smem_u32(slots), 16),
                      v_desc = tc::smem_desc(smem_u32(slots), HALF);
+      const uint32_t tm = tc::uniform(tmem);
+      auto commit = [&](uint64_t* bar) {
+        if (tc::elect()) tc::commit(bar);
+      };
       uint32_t t = t0;
       bool ok = true;
       while (ok && t < t1) {
         Part g;
         if (!part_at(t, g)) break;
-        ok = wait(&sh.q_full, n_seg & 1);
-        if (!ok) break;
-        const int items = MT * g.n;
-        auto slot_of = [&](int s) { return (n_slot + (uint32_t)s) % W::NS; };
-        auto full = [&](int s) { return wait(&sh.full[slot_of(s)], ((n_slot + (uint32_t)s) / W::NS) & 1); };
-        auto scores = [&](int j) {  // S of item j of stream j & 1
-          const uint32_t s = j & 1;
-          const int ks = k_slot(MT == 2 ? j >> 1 : j);
-          if (!full(ks)) return false;
-          tc::fence_after();
-          const uint64_t qa = q_desc + (MT == 2 ? s * (uint32_t)(HB * HALF >> 4) : 0u);
-          const uint64_t ka = k_desc + slot_of(ks) * (uint32_t)(W::SLOT >> 4);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            constexpr int STEP = 32 >> 4;
-            const int o = (k >> 2) * (HALF >> 4) + (k & 3) * STEP;
-            tc::mma_ss(tmem + s * kKeys, qa + o, ka + o, id_qk, k > 0);
+        const int n = (int)tc::uniform((uint32_t)g.n);
+        // a place of the ring: slot and the parity of its use
+        struct Place {
+          uint32_t st, par;
+        };
+        auto step = [&](Place& x, uint32_t by) {
+          x.st += by;
+          if (x.st >= (uint32_t)W::NS) {
+            x.st -= W::NS;
+            x.par ^= 1;
           }
-          tc::commit(&sh.s_full[s]);
-          if (MT == 1 || s == 1) tc::commit(&sh.empty[slot_of(ks)]);
-          if (j == items - 1) tc::commit(&sh.q_empty);
+        };
+        Place first{at, at_par};
+        auto full = [&](const Place& x) { return __all_sync(0xffffffffu, wait(&sh.full[x.st], x.par)) != 0; };
+        auto qk = [&](uint32_t s, const Place& k) {  // scores of stream s with the K tile of a place
+          const uint64_t qa = q_desc + (MT == 2 ? s * (uint32_t)(HB * HALF >> 4) : 0u);
+          const uint64_t ka = k_desc + tc::uniform(k.st) * (uint32_t)(W::SLOT >> 4);
+          if (tc::elect()) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const int o = (i >> 2) * (HALF >> 4) + (i & 3) * (32 >> 4);
+              tc::mma_ss(tm + s * kKeys, qa + o, ka + o, id_qk, i > 0);
+            }
+            tc::commit(&sh.s_full[s]);
+          }
+        };
+        auto pv = [&](uint32_t s, const Place& v, bool add) {
+          const uint64_t va = v_desc + tc::uniform(v.st) * (uint32_t)(W::SLOT >> 4);
+          if (tc::elect()) {
+#pragma unroll
+            for (int i = 0; i < kKeys / 16; ++i)
+              tc::mma_ts(tm + 2 * kKeys + s * D, tm + s * kKeys + i * 8, va + i * (2048 >> 4), id_pv, add || i > 0);
+            tc::commit(&sh.pv_done[s]);
+          }
+        };
+        // weights of a stream are there, and before a segment's first product
+        // its output has been read
+        auto weights = [&](uint32_t s, bool first_item) {
+          if (first_item && ((o_used >> s) & 1)) {
+            if (!__all_sync(0xffffffffu, wait(&sh.o_empty[s], o_par[s]))) return false;
+            o_par[s] ^= 1;
+          }
+          if (!__all_sync(0xffffffffu, wait(&sh.p_full[s], p_par[s]))) return false;
+          p_par[s] ^= 1;
+          tc::fence_after();
           return true;
         };
-        ok = scores(0) && (items < 2 || scores(1));
-        for (int j = 0; ok && j < items; ++j) {
-          const uint32_t s = j & 1;
-          const int i = j >> 1;  // local item of the stream
-          const int vs = v_slot(MT == 2 ? i : j, g.n);
-          if (i == 0 && done[s]) ok = wait(&sh.o_empty[s], (seen[s] - 1) & 1);
-          ok = ok && full(vs) && wait(&sh.p_full[s], (done[s] + (uint32_t)i) & 1);
-          if (!ok) break;
-          tc::fence_after();
-          const uint64_t va = v_desc + slot_of(vs) * (uint32_t)(W::SLOT >> 4);
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            tc::mma_ts(tmem + 2 * kKeys + s * D, tmem + s * kKeys + k * 8, va + k * (2048 >> 4), id_pv, i > 0 || k > 0);
-          tc::commit(&sh.pv_done[s]);
-          if (MT == 1 || s == 1) tc::commit(&sh.empty[slot_of(vs)]);
-          if (j + 2 < items) ok = scores(j + 2);
+        ok = __all_sync(0xffffffffu, wait(&sh.q_full, n_seg & 1)) && full(first);
+        if (!ok) break;
+        tc::fence_after();
+        if (MT == 2) {
+          Place k = first, v = first;
+          step(v, 1);
+          qk(0, k);
+          qk(1, k);
+          commit(&sh.empty[k.st]);
+          if (n == 1) commit(&sh.q_empty);
+          for (int i = 0; i < n; ++i) {
+            const bool more = i + 1 < n;
+            step(k, 2);
+            ok = full(v) && weights(0, i == 0);
+            if (!ok) break;
+            pv(0, v, i > 0);
+            if (more) {
+              ok = full(k);
+              if (!ok) break;
+              qk(0, k);
+            }
+            ok = weights(1, i == 0);
+            if (!ok) break;
+            pv(1, v, i > 0);
+            commit(&sh.empty[v.st]);
+            if (more) {
+              qk(1, k);
+              commit(&sh.empty[k.st]);
+              if (i + 2 == n) commit(&sh.q_empty);
+            }
+            step(v, 2);
+          }
+        } else {
+          // K0 K1 V0 K2 V1 ... V(n-1)
+          Place k = first, v = first;
+          qk(0, k);
+          commit(&sh.empty[k.st]);
+          if (n > 1) {
+            step(k, 1);
+            ok = full(k);
+            if (!ok) break;
+            qk(1, k);
+            commit(&sh.empty[k.st]);
+          }
+          if (n <= 2) commit(&sh.q_empty);
+          step(v, n > 1 ? 2 : 1);
+          for (int i = 0; i < n; ++i) {
+            const uint32_t s = i & 1;
+            ok = full(v) && weights(s, i < 2);
+            if (!ok) break;
+            pv(s, v, i > 1);
+            commit(&sh.empty[v.st]);
+            if (i + 2 < n) {
+              step(k, 2);
+              ok = full(k);
+              if (!ok) break;
+              qk(s, k);
+              commit(&sh.empty[k.st]);
+              if (i + 3 == n) commit(&sh.q_empty);
+            }
+            step(v, i + 2 < n ? 2 : 1);
+          }
         }
-        n_slot += 2 * (uint32_t)g.n;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          done[s] += (uint32_t)items_of(s, g.n);
-          seen[s] += items_of(s, g.n) > 0;
+        o_used |= MT == 2 || n > 1 ? 3u : 1u;
+        Place nx{at, at_par};
+        for (uint32_t left = 2 * (uint32_t)n; left > 0;) {  // 2 n places on
+          const uint32_t by = min(left, (uint32_t)W::NS);
+          step(nx, by);
+          left -= by;
         }
+        at = nx.st;
+        at_par = nx.par;
         ++n_seg;
-        t += (uint32_t)g.n;
+        t += (uint32_t)n;
       }
     }
     __syncwarp();
   } else {
     // ----------------------------------------------------------- softmax --
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int st = warp >> 2;                              // stream
     const int tile = MT == 2 ? st : 0;                     // row tile of the CTA
     const int r = (warp & 3) * 32 + lane;                  // row of it
@@ -700,37 +782,48 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
 }
 
 // Joins the parts of the segment that starts in CTA blockIdx.x and ends in a
-// later one, in the order of the CTAs. A lane is a row, a warp a column group.
+// later one, in the order of the CTAs. A lane is a row, a warp four columns.
 template <class T, int D, int MT>
 __global__ void __launch_bounds__(256) wide_join_kernel(const __grid_constant__ AttendLaunch p) {
-  constexpr int ROWS = 128 * MT;
+  constexpr int ROWS = 128 * MT, AHEAD = 8;  // parts loaded at a time
+  grid_wait();
   const int4 ds = p.desc[blockIdx.x];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = blockIdx.z * 8 + (threadIdx.x >> 5);
   const int i = blockIdx.y * 32 + lane;
   if (ds.x < 0 || blockIdx.y * 32 >= ds.z) return;
   const int c0 = blockIdx.x, c1 = ds.w;
   const float cexp = p.scale * kLog2e;
-  float mm = DARIC_NEG_INF;
-  for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, p.part_ml[(int64_t)(c * 2 + (c == c0)) * ROWS + i].x);
-  const float base = mm == DARIC_NEG_INF ? 0.f : mm;
-  float ll = 0.f;
-  constexpr int V = D / 32;  // groups of four columns of a warp
-  float4 o[V];
+  float mm = DARIC_NEG_INF, ll = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* part = reinterpret_cast<const float4*>(p.part);
+  for (int c = c0; c <= c1; c += AHEAD) {
+    float2 ml[AHEAD];
+    float4 x[AHEAD];
+    float top = mm;
 #pragma unroll
-  for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t s = c * 2 + (c == c0);
-    const float2 ml = p.part_ml[s * ROWS + i];
-    const float w = exp2_fast((ml.x - base) * cexp);
-    ll += ml.y * w;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float4 x = reinterpret_cast<const float4*>(p.part)[(s * (D / 4) + warp * V + v) * ROWS + i];
-      o[v].x += x.x * w;
-      o[v].y += x.y * w;
-      o[v].z += x.z * w;
-      o[v].w += x.w * w;
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t s = (c + k) * 2 + (c + k == c0);
+      ml[k] = c + k <= c1 ? p.part_ml[s * ROWS + i] : make_float2(DARIC_NEG_INF, 0.f);
+      x[k] = c + k <= c1 ? part[(s * (D / 4) + warp) * ROWS + i] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) top = fmaxf(top, ml[k].x);
+    const float base = top == DARIC_NEG_INF ? 0.f : top, a = exp2_fast((mm - base) * cexp);
+    ll *= a;
+    o.x *= a;
+    o.y *= a;
+    o.z *= a;
+    o.w *= a;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float w = exp2_fast((ml[k].x - base) * cexp);
+      ll = __fmaf_rn(ml[k].y, w, ll);
+      o.x = __fmaf_rn(x[k].x, w, o.x);
+      o.y = __fmaf_rn(x[k].y, w, o.y);
+      o.z = __fmaf_rn(x[k].z, w, o.z);
+      o.w = __fmaf_rn(x[k].w, w, o.w);
+    }
+    mm = top;
   }
   if (i >= ds.z) return;
   const int rt = ds.y >> 12, h = ds.y & 4095;
@@ -738,11 +831,8 @@ __global__ void __launch_bounds__(256) wide_join_kernel(const __grid_constant__ 
   const int64_t row = ds.x + pi / p.sq.group;
   const int head = h * p.sq.group + pi % p.sq.group;
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  uint8_t* out = p.out + row * p.out_row + (int64_t)head * p.out_head + warp * V * 8;
-#pragma unroll
-  for (int v = 0; v < V; ++v)
-    *reinterpret_cast<uint2*>(out + v * 8) =
-        make_uint2(Mma<T>::pack(o[v].x * inv, o[v].y * inv), Mma<T>::pack(o[v].z * inv, o[v].w * inv));
+  *reinterpret_cast<uint2*>(p.out + row * p.out_row + (int64_t)head * p.out_head + warp * 8) =
+      make_uint2(Mma<T>::pack(o.x * inv, o.y * inv), Mma<T>::pack(o.z * inv, o.w * inv));
   if (warp == 0 && p.lse) p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : __fmaf_rn(mm, p.scale, logf(ll));
 }
 
@@ -753,8 +843,7 @@ void wide_one(const AttendLaunch& p, int grid, cudaStream_t s) {
   allow_smem(wide_kernel<T, D, MT>, wide_smem<D, MT>(), done);
   wide_kernel<T, D, MT><<<grid, Wide<D, MT>::THREADS, wide_smem<D, MT>(), s>>>(p);
   DARIC_CUDA(cudaGetLastError());
-  wide_join_kernel<T, D, MT><<<dim3((unsigned)grid, 4 * MT), 256, 0, s>>>(p);
-  DARIC_CUDA(cudaGetLastError());
+  launch_after(wide_join_kernel<T, D, MT>, dim3((unsigned)grid, 4 * MT, D / 32), 256, s, p);
 }
 
 template <class T>
