@@ -24,7 +24,9 @@ from .cache_ops import CacheCopier, kv_dtype_code
 
 __all__ = ["tree_attention", "sparse_attention"]
 
-_workspace_bytes: dict[tuple, int] = {}
+_workspaces: dict[tuple, torch.Tensor] = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 def layer_tensor(copier: CacheCopier, layer_name: str) -> torch.Tensor:
@@ -34,20 +36,26 @@ def layer_tensor(copier: CacheCopier, layer_name: str) -> torch.Tensor:
     return kv
 
 
-def check_rows(q: torch.Tensor, name: str = "q") -> None:
-    if not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
-        raise RuntimeError(f"{name} must be a CUDA [rows, heads, head_dim] tensor with unit last stride")
+def kv_heads_of(kv: torch.Tensor) -> int:
+    return kv.shape[3] if kv.dim() == 5 else kv.shape[1] if kv.dim() == 4 else -1
+
+
+def check_rows(q: torch.Tensor, dev: torch.device, dtype: torch.dtype) -> None:
+    if q.device != dev or q.dtype != dtype:
+        raise RuntimeError(f"q must be {dtype} on {dev} like the KV cache, got {q.dtype} on {q.device}")
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise RuntimeError("q must be a [rows, heads, head_dim] tensor with unit last stride")
 
 
 def check_batch(dev: torch.device, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: Optional[torch.Tensor]) -> int:
     """Checks the batch's tables; returns the number of sequences."""
-    if block_table.device != dev or block_table.dtype != torch.int32 or block_table.dim() != 2 or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev or \
+            (block_table.stride(1) != 1 and block_table.shape[1] > 1):
         raise RuntimeError("block_table must be an int32 [sequences, pages] matrix with unit column stride on the cache's device")
     n = block_table.shape[0]
-    if seq_lens.device != dev or seq_lens.dtype != torch.int32 or seq_lens.shape != (n,) or not seq_lens.is_contiguous():
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (n,) or seq_lens.device != dev or not seq_lens.is_contiguous():
         raise RuntimeError("seq_lens must be a contiguous int32 vector, one entry per sequence, on the cache's device")
-    if cu_q is not None and (cu_q.device != dev or cu_q.dtype != torch.int32 or cu_q.shape != (n + 1,)
+    if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.shape != (n + 1,) or cu_q.device != dev
                              or not cu_q.is_contiguous()):
         raise RuntimeError("cu_q must be a contiguous int32 vector of sequences + 1 entries on the cache's device")
     return n
@@ -70,53 +78,51 @@ def check_lse(lse: torch.Tensor, q: torch.Tensor) -> None:
 
 
 class on_stream:
-    """Allocations of a call are made on the stream that uses them, and the
-    caller's tensors are kept from reuse until that stream is done with them."""
+    """A call on the stream of the given handle: allocations are made on the
+    stream that uses them, and the caller's tensors are kept from reuse until
+    that stream is done with them."""
 
     def __init__(self, stream: int, dev: torch.device, *tensors):
-        self.ctx = None
-        if stream:
-            ext = torch.cuda.ExternalStream(stream, device=dev)
-            self.ctx = torch.cuda.stream(ext)
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(ext)
-            self.ptr = int(stream)
-        else:
-            self.ptr = torch.cuda.current_stream(dev).cuda_stream
+        ext = torch.cuda.ExternalStream(stream, device=dev)
+        self.ctx = torch.cuda.stream(ext)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(ext)
 
-    def __enter__(self) -> int:
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return self.ptr
+    def __enter__(self):
+        return self.ctx.__enter__()
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
+        return self.ctx.__exit__(*exc)
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _attend_workspace(dev: torch.device, head_dim: int) -> torch.Tensor:
-    key = (dev.index, head_dim)
-    n = _workspace_bytes.get(key)
-    if n is None:
+def _attend_workspace(dev: torch.device, head_dim: int, stream: int, kept: bool) -> torch.Tensor:
+    """Workspace of an attention call. Calls on one stream follow each other,
+    so they share one that is kept; a captured call has its own, which belongs
+    to its graph, and so has one on a stream given by its handle."""
+    kept = kept and not _capturing()
+    key = (dev.index, head_dim, stream)
+    ws = _workspaces.get(key) if kept else None
+    if ws is None:
         v = C.c_int64(0)
         check(_lib.load().daric_attend_workspace(dev.index, head_dim, C.byref(v)))
-        n = _workspace_bytes[key] = v.value
-    return torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = torch.empty(v.value, dtype=torch.uint8, device=dev)
+        if kept:
+            _workspaces[key] = ws
+    return ws
 
 
 def _outputs(q, out, lse):
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.device != q.device or out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1:
         raise RuntimeError("out must be like q: same shape, dtype and device, unit last stride")
     if lse is None:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     else:
         check_lse(lse, q)
     return out, lse
@@ -141,25 +147,32 @@ def tree_attention(copier: CacheCopier, layer_name: str, q: torch.Tensor, block_
     log of the sum of exp of the scaled logits). A row that sees nothing gets
     out 0 and lse -inf. Rows outside every sequence are not written."""
     kv = layer_tensor(copier, layer_name)
-    check_rows(q)
     dev = kv.device
-    if q.device != dev or q.dtype != kv.dtype:
-        raise RuntimeError(f"q must be {kv.dtype} on {dev} like the KV cache, got {q.dtype} on {q.device}")
+    check_rows(q, dev, kv.dtype)
     n = check_batch(dev, block_table, seq_lens, cu_q)
     rows, heads, dim = q.shape
     words = check_mask(tree_mask, rows, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    with on_stream(stream, dev, q, block_table, seq_lens, cu_q, tree_mask, out, lse) as s:
-        out, lse = _outputs(q, out, lse)
-        if n == 0 or rows == 0:
-            return out, lse
-        ws = _attend_workspace(dev, dim)
-        check(_lib.load().daric_copier_tree_attention(
-            copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
-            heads, dim, block_table.data_ptr(), block_table.stride(0), n, block_table.shape[1], seq_lens.data_ptr(),
-            _ptr(cu_q), _ptr(tree_mask), words, scale, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
-            lse.stride(0), ws.data_ptr(), ws.numel(), dev.index, s))
+    if stream:
+        with on_stream(stream, dev, q, block_table, seq_lens, cu_q, tree_mask, out, lse):
+            return _tree(copier, layer_name, kv, q, block_table, seq_lens, cu_q, tree_mask, words, n, scale, out, lse, False)
+    return _tree(copier, layer_name, kv, q, block_table, seq_lens, cu_q, tree_mask, words, n, scale, out, lse, True)
+
+
+def _tree(copier, layer_name, kv, q, block_table, seq_lens, cu_q, tree_mask, words, n, scale, out, lse, kept):
+    out, lse = _outputs(q, out, lse)
+    rows, heads, dim = q.shape
+    if n == 0 or rows == 0:
+        return out, lse
+    dev = kv.device
+    s = _raw_stream(dev.index)
+    ws = _attend_workspace(dev, dim, s, kept)
+    check(_lib.load().daric_copier_tree_attention(
+        copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
+        heads, dim, block_table.data_ptr(), block_table.stride(0), n, block_table.shape[1], seq_lens.data_ptr(),
+        _ptr(cu_q), _ptr(tree_mask), words, scale, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+        lse.stride(0), ws.data_ptr(), ws.numel(), dev.index, s))
     return out, lse
 
 
@@ -176,28 +189,35 @@ def sparse_attention(copier: CacheCopier, layer_name: str, q: torch.Tensor, page
     A row sees the listed positions up to its own. The rest is as in
     :func:`tree_attention` (without a mask)."""
     kv = layer_tensor(copier, layer_name)
-    check_rows(q)
     dev = kv.device
-    if q.device != dev or q.dtype != kv.dtype:
-        raise RuntimeError(f"q must be {kv.dtype} on {dev} like the KV cache, got {q.dtype} on {q.device}")
+    check_rows(q, dev, kv.dtype)
     n = check_batch(dev, block_table, seq_lens, cu_q)
     rows, heads, dim = q.shape
     if pages.device != dev or pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[0] != rows or \
             (pages.shape[2] > 1 and pages.stride(2) != 1):
         raise RuntimeError("pages must be an int32 [rows, KV heads, k] tensor with unit last stride on the cache's device")
-    kv_heads = kv.shape[1] if kv.dim() == 4 else kv.shape[3] if kv.dim() == 5 else -1
+    kv_heads = kv_heads_of(kv)
     if pages.shape[1] != kv_heads:
         raise RuntimeError(f"pages must list pages for each of the {kv_heads} KV heads, got {pages.shape[1]}")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    with on_stream(stream, dev, q, pages, block_table, seq_lens, cu_q, out, lse) as s:
-        out, lse = _outputs(q, out, lse)
-        if n == 0 or rows == 0:
-            return out, lse
-        ws = _attend_workspace(dev, dim)
-        check(_lib.load().daric_copier_sparse_attention(
-            copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
-            heads, dim, pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[2], block_table.data_ptr(),
-            block_table.stride(0), n, block_table.shape[1], seq_lens.data_ptr(), _ptr(cu_q), scale, out.data_ptr(),
-            out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0), ws.data_ptr(), ws.numel(), dev.index, s))
+    if stream:
+        with on_stream(stream, dev, q, pages, block_table, seq_lens, cu_q, out, lse):
+            return _sparse(copier, layer_name, kv, q, pages, block_table, seq_lens, cu_q, n, scale, out, lse, False)
+    return _sparse(copier, layer_name, kv, q, pages, block_table, seq_lens, cu_q, n, scale, out, lse, True)
+
+
+def _sparse(copier, layer_name, kv, q, pages, block_table, seq_lens, cu_q, n, scale, out, lse, kept):
+    out, lse = _outputs(q, out, lse)
+    rows, heads, dim = q.shape
+    if n == 0 or rows == 0:
+        return out, lse
+    dev = kv.device
+    s = _raw_stream(dev.index)
+    ws = _attend_workspace(dev, dim, s, kept)
+    check(_lib.load().daric_copier_sparse_attention(
+        copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
+        heads, dim, pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[2], block_table.data_ptr(),
+        block_table.stride(0), n, block_table.shape[1], seq_lens.data_ptr(), _ptr(cu_q), scale, out.data_ptr(),
+        out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0), ws.data_ptr(), ws.numel(), dev.index, s))
     return out, lse

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .attend import check_batch, check_rows, layer_tensor, on_stream, _ptr
+from .attend import check_batch, check_rows, layer_tensor, on_stream, _ptr, _raw_stream
 from .cache_ops import CacheCopier, kv_dtype_code
 
 __all__ = ["new_bounds", "page_bounds", "select_pages"]
@@ -56,13 +56,16 @@ def page_bounds(copier: CacheCopier, layer_name: str, block_table: torch.Tensor,
     if bounds is not None and (bounds.device != dev or bounds.dtype != kv.dtype
                                or bounds.shape != (nb, heads, 2, dim) or not bounds.is_contiguous()):
         raise RuntimeError(f"bounds must be a contiguous {kv.dtype} [{nb}, {heads}, 2, {dim}] tensor on {dev}")
-    with on_stream(stream, dev, block_table, seq_lens, bounds, start) as s:
-        if bounds is None:
-            bounds = new_bounds(copier, layer_name)
-        if n and block_table.shape[1]:
-            check(_lib.load().daric_copier_page_bounds(
-                copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), block_table.data_ptr(), block_table.stride(0),
-                n, block_table.shape[1], seq_lens.data_ptr(), _ptr(start), bounds.data_ptr(), dev.index, s))
+    if stream:
+        with on_stream(stream, dev, block_table, seq_lens, bounds, start):
+            return page_bounds(copier, layer_name, block_table, seq_lens, bounds, start=start)
+    if bounds is None:
+        bounds = new_bounds(copier, layer_name)
+    if n and block_table.shape[1]:
+        check(_lib.load().daric_copier_page_bounds(
+            copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), block_table.data_ptr(), block_table.stride(0), n,
+            block_table.shape[1], seq_lens.data_ptr(), _ptr(start), bounds.data_ptr(), dev.index,
+            _raw_stream(dev.index)))
     return bounds
 
 
@@ -78,8 +81,10 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     highest first, ties to the lower page. The order is that of the score in
     exact arithmetic, whatever the rounding of the fast pass. NaN ranks
     highest. Rows outside every sequence are not written."""
-    check_rows(q)
     dev = q.device
+    if not q.is_cuda:
+        raise RuntimeError("q must be a CUDA tensor")
+    check_rows(q, dev, q.dtype)
     n = check_batch(dev, block_table, seq_lens, cu_q)
     if bounds.device != dev or bounds.dtype != q.dtype or bounds.dim() != 4 or bounds.shape[2] != 2 or \
             bounds.shape[3] != q.shape[2] or not bounds.is_contiguous():
@@ -90,16 +95,19 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     if out is not None and (out.device != dev or out.dtype != torch.int32 or out.shape != (rows, kv_heads, k)
                             or not out.is_contiguous()):
         raise RuntimeError(f"out must be a contiguous int32 [{rows}, {kv_heads}, {k}] tensor on {dev}")
+    if stream:
+        with on_stream(stream, dev, q, bounds, block_table, seq_lens, cu_q, out):
+            return select_pages(q, bounds, block_table, seq_lens, k, block_size, cu_q=cu_q, first=first, last=last, out=out)
+    if out is None:
+        out = q.new_empty((rows, kv_heads, max(k, 0)), dtype=torch.int32)
+    if n == 0 or rows == 0:
+        return out
     cols = block_table.shape[1]
-    with on_stream(stream, dev, q, bounds, block_table, seq_lens, cu_q, out) as s:
-        if out is None:
-            out = torch.empty((rows, kv_heads, max(k, 0)), dtype=torch.int32, device=dev)
-        if n == 0 or rows == 0:
-            return out
-        words = rows * kv_heads * (cols + (cols + 511) // 512)
-        ws = torch.empty(max(words, 1), dtype=torch.int32, device=dev)
-        check(_lib.load().daric_select_pages(
-            q.data_ptr(), kv_dtype_code(q.dtype), q.stride(0), q.stride(1), rows, heads, dim, bounds.data_ptr(), nb,
-            kv_heads, block_table.data_ptr(), block_table.stride(0), n, cols, seq_lens.data_ptr(), _ptr(cu_q),
-            int(block_size), k, int(first), int(last), out.data_ptr(), ws.data_ptr(), ws.numel() * 4, dev.index, s))
+    words = rows * kv_heads * (cols + (cols + 511) // 512)
+    ws = q.new_empty(max(words, 1), dtype=torch.int32)
+    check(_lib.load().daric_select_pages(
+        q.data_ptr(), kv_dtype_code(q.dtype), q.stride(0), q.stride(1), rows, heads, dim, bounds.data_ptr(), nb,
+        kv_heads, block_table.data_ptr(), block_table.stride(0), n, cols, seq_lens.data_ptr(), _ptr(cu_q),
+        int(block_size), k, int(first), int(last), out.data_ptr(), ws.data_ptr(), words * 4, dev.index,
+        _raw_stream(dev.index)))
     return out

@@ -386,7 +386,7 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
     DARIC_CHECK(copier, "copier is NULL");
     DARIC_CHECK(mode == DARIC_ROPE_NONE || mode == DARIC_ROPE_FLEXIBLE, "compact: mode must be NONE or FLEXIBLE");
     if (num_layers <= 0 || num_segs <= 0) return;
-    DARIC_CHECK(layer_names && idx && count && out_off && seg_cap && seg_blk_off, "NULL argument");
+    DARIC_CHECK(layer_names && idx && count && out_off && seg_cap, "NULL argument");
     DARIC_CHECK(block_table != nullptr, "block_table is NULL");
     std::vector<LayerRef> all;
     for (int64_t l = 0; l < num_layers; ++l) all.push_back(layer_ref(copier, layer_names[l]));
@@ -448,7 +448,7 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
     p.table_row = A.table_row;
     p.max_pos = A.max_pos;
     for (int64_t s = 0; s < num_segs; ++s) {
-      DARIC_CHECK(out_off[s] >= 0 && seg_cap[s] >= 0 && seg_blk_off[s] >= 0 && (!dst_start || dst_start[s] >= 0),
+      DARIC_CHECK(out_off[s] >= 0 && seg_cap[s] >= 0 && (!seg_blk_off || seg_blk_off[s] >= 0) && (!dst_start || dst_start[s] >= 0),
                   "negative segment field at segment " + std::to_string(s));
       DARIC_CHECK(out_off[s] + seg_cap[s] <= idx_row || lists == 1, "segment " + std::to_string(s) + " exceeds the selection's row");
       DARIC_CHECK(seg_cap[s] + (dst_start ? dst_start[s] : 0) <= INT32_MAX, "positions exceed int32");
@@ -464,7 +464,7 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
       for (int64_t s0 = 0; s0 < num_segs; s0 += kCompactSegs) {
         p.num_segs = (int32_t)std::min<int64_t>(kCompactSegs, num_segs - s0);
         for (int s = 0; s < p.num_segs; ++s)
-          p.segs[s] = CompactSeg{seg_blk_off[s0 + s], out_off[s0 + s], (int32_t)seg_cap[s0 + s],
+          p.segs[s] = CompactSeg{seg_blk_off ? seg_blk_off[s0 + s] : 0, out_off[s0 + s], (int32_t)seg_cap[s0 + s],
                                  (int32_t)(dst_start ? dst_start[s0 + s] : 0), (int32_t)(s0 + s)};
         launch_compact(p, kv_dtype, A.tab_dtype, es, di.sm_count, (cudaStream_t)stream);
       }

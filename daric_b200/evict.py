@@ -19,7 +19,8 @@ import torch
 
 from . import _lib
 from ._lib import check, i64, names_array
-from .attend import check_batch, check_lse, check_mask, check_rows, layer_tensor, on_stream, _ptr
+from .attend import (check_batch, check_lse, check_mask, check_rows, kv_heads_of, layer_tensor, on_stream, _ptr,
+                     _raw_stream)
 from .cache_ops import CacheCopier, kv_dtype_code, mode_code
 from .select import Selection
 
@@ -43,16 +44,14 @@ def attention_scores(copier: CacheCopier, layer_name: str, q: torch.Tensor, bloc
     here. Rows with lse -inf add nothing. The sums have one fixed order.
     Returns ``scores``."""
     kv = layer_tensor(copier, layer_name)
-    check_rows(q)
     dev = kv.device
-    if q.device != dev or q.dtype != kv.dtype:
-        raise RuntimeError(f"q must be {kv.dtype} on {dev} like the KV cache, got {q.dtype} on {q.device}")
+    check_rows(q, dev, kv.dtype)
     n = check_batch(dev, block_table, seq_lens, cu_q)
     rows, heads, dim = q.shape
     words = check_mask(tree_mask, rows, dev)
     if lse is not None:
         check_lse(lse, q)
-    kv_heads = kv.shape[1] if kv.dim() == 4 else kv.shape[3] if kv.dim() == 5 else -1
+    kv_heads = kv_heads_of(kv)
     if scores.device != dev or scores.dtype != torch.float32 or scores.dim() != 2 or scores.shape[0] != kv_heads or \
             (scores.shape[1] > 1 and scores.stride(1) != 1):
         raise RuntimeError(f"scores must be a float32 [{kv_heads}, columns] matrix with unit column stride on {dev}")
@@ -61,20 +60,23 @@ def attention_scores(copier: CacheCopier, layer_name: str, q: torch.Tensor, bloc
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     cols = block_table.shape[1]
-    with on_stream(stream, dev, q, block_table, seq_lens, scores, col_off, cu_q, tree_mask, lse) as s:
-        if n == 0 or cols == 0:
-            return scores
-        ws = None
-        if lse is None and rows:
-            block = kv.shape[2]
-            splits = (cols * block + 255) // 256
-            ws = torch.empty(rows * heads * (splits * 2 + 1) + 4, dtype=torch.float32, device=dev)
-        check(_lib.load().daric_copier_attention_scores(
-            copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
-            heads, dim, block_table.data_ptr(), block_table.stride(0), n, cols, seq_lens.data_ptr(), _ptr(cu_q),
-            _ptr(tree_mask), words, _ptr(lse), 0 if lse is None else lse.stride(0), scale, scores.data_ptr(),
-            scores.stride(0), scores.shape[1], col_off.data_ptr(), int(bool(accumulate)), _ptr(ws),
-            0 if ws is None else ws.numel() * 4, dev.index, s))
+    if stream:
+        with on_stream(stream, dev, q, block_table, seq_lens, scores, col_off, cu_q, tree_mask, lse):
+            return attention_scores(copier, layer_name, q, block_table, seq_lens, scores, col_off, cu_q=cu_q,
+                                    tree_mask=tree_mask, lse=lse, scale=scale, accumulate=accumulate)
+    if n == 0 or cols == 0:
+        return scores
+    ws, ws_bytes = None, 0
+    if lse is None and rows:
+        splits = (cols * kv.shape[2] + 255) // 256
+        ws = q.new_empty(rows * heads * (splits * 2 + 1) + 4, dtype=torch.float32)
+        ws_bytes = ws.numel() * 4
+    check(_lib.load().daric_copier_attention_scores(
+        copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
+        heads, dim, block_table.data_ptr(), block_table.stride(0), n, cols, seq_lens.data_ptr(), _ptr(cu_q),
+        _ptr(tree_mask), words, _ptr(lse), 0 if lse is None else lse.stride(0), scale, scores.data_ptr(),
+        scores.stride(0), scores.shape[1], col_off.data_ptr(), 1 if accumulate else 0, _ptr(ws), ws_bytes, dev.index,
+        _raw_stream(dev.index)))
     return scores
 
 
@@ -99,29 +101,33 @@ def compact(copier: CacheCopier, layer_names: Sequence[str], keep: Selection, bl
     names = list(layer_names)
     if not names or keep.idx.numel() == 0:
         return
+    layers = copier._layers
     kv = layer_tensor(copier, names[0])
-    dev = kv.device
+    dev, dtype = kv.device, kv.dtype
     for t, what in ((keep.idx, "keep.idx"), (keep.count, "keep.count")):
-        if t.device != dev or t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        if t.dtype != torch.int32 or t.dim() != 2 or t.device != dev or (t.shape[1] > 1 and t.stride(1) != 1):
             raise RuntimeError(f"{what} must be an int32 matrix with unit column stride on the cache's device")
-    if block_table.device != dev or block_table.dtype != torch.int32 or not block_table.is_contiguous():
+    if block_table.dtype != torch.int32 or block_table.device != dev or not block_table.is_contiguous():
         raise RuntimeError("block_table must be a contiguous CUDA int32 tensor on the cache's device")
-    for name in names:
-        if layer_tensor(copier, name).dtype != kv.dtype:
-            raise RuntimeError("compact: layers of one call must share the KV dtype")
+    if len(names) > 1 and any(name in layers and layers[name].dtype != dtype for name in names):
+        raise RuntimeError("compact: layers of one call must share the KV dtype")
     lists, width = keep.idx.shape
     nseg = keep.count.shape[1]
     off, offp = i64(keep.out_off)
     if keep.count.shape[0] != lists or len(off) != nseg:
         raise RuntimeError("keep.count and keep.out_off must have one entry per row and segment")
-    ends = np.append(off[1:], width)
-    cap, capp = i64(ends - off)
-    blk, blkp = i64(seg_blk_off if seg_blk_off is not None else [0] * nseg)
-    dst, dstp = i64(dst_start if dst_start is not None else [0] * nseg)
-    if len(blk) != nseg or len(dst) != nseg:
+    cap = np.empty(nseg, np.int64)  # room of each segment: up to the next one's entries
+    np.subtract(off[1:], off[:-1], out=cap[:-1])
+    cap[-1:] = width - off[-1:]
+    blk, blkp = (None, None) if seg_blk_off is None else i64(seg_blk_off)
+    dst, dstp = (None, None) if dst_start is None else i64(dst_start)
+    if (blk is not None and len(blk) != nseg) or (dst is not None and len(dst) != nseg):
         raise RuntimeError("seg_blk_off and dst_start must have one entry per segment")
-    with on_stream(stream, dev, keep.idx, keep.count, block_table) as s:
-        check(_lib.load().daric_copier_compact(
-            copier._h, len(names), names_array(names), kv_dtype_code(kv.dtype), mode_code(mode), lists,
-            int(bool(per_head)), keep.idx.data_ptr(), keep.idx.stride(0), keep.count.data_ptr(), keep.count.stride(0),
-            nseg, offp, capp, blkp, dstp, block_table.data_ptr(), block_table.numel(), dev.index, s))
+    if stream:
+        with on_stream(stream, dev, keep.idx, keep.count, block_table):
+            return compact(copier, names, keep, block_table, per_head=per_head, seg_blk_off=seg_blk_off,
+                           dst_start=dst_start, mode=mode)
+    check(_lib.load().daric_copier_compact(
+        copier._h, len(names), names_array(names), kv_dtype_code(dtype), mode_code(mode), lists, 1 if per_head else 0,
+        keep.idx.data_ptr(), keep.idx.stride(0), keep.count.data_ptr(), keep.count.stride(0), nseg, offp,
+        cap.ctypes.data, blkp, dstp, block_table.data_ptr(), block_table.numel(), dev.index, _raw_stream(dev.index)))

@@ -376,7 +376,7 @@ DARIC_API int daric_copier_attention_scores(daric_copier* copier, const char* la
 /* Kept tokens move to the front, in place: token n of list r and segment s,
  * idx[r*idx_row + out_off[s] + n] for n < min(count[r*count_row + s],
  * seg_cap[s]), goes to position dst_start[s] + n (NULL: n) of the block table
- * at block_table + seg_blk_off[s], K and V. lists = num_layers (or 1 for all
+ * at block_table + seg_blk_off[s] (NULL: 0), K and V. lists = num_layers (or 1 for all
  * layers), times the KV heads with per_head (row layer*heads + head).
  * Positions ascend and are >= dst_start[s] + n; an entry that breaks this is
  * left out (bit 4), as is one outside the block table (4), with a bad block
