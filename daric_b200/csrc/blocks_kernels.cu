@@ -77,10 +77,15 @@ __global__ void __launch_bounds__(kBoundWarps * 32) bounds_kernel(const __grid_c
   const int p0 = (int)fdiv((uint32_t)start, p.kv.page_div);
   const int pages = (s.len + bs - 1) / bs - p0;
   const int c = lane % CH, t0 = lane / CH;
-  for (int64_t w = (int64_t)blockIdx.x * kBoundWarps + warp; w < (int64_t)pages * H;
-       w += (int64_t)gridDim.x * kBoundWarps) {
+  const int32_t* trow = p.sq.table + (int64_t)b * p.sq.table_ld + p0;
+  const int64_t items = (int64_t)pages * H, stride = (int64_t)gridDim.x * kBoundWarps;
+  int nxt = 0;
+  if ((int64_t)blockIdx.x * kBoundWarps + warp < items)
+    nxt = ld_ahead(&trow[((int64_t)blockIdx.x * kBoundWarps + warp) / H]);
+  for (int64_t w = (int64_t)blockIdx.x * kBoundWarps + warp; w < items; w += stride) {
     const int pg = p0 + (int)(w / H), h = (int)(w % H);
-    const int blk = __ldg(&p.sq.table[(int64_t)b * p.sq.table_ld + pg]);
+    const int blk = nxt;
+    if (w + stride < items) nxt = ld_ahead(&trow[(w + stride) / H]);
     if (blk < 0 || blk >= p.kv.num_pages) {
       if (lane == 0) atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
       continue;
@@ -323,8 +328,9 @@ __global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, 
   extern __shared__ uint32_t dyn[];  // [bitmap words | staged keys]
   __shared__ uint32_t hist[kBins];
   __shared__ int sm[32];
-  __shared__ int s_digit, s_above, s_near;
-  __shared__ float s_e;
+  __shared__ int s_digit, s_above, s_near, s_in, s_count;
+  __shared__ uint32_t s_kth;
+  __shared__ float s_e, s_lo[32], s_hi[32];
   __shared__ int near_page[kNear];
   __shared__ unsigned long long near_key[kNear];
   const int n = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
@@ -345,7 +351,7 @@ __global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, 
   // eligible pages [e0, e1); the ones before and after are always taken
   const int e0 = p.first, e1 = P - p.last;
   const int kk = p.k - p.first - p.last;
-  if (tid == 0) s_near = 0;
+  if (tid == 0) s_near = s_in = 0;
   float mag = 0.f;
   for (int i = tid; i < (P + kScoreChunk - 1) / kScoreChunk; i += blockDim.x) mag = fmaxf(mag, p.mags[item * chunks + i]);
 #pragma unroll
@@ -364,10 +370,65 @@ __global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, 
   const float E = s_e;
 
   if (kk > 0) {
-    // k-th largest fp32 key: digits of 11, 11 and 10 bits
     uint32_t prefix = 0, mask = 0;
     int rem = kk;
-    for (int pass = 0; pass < 3; ++pass) {
+    // The k-th largest fp32 key. Scores of one row lie close together (their
+    // leading bits are the same), so they are first spread over bins of equal
+    // width between the smallest and the largest; the keys of the bin that
+    // holds the k-th are few and are ranked against each other.
+    bool found = false;
+    if (E < 1e38f) {  // all scores are finite then
+      float lo = __int_as_float(0x7f800000), hi = DARIC_NEG_INF;
+      for (int i = e0 + tid; i < e1; i += blockDim.x) {
+        const float v = value_of(key_at(i));
+        lo = fminf(lo, v);
+        hi = fmaxf(hi, v);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      for (int i = tid; i < kBins; i += blockDim.x) hist[i] = 0;
+      if (lane == 0) {
+        s_lo[warp] = lo;
+        s_hi[warp] = hi;
+      }
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      for (int w = 0; w < nw; ++w) {
+        lo = fminf(lo, s_lo[w]);
+        hi = fmaxf(hi, s_hi[w]);
+      }
+      // monotone in v: each step of it is
+      const float scale = (float)(kBins - 1) / fmaxf(hi - lo, 1e-30f);
+      auto bin_of = [&](float v) { return min(max((int)((v - lo) * scale), 0), kBins - 1); };
+      for (int i = e0 + tid; i < e1; i += blockDim.x) atomicAdd(&hist[bin_of(value_of(key_at(i)))], 1u);
+      __syncthreads();
+      find_digit(hist, kBins, rem, &s_digit, &s_above, sm);
+      const int bin = s_digit, left = rem - s_above;
+      if (hist[bin] <= (uint32_t)kNear) {
+        for (int i = e0 + tid; i < e1; i += blockDim.x) {
+          const uint32_t k = key_at(i);
+          if (bin_of(value_of(k)) == bin) near_key[atomicAdd(&s_count, 1)] = k;
+        }
+        __syncthreads();
+        const int n = s_count;
+        for (int i = tid; i < n; i += blockDim.x) {  // ties do not matter: one value is wanted
+          int above = 0, same = 0;
+          for (int j = 0; j < n; ++j) {
+            above += near_key[j] > near_key[i];
+            same += near_key[j] == near_key[i];
+          }
+          if (above < left && left <= above + same) s_kth = (uint32_t)near_key[i];
+        }
+        __syncthreads();
+        prefix = s_kth;
+        found = true;
+      }
+    }
+    // otherwise digits of 11, 11 and 10 bits
+    for (int pass = 0; pass < 3 && !found; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
       for (int i = tid; i < kBins; i += blockDim.x) hist[i] = 0;
       __syncthreads();
@@ -386,26 +447,26 @@ __global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, 
     const float t = value_of(prefix);
     const bool wide = !(E < 1e38f) || !(fabsf(t) < 1e38f);  // infinities or NaN about: settle all in 64 bits
     const float hi = t + 2.f * E, lo = t - 2.f * E;
-    int in = 0, near = 0;
-    for (int i0 = e0; i0 < e1; i0 += blockDim.x) {
+    for (int i0 = 0; i0 < words * 32; i0 += blockDim.x) {  // a warp: one word of the bitmap
       const int i = i0 + tid;
       bool sure = false, maybe = false;
-      if (i < e1) {
+      if (i >= e0 && i < e1) {
         const float v = value_of(key_at(i));
         sure = !wide && v > hi;
         maybe = wide || (v >= lo && v <= hi);
       }
-      if (sure) atomicOr(&taken[i >> 5], 1u << (i & 31));
+      const unsigned m = __ballot_sync(0xffffffffu, sure);
+      if (lane == 0 && i < words * 32) {
+        taken[i >> 5] = m;
+        if (m) atomicAdd(&s_in, __popc(m));
+      }
       if (maybe) {
         const int at = atomicAdd(&s_near, 1);
         if (at < kNear) near_page[at] = i;
       }
-      in += sure;
-      near += maybe;
     }
-    int n_in, n_near;
-    block_prefix(in, &n_in, sm);
-    block_prefix(near, &n_near, sm);
+    __syncthreads();
+    const int n_in = s_in, n_near = s_near;
     const int need = kk - n_in;  // of the candidates
     if (n_near <= need) {
       for (int i = tid; i < n_near && i < kNear; i += blockDim.x) atomicOr(&taken[near_page[i] >> 5], 1u << (near_page[i] & 31));
