@@ -103,7 +103,7 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     if n == 0 or rows == 0:
         return out
     cols = block_table.shape[1]
-    words = rows * kv_heads * (cols + (cols + 511) // 512)
+    words = rows * kv_heads * ((cols + 3) // 4 * 4 + (cols + 63) // 64)
     ws = q.new_empty(max(words, 1), dtype=torch.int32)
     check(_lib.load().daric_select_pages(
         q.data_ptr(), kv_dtype_code(q.dtype), q.stride(0), q.stride(1), rows, heads, dim, bounds.data_ptr(), nb,

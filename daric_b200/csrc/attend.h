@@ -97,11 +97,13 @@ struct SelectPagesLaunch {
   const uint8_t* bounds;  // [num_pages, heads, 2, head_dim]
   int32_t num_pages, heads, head_dim, page_size;
   int32_t k, first, last;
-  uint32_t* keys;         // workspace: [N, heads, table_cols] ordered scores
+  int32_t chunk, sm_count;  // pages a CTA scores
+  uint32_t* keys;         // workspace: [N, heads, keys_row] ordered scores
+  int32_t keys_row;       // table_cols, whole 16-byte vectors
   float* mags;            // workspace: [N, heads, chunks] largest sum of |q||bound| of a chunk of pages
   int32_t* out;           // [N, heads, k] contiguous
 };
-constexpr int kScoreChunk = 512;  // pages a CTA scores
+constexpr int kScoreChunk = 64;  // least pages a CTA scores
 void launch_select_pages(const SelectPagesLaunch& p, int dtype, cudaStream_t s);
 
 struct ScoresLaunch {

@@ -264,7 +264,7 @@ int daric_select_pages_workspace(int64_t num_rows, int64_t kv_heads, int64_t tab
     DARIC_CHECK(out_bytes, "out_bytes is NULL");
     DARIC_CHECK(num_rows >= 0 && kv_heads >= 1 && table_cols >= 1 && table_cols <= (1 << 20), "select_pages: sizes out of range");
     const int64_t items = num_rows * kv_heads;
-    *out_bytes = items * 4 * (table_cols + (table_cols + kScoreChunk - 1) / kScoreChunk) + 16;
+    *out_bytes = items * 4 * ((table_cols + 3) / 4 * 4 + (table_cols + kScoreChunk - 1) / kScoreChunk);
   });
 }
 
@@ -291,10 +291,11 @@ int daric_select_pages(const void* q, int kv_dtype, int64_t q_row, int64_t q_hea
     DARIC_CHECK(q && bounds && out, "NULL query, bounds or output");
     DARIC_CHECK(aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
     DARIC_CHECK((uintptr_t)bounds % 16 == 0, "bounds must be 16-byte aligned");
-    DARIC_CHECK(workspace && (uintptr_t)workspace % 4 == 0, "workspace must be a device buffer");
+    DARIC_CHECK(workspace && (uintptr_t)workspace % 16 == 0, "workspace must be a 16-byte aligned device buffer");
     const int64_t items = num_rows * kv_heads;
     const int64_t chunks = (table_cols + kScoreChunk - 1) / kScoreChunk;
-    DARIC_CHECK(items * 4 * (table_cols + chunks) <= workspace_bytes, "workspace is too small");
+    const int64_t keys_row = (table_cols + 3) / 4 * 4;
+    DARIC_CHECK(items * 4 * (keys_row + chunks) <= workspace_bytes, "workspace is too small");
     const DeviceInfo di = device_info(device);
     p.sq.err = di.err;
     p.q = (const uint8_t*)q;
@@ -305,11 +306,13 @@ int daric_select_pages(const void* q, int kv_dtype, int64_t q_row, int64_t q_hea
     p.heads = (int32_t)kv_heads;
     p.head_dim = (int32_t)head_dim;
     p.page_size = (int32_t)block_size;
+    p.sm_count = di.sm_count;
     p.k = (int32_t)k;
     p.first = (int32_t)first;
     p.last = (int32_t)last;
     p.keys = (uint32_t*)workspace;
-    p.mags = (float*)workspace + items * table_cols;
+    p.keys_row = (int32_t)keys_row;
+    p.mags = (float*)workspace + items * keys_row;
     p.out = out;
     OnDevice on(device);
     launch_select_pages(p, kv_dtype, (cudaStream_t)stream);

@@ -169,55 +169,128 @@ __device__ __forceinline__ uint32_t q_part(uint32_t w, bool maxima) {
   return a | (b << 16);
 }
 
-constexpr int kScoreWarps = 8;
+constexpr int kScoreWarps = 4;
+constexpr int kScoreStages = 3;
 
+// N pieces of 16 bytes, 64 bytes apart, to slots STEP bytes apart.
+template <int N, int STEP, int I = 0>
+__device__ __forceinline__ void copy_row(uint32_t dst, const uint8_t* src, int n) {
+  if constexpr (I < N) {
+    cp16_at<I * STEP, I * 64>(dst, src, n);
+    copy_row<N, STEP, I + 1>(dst, src, n);
+  }
+}
+
+// A warp scores 16 pages at a time, the minima and then the maxima, each a
+// stage of its threads' own ring slots (a thread copies the fragment pieces
+// that it multiplies). Four CTAs of four warps an SM keep the loads going.
 template <class T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const __grid_constant__ SelectPagesLaunch p) {
-  constexpr int KB = D / 16;  // 64-byte pieces of (mn, mx): 2 D elements of 2 bytes
+__global__ void __launch_bounds__(kScoreWarps * 32, D > 128 ? 2 : 4) page_score_kernel(const __grid_constant__ SelectPagesLaunch p) {
+  constexpr int KB = D / 32;  // 64-byte pieces of the minima (or maxima) of a page
+  constexpr int TH = kScoreWarps * 32, S = kScoreStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_mag[kScoreWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = blockIdx.x, h = blockIdx.z, chunk = blockIdx.y;
   const int g = lane >> 2, t = lane & 3;
-  __shared__ float s_mag[kScoreWarps];
   const RowView rv = row_view(p.sq, p.page_size, n);
-  if (rv.pages <= p.k || chunk * kScoreChunk >= rv.pages) return;  // every page is taken, or none is here
+  if (rv.pages <= p.k || chunk * p.chunk >= rv.pages) return;  // every page is taken, or none is here
   const int group = p.sq.group;
   const int32_t* trow = p.sq.table + (int64_t)rv.seq * p.sq.table_ld;
-  uint32_t* keys = p.keys + ((int64_t)n * p.heads + h) * p.sq.table_cols;
-  float mag = 0.f;
-  for (int it = 0; it < kScoreChunk / (kScoreWarps * 16); ++it) {
-    const int g0 = chunk * kScoreChunk + (it * kScoreWarps + warp) * 16;
-    if (g0 >= rv.pages) break;
-    // rows g and g + 8 of the tile: two pages
-    uint4 a[2][KB];
+  uint32_t* keys = p.keys + ((int64_t)n * p.heads + h) * p.keys_row;
+  const int first = chunk * p.chunk + warp * 16;
+  const int tiles = first >= rv.pages ? 0
+                                      : min(p.chunk / (kScoreWarps * 16),
+                                            (rv.pages - first + kScoreWarps * 16 - 1) / (kScoreWarps * 16));
+  uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;  // [stage][row][piece][thread]
+  int blk[2];  // pages g and g + 8 of the tile that is copied next
+  auto lookup = [&](int it) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int pg = g0 + g + 8 * r;
-      int blk = pg < rv.pages ? __ldg(&trow[pg]) : -1;
-      if (pg < rv.pages && (blk < 0 || blk >= p.num_pages)) {
-        atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
-        blk = -1;
-      }
-      const uint4* src = reinterpret_cast<const uint4*>(p.bounds + ((int64_t)max(blk, 0) * p.heads + h) * (4 * D)) + t;
-#pragma unroll
-      for (int k = 0; k < KB; ++k) a[r][k] = blk >= 0 ? __ldg(src + 4 * k) : make_uint4(0, 0, 0, 0);
+      const int pg = first + it * kScoreWarps * 16 + g + 8 * r;
+      blk[r] = it < tiles && pg < rv.pages ? ld_ahead(&trow[pg]) : -1;
     }
+  };
+  const uint8_t* src[2];
+  bool in[2];
+  auto issue = [&](int half, int st) {  // half 2 it: minima of tile it, half 2 it + 1: its maxima
+    if (half < 2 * tiles) {
+      if (!(half & 1)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          in[r] = blk[r] >= 0 && blk[r] < p.num_pages;
+          if (!in[r] && first + (half >> 1) * kScoreWarps * 16 + g + 8 * r < rv.pages) atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
+          src[r] = p.bounds + ((int64_t)(in[r] ? blk[r] : 0) * p.heads + h) * (4 * D) + t * 16;
+        }
+        lookup((half >> 1) + 1);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        copy_row<KB, TH * 16>(smem_u32(ring + (st * 2 + r) * KB * TH), src[r] + (half & 1) * 2 * D, in[r] ? 16 : 0);
+    }
+    cp_commit();
+  };
+  lookup(0);
+#pragma unroll
+  for (int k = 0; k < S - 1; ++k) issue(k, k);
+  // the parts of the first eight query heads that meet minima and maxima
+  uint4 w[2][KB];
+  auto query = [&](int q0) {
+    const bool real = q0 + g < group;
+    const uint4* qp = reinterpret_cast<const uint4*>(
+        p.q + (int64_t)n * p.q_row + (int64_t)(h * group + (real ? q0 + g : 0)) * p.q_head) + t;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      const uint4 v = real ? __ldg(qp + 4 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) w[m][k] = make_uint4(q_part(v.x, m), q_part(v.y, m), q_part(v.z, m), q_part(v.w, m));
+    }
+  };
+  query(0);
+  float mag = 0.f;
+  int st = 0;
+  for (int it = 0; it < tiles; ++it) {
     uint32_t best[2] = {0u, 0u};
+    // heads eight at a time; all of a page's bytes stay in the ring meanwhile
+    // only for the first eight, so more heads read them again from global
     for (int q0 = 0; q0 < group; q0 += 8) {
       float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      const bool real = q0 + g < group;
-      const uint4* qp = reinterpret_cast<const uint4*>(
-          p.q + (int64_t)n * p.q_row + (int64_t)(h * group + (real ? q0 + g : 0)) * p.q_head) + t;
+      if (group > 8) query(q0);
 #pragma unroll
-      for (int k = 0; k < KB; ++k) {
-        const bool maxima = k >= KB / 2;
-        uint4 w = real ? __ldg(qp + 4 * (k - (maxima ? KB / 2 : 0))) : make_uint4(0, 0, 0, 0);
-        w = make_uint4(q_part(w.x, maxima), q_part(w.y, maxima), q_part(w.z, maxima), q_part(w.w, maxima));
-        const uint4 u = a[0][k], v = a[1][k];
-        constexpr uint32_t M = 0x7fff7fffu;
-        { uint32_t f[4] = {u.x, v.x, u.y, v.y}; Mma<T>::run(x, f, w.x, w.y); }
-        { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x, f, w.z, w.w); }
-        { uint32_t f[4] = {u.x & M, v.x & M, u.y & M, v.y & M}; Mma<T>::run(y, f, w.x & M, w.y & M); }
-        { uint32_t f[4] = {u.z & M, v.z & M, u.w & M, v.w & M}; Mma<T>::run(y, f, w.z & M, w.w & M); }
+      for (int m = 0; m < 2; ++m) {
+        if (q0 == 0) {
+          issue(2 * it + m + S - 1, st == 0 ? S - 1 : st - 1);
+          cp_wait<S - 1>();
+        }
+        const uint4* a = ring + st * 2 * KB * TH;
+        const uint8_t* again[2] = {nullptr, nullptr};
+        if (q0 > 0) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int pg = first + it * kScoreWarps * 16 + g + 8 * r;
+            const int bk = pg < rv.pages ? __ldg(&trow[pg]) : -1;
+            if (bk >= 0 && bk < p.num_pages)
+              again[r] = p.bounds + ((int64_t)bk * p.heads + h) * (4 * D) + m * 2 * D + t * 16;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+          uint4 u, v;
+          if (q0 == 0) {
+            u = a[k * TH];
+            v = a[(KB + k) * TH];
+          } else {
+            u = again[0] ? __ldg(reinterpret_cast<const uint4*>(again[0] + k * 64)) : make_uint4(0, 0, 0, 0);
+            v = again[1] ? __ldg(reinterpret_cast<const uint4*>(again[1] + k * 64)) : make_uint4(0, 0, 0, 0);
+          }
+          const uint4 z = w[m][k];
+          constexpr uint32_t M = 0x7fff7fffu;
+          { uint32_t f[4] = {u.x, v.x, u.y, v.y}; Mma<T>::run(x, f, z.x, z.y); }
+          { uint32_t f[4] = {u.z, v.z, u.w, v.w}; Mma<T>::run(x, f, z.z, z.w); }
+          { uint32_t f[4] = {u.x & M, v.x & M, u.y & M, v.y & M}; Mma<T>::run(y, f, z.x & M, z.y & M); }
+          { uint32_t f[4] = {u.z & M, v.z & M, u.w & M, v.w & M}; Mma<T>::run(y, f, z.z & M, z.w & M); }
+        }
+        if (q0 == 0) st = st + 1 == S ? 0 : st + 1;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -227,20 +300,22 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const __gr
           mag = (y[e] <= mag) ? mag : (y[e] == y[e] ? y[e] : __int_as_float(0x7f800000));
         }
     }
+    if (group > 8) query(0);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
       best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
-      const int pg = g0 + g + 8 * r;
+      const int pg = first + it * kScoreWarps * 16 + g + 8 * r;
       if (t == 0 && pg < rv.pages) keys[pg] = best[r];
     }
   }
+  cp_wait<0>();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
   if (lane == 0) s_mag[warp] = mag;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kScoreWarps; ++w) mag = fmaxf(mag, s_mag[w]);
+    for (int i = 1; i < kScoreWarps; ++i) mag = fmaxf(mag, s_mag[i]);
     p.mags[((int64_t)n * p.heads + h) * gridDim.y + chunk] = mag;
   }
 }
@@ -299,32 +374,56 @@ __device__ __forceinline__ void find_digit(const uint32_t* hist, int bins, int r
   __syncthreads();
 }
 
-// Score of a page in 64 bits (all lanes of a warp call it with one page).
+// Score of a page in 64 bits (all lanes of a warp call it with one page):
+// four heads at a time, so that their sums go side by side.
 template <class T, int D>
 __device__ __forceinline__ unsigned long long exact_key(const SelectPagesLaunch& p, int n, int h, int blk) {
   const int lane = threadIdx.x & 31, group = p.sq.group;
   const uint16_t* bd = reinterpret_cast<const uint16_t*>(p.bounds + ((int64_t)max(blk, 0) * p.heads + h) * (4 * D));
+  uint16_t lo[D / 32], hi[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) {
+    lo[k] = blk >= 0 ? __ldg(&bd[lane + 32 * k]) : 0;
+    hi[k] = blk >= 0 ? __ldg(&bd[D + lane + 32 * k]) : 0;
+  }
   unsigned long long best = 0;
-  for (int e = 0; e < group; ++e) {
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + (int64_t)n * p.q_row + (int64_t)(h * group + e) * p.q_head);
-    double u = 0.0;
-    for (int d = lane; d < D; d += 32) {
-      const double qv = (double)Mma<T>::widen(__ldg(&q[d]));
-      const double lo = blk >= 0 ? (double)Mma<T>::widen(__ldg(&bd[d])) : 0.0;
-      const double hi = blk >= 0 ? (double)Mma<T>::widen(__ldg(&bd[D + d])) : 0.0;
-      u += (qv > 0.0 ? qv : 0.0) * hi + (qv < 0.0 ? qv : 0.0) * lo;
-      if (qv != qv) u = qv;
+  for (int e0 = 0; e0 < group; e0 += 4) {
+    uint16_t qw[4][D / 32];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k)
+        qw[e][k] = e0 + e < group ? __ldg(reinterpret_cast<const uint16_t*>(p.q + (int64_t)n * p.q_row +
+                                                                             (int64_t)(h * group + e0 + e) * p.q_head) +
+                                          lane + 32 * k)
+                                  : 0;
+    double u[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      const double l = (double)Mma<T>::widen(lo[k]), m = (double)Mma<T>::widen(hi[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const double qv = (double)Mma<T>::widen(qw[e][k]);
+        u[e] += (qv > 0.0 ? qv : 0.0) * m + (qv < 0.0 ? qv : 0.0) * l;
+        if (qv != qv) u[e] = qv;
+      }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    const unsigned long long k = key64_of(u);
-    best = k > best ? k : best;
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] += __shfl_xor_sync(0xffffffffu, u[e], o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e0 + e < group) {
+        const unsigned long long k = key64_of(u[e]);
+        best = k > best ? k : best;
+      }
   }
   return best;
 }
 
 template <class T, int D>
-__global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, int chunks, int staged) {
+__global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant__ SelectPagesLaunch p, int chunks, int staged) {
   extern __shared__ uint32_t dyn[];  // [bitmap words | staged keys]
   __shared__ uint32_t hist[kBins];
   __shared__ int sm[32];
@@ -343,22 +442,23 @@ __global__ void page_select_kernel(const __grid_constant__ SelectPagesLaunch p, 
     return;
   }
   const int64_t item = (int64_t)n * p.heads + h;
-  const uint32_t* gkeys = p.keys + item * p.sq.table_cols;
+  const uint32_t* gkeys = p.keys + item * p.keys_row;
   const int words = (P + 31) / 32;
   uint32_t* taken = dyn;
-  uint32_t* skeys = dyn + (p.sq.table_cols + 31) / 32;
+  uint32_t* skeys = dyn + ((p.sq.table_cols + 31) / 32 + 3) / 4 * 4;
   const int32_t* trow = p.sq.table + (int64_t)rv.seq * p.sq.table_ld;
   // eligible pages [e0, e1); the ones before and after are always taken
   const int e0 = p.first, e1 = P - p.last;
   const int kk = p.k - p.first - p.last;
   if (tid == 0) s_near = s_in = 0;
   float mag = 0.f;
-  for (int i = tid; i < (P + kScoreChunk - 1) / kScoreChunk; i += blockDim.x) mag = fmaxf(mag, p.mags[item * chunks + i]);
+  for (int i = tid; i < (P + p.chunk - 1) / p.chunk; i += blockDim.x) mag = fmaxf(mag, p.mags[item * chunks + i]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
   if (lane == 0) sm[warp] = __float_as_int(mag);
-  if (staged)
-    for (int i = tid; i < P; i += blockDim.x) skeys[i] = gkeys[i];
+  if (staged)  // rows of keys are whole 16-byte vectors
+    for (int i = tid; i < (P + 3) / 4; i += blockDim.x)
+      reinterpret_cast<uint4*>(skeys)[i] = __ldg(reinterpret_cast<const uint4*>(gkeys) + i);
   for (int i = tid; i < words; i += blockDim.x) taken[i] = 0;
   __syncthreads();
   if (tid == 0) {
@@ -580,17 +680,26 @@ void bounds_d(const BoundsLaunch& p, int sm_count, cudaStream_t s) {
 }
 
 template <class T, int D>
-void select_d(const SelectPagesLaunch& p, cudaStream_t s) {
-  const int chunks = (p.sq.table_cols + kScoreChunk - 1) / kScoreChunk;
+void select_d(const SelectPagesLaunch& p0, cudaStream_t s) {
+  SelectPagesLaunch p = p0;
+  // pages of a CTA: 512, fewer while that leaves less than four CTAs an SM
+  p.chunk = 512;
+  while (p.chunk > kScoreChunk &&
+         (int64_t)(p.sq.table_cols + p.chunk - 1) / p.chunk * p.sq.num_rows * p.heads < 4 * (int64_t)p.sm_count)
+    p.chunk /= 2;
+  const int chunks = (p.sq.table_cols + p.chunk - 1) / p.chunk;
   if (p.sq.table_cols > p.k) {
+    constexpr int bytes = kScoreStages * 2 * (D / 32) * kScoreWarps * 32 * 16;
+    static std::atomic<uint64_t> ready{0};
+    allow_smem(page_score_kernel<T, D>, bytes, ready);
     page_score_kernel<T, D>
-        <<<dim3((unsigned)p.sq.num_rows, (unsigned)chunks, (unsigned)p.heads), kScoreWarps * 32, 0, s>>>(p);
+        <<<dim3((unsigned)p.sq.num_rows, (unsigned)chunks, (unsigned)p.heads), kScoreWarps * 32, bytes, s>>>(p);
     DARIC_CUDA(cudaGetLastError());
   }
   // keys are staged in shared memory while they fit
-  const int words = (p.sq.table_cols + 31) / 32;
+  const int words = ((p.sq.table_cols + 31) / 32 + 3) / 4 * 4;
   const int staged = p.sq.table_cols <= 40960;
-  const int bytes = (words + (staged ? p.sq.table_cols : 0)) * 4;
+  const int bytes = (words + (staged ? p.keys_row : 0)) * 4;
   // a thread per eight keys, so that short tables keep many CTAs on an SM
   const int threads = std::min(1024, std::max(128, (p.sq.table_cols / 8 + 31) / 32 * 32));
   static std::atomic<uint64_t> done{0};

@@ -105,6 +105,13 @@ def test_long_sequences():
     check_select(bt, page_bounds(bt.copier, "l", bt.table, bt.seq_lens), 100)
 
 
+@pytest.mark.parametrize("bs,n,d", [(8, 66001, 128), (1, 41500, 64), (8, 66001, 256)])
+def test_very_long_sequences(bs, n, d):
+    """The widest selection CTAs, and more pages than their keys fit in shared memory."""
+    bt = Batch([n, 5], [1, 1], kvh=1, group=2, d=d, bs=bs, seed=31)
+    check_select(bt, page_bounds(bt.copier, "l", bt.table, bt.seq_lens), 64)
+
+
 def test_ties_go_to_the_lower_page():
     """All pages alike, and few different scores: thousands of candidates at the border."""
     bt = Batch([6000, 5000], [1, 1], kvh=2, group=3, d=64, seed=4)
