@@ -312,12 +312,21 @@ __device__ __forceinline__ void block_products(const KeyTile<D, M>& kt, const Qu
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[m][e] = 0.f;
   const uint8_t* q = qb.rows + (i + g) * QueryBlock<D>::PITCH + t * 16;
+  float y[M][4];  // every other piece: two shorter chains of products
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[m][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) {
     const uint4 w = *reinterpret_cast<const uint4*>(q + k * 64);
 #pragma unroll
-    for (int m = 0; m < M; ++m) products<T>(x[m], kt.a[2 * m][k], kt.a[2 * m + 1][k], w);
+    for (int m = 0; m < M; ++m) products<T>(k & 1 ? y[m] : x[m], kt.a[2 * m][k], kt.a[2 * m + 1][k], w);
   }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[m][e] += y[m][e];
 }
 
 template <class T, int D, int M>
@@ -378,14 +387,24 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) weight_bloc
 
 // ---------------------------------------------------------------- lse --
 // Maximum and sum of each query row over the kLseKeys keys of a CTA (a split).
+// Here query rows are the rows of the fragments, so a thread keeps the
+// maximum and sum of its own columns to the end. The keys lie in shared
+// memory; eight warps take (16 rows) x (a share of the keys) each, shares as
+// the rows leave warps over.
+template <int D>
+constexpr int lse_smem() {
+  return kLseKeys * (D * 2 + 16);
+}
+
 template <class T, int D>
 __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) lse_kernel(const __grid_constant__ ScoresLaunch p) {
-  constexpr int M = 2, KEYS = 16 * M;
-  static_assert(kBlockWarps * KEYS == kLseKeys, "one tile per warp");
-  __shared__ __align__(16) QueryBlock<D> qb;
-  __shared__ float2 s_ml[kBlockWarps][kBlockRows / 2];
+  constexpr int PITCH = D * 2 + 16, CH = D / 8, RPI = 32 / CH, CHUNK = 32;
+  extern __shared__ __align__(128) uint8_t ktile[];
+  __shared__ float2 s_ml[kBlockWarps][16];
+  __shared__ uint32_t s_valid[kBlockWarps];  // 32 keys each
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.z, h = blockIdx.x, group = p.sq.group, split = blockIdx.y;
+  grid_next();
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int pairs = s.rows * group;
@@ -394,65 +413,127 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) lse_kernel(
     const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
     return ((int64_t)(s.row0 + j) * (p.kv.heads * group) + h * group + i - j * group) * p.splits + split;
   };
-  if (split * kLseKeys >= s.len) {  // behind the end: empty parts
+  const int key0 = split * kLseKeys;
+  if (key0 >= s.len) {  // behind the end: empty parts
     for (int i = threadIdx.x; i < pairs; i += kBlockWarps * 32) p.part[at(i)] = make_float2(DARIC_NEG_INF, 0.f);
     return;
   }
-  const int key0 = split * kLseKeys + warp * KEYS;
-  KeyTile<D, M> kt;
-  kt.load(p, s, b, h, key0);
-  const bool draft = key0 + KEYS > s.ctx;
-  for (int i0 = 0; i0 < pairs; i0 += kBlockRows) {
-    qb.load(p, s, h, i0, pairs);
-    // the warps meet twice a block, over half of its rows each
-    for (int c0 = 0; c0 < kBlockRows && i0 + c0 < pairs; c0 += kBlockRows / 2) {
-      if (c0) __syncthreads();
-#pragma unroll 2
-      for (int i = c0; i < c0 + kBlockRows / 2 && i0 + i < pairs; i += 8) {
-        float x[M][4];
-        block_products<T, D, M>(kt, qb, i, x);
+  {  // a warp brings 32 keys, a lane looks one up
+    const int64_t off = key_offset(p, s, b, h, key0 + warp * 32 + lane);
+    const unsigned ok = __ballot_sync(0xffffffffu, off >= 0);
+    if (lane == 0) s_valid[warp] = ok;
+    const uint32_t dst = smem_u32(ktile) + (warp * 32 + lane / CH) * PITCH + (lane % CH) * 16;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = qb.row[i + 2 * t + e];
-          float y[2 * M], mx = DARIC_NEG_INF, l = 0.f;
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int64_t o = __shfl_sync(0xffffffffu, off, i * RPI + lane / CH);
+      cp16(dst + i * RPI * PITCH, p.kv.base + (o >= 0 ? o + (lane % CH) * 16 : 0), o >= 0);
+    }
+    cp_commit();
+  }
+  const int row_groups = (pairs + 15) / 16;
+  int shares = 1;  // of the keys per row group: 1, 2, 4 or 8
+  while (shares < kBlockWarps && row_groups * shares * 2 <= kBlockWarps) shares *= 2;
+  const int share = warp % shares, lanes_rg = kBlockWarps / shares;
+  const int k_first = share * (kLseKeys / shares);
+  for (int r0 = 0; r0 < row_groups; r0 += lanes_rg) {
+    const int pi = (r0 + warp / shares) * 16;  // first pair of this warp's rows
+    float m[2] = {DARIC_NEG_INF, DARIC_NEG_INF}, l[2] = {0.f, 0.f};
+    int row[2] = {0, 0};
+    uint32_t qf[D / 16][4];
 #pragma unroll
-          for (int r = 0; r < 2 * M; ++r) {
-            y[r] = x[r >> 1][(r & 1) * 2 + e];
-            bool ok = (kt.valid >> r) & 1u;
-            if (ok && draft) {
-              const int d = key0 + g + 8 * r - s.ctx;
-              ok = d < 0 || (i0 + i + 2 * t + e < pairs && sees_draft(p.sq, row, row - s.row0, d));
-            }
-            if (!ok) y[r] = DARIC_NEG_INF;
-            mx = fmaxf(mx, y[r]);
+    for (int r = 0; r < 2; ++r) {
+      const int i = pi + g + 8 * r, j = (int)fdiv((uint32_t)i, p.sq.group_div);
+      row[r] = s.row0 + j;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q + (int64_t)(s.row0 + j) * p.q_row +
+                                                            (int64_t)(h * group + i - j * group) * p.q_head) + t;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][r] = i < pairs ? __ldg(q + 8 * k) : 0u;
+        qf[k][2 + r] = i < pairs ? __ldg(q + 8 * k + 4) : 0u;
+      }
+    }
+    if (r0 == 0) {
+      cp_wait<0>();
+      __syncthreads();
+    }
+    if (pi < pairs) {
+      for (int c = k_first; c < k_first + kLseKeys / shares && key0 + c < s.len; c += CHUNK) {
+        float x[CHUNK / 8][4];
+#pragma unroll
+        for (int n = 0; n < CHUNK / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
+        const uint32_t ka = smem_u32(ktile) + (c + (lane >> 4) * 8 + (lane & 7)) * PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int n = 0; n < CHUNK / 16; ++n) {
+            uint32_t kf[4];
+            ldsm4(ka + n * 16 * PITCH + k * 32, kf);
+            Mma<T>::run(x[2 * n], qf[k], kf[0], kf[1]);
+            Mma<T>::run(x[2 * n + 1], qf[k], kf[2], kf[3]);
           }
+        const uint32_t valid = s_valid[c / 32];
+        const bool draft = key0 + c + CHUNK > s.ctx;
+        if (valid != 0xffffffffu || draft) {
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          for (int n = 0; n < CHUNK / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = n * 8 + 2 * t + (e & 1), d = key0 + c + key - s.ctx, i = pi + g + 8 * (e >> 1);
+              const bool ok = ((valid >> key) & 1u) &&
+                              (d < 0 || (i < pairs && sees_draft(p.sq, row[e >> 1], row[e >> 1] - s.row0, d)));
+              if (!ok) x[n][e] = DARIC_NEG_INF;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float mx = m[r];
+#pragma unroll
+          for (int n = 0; n < CHUNK / 8; ++n) mx = fmaxf(mx, fmaxf(x[n][2 * r], x[n][2 * r + 1]));
           const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
+          float sum = l[r] * exp2_fast((m[r] - bs) * cexp);
 #pragma unroll
-          for (int r = 0; r < 2 * M; ++r) l += exp2_fast((y[r] - bs) * cexp);
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-          if (g == 0) s_ml[warp][i - c0 + 2 * t + e] = make_float2(mx, l);
+          for (int n = 0; n < CHUNK / 8; ++n)
+            sum += exp2_fast((x[n][2 * r] - bs) * cexp) + exp2_fast((x[n][2 * r + 1] - bs) * cexp);
+          l[r] = sum;
+          m[r] = mx;
         }
       }
-      __syncthreads();
-      const int i = i0 + c0 + (int)threadIdx.x;
-      if (threadIdx.x < kBlockRows / 2 && i < pairs) {
-        float mx = DARIC_NEG_INF, l = 0.f;
+    }
 #pragma unroll
-        for (int w = 0; w < kBlockWarps; ++w) mx = fmaxf(mx, s_ml[w][threadIdx.x].x);
-        const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int w = 0; w < kBlockWarps; ++w) l += s_ml[w][threadIdx.x].y * exp2_fast((s_ml[w][threadIdx.x].x - bs) * cexp);
-        p.part[at(i)] = make_float2(mx, l);
+      for (int o = 1; o < 4; o <<= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m[r], o), ol = __shfl_xor_sync(0xffffffffu, l[r], o);
+        const float mx = fmaxf(m[r], om), bs = mx == DARIC_NEG_INF ? 0.f : mx;
+        l[r] = l[r] * exp2_fast((m[r] - bs) * cexp) + ol * exp2_fast((om - bs) * cexp);
+        m[r] = mx;
       }
+    if (r0) __syncthreads();  // the shares of the rows before are joined
+    if (t == 0) {
+      s_ml[warp][g] = make_float2(m[0], l[0]);
+      s_ml[warp][g + 8] = make_float2(m[1], l[1]);
+    }
+    __syncthreads();
+    const int rg = threadIdx.x / 16, i = (r0 + rg) * 16 + (threadIdx.x & 15);
+    if (rg < lanes_rg && i < pairs) {
+      float mx = DARIC_NEG_INF, ll = 0.f;
+      for (int w = 0; w < shares; ++w) mx = fmaxf(mx, s_ml[rg * shares + w][threadIdx.x & 15].x);
+      const float bs = mx == DARIC_NEG_INF ? 0.f : mx;
+      for (int w = 0; w < shares; ++w) {
+        const float2 v = s_ml[rg * shares + w][threadIdx.x & 15];
+        ll += v.y * exp2_fast((v.x - bs) * cexp);
+      }
+      p.part[at(i)] = make_float2(mx, ll);
     }
   }
 }
 
 // lse of each query row and head from its parts (one warp each).
-__global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ ScoresLaunch p, int64_t items) {
+__global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ ScoresLaunch p) {
+  const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
+  grid_wait();
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (at >= items) return;
@@ -495,10 +576,12 @@ void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
   const int64_t cap = (int64_t)p.sq.table_cols * p.kv.page_size;
   if (!p.lse) {
     const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
-    lse_kernel<T, D><<<dim3((unsigned)p.kv.heads, (unsigned)p.splits, (unsigned)p.sq.num_seqs), kBlockWarps * 32, 0, s>>>(p);
+    static std::atomic<uint64_t> done{0};
+    allow_smem(lse_kernel<T, D>, lse_smem<D>(), done);
+    lse_kernel<T, D><<<dim3((unsigned)p.kv.heads, (unsigned)p.splits, (unsigned)p.sq.num_seqs), kBlockWarps * 32,
+                       lse_smem<D>(), s>>>(p);
     DARIC_CUDA(cudaGetLastError());
-    lse_join_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(p, items);
-    DARIC_CUDA(cudaGetLastError());
+    launch_after(lse_join_kernel, dim3((unsigned)((items + 7) / 8)), 256, s, p);
     p.lse = p.lse_work;
     p.lse_row = (int64_t)p.kv.heads * p.sq.group;
   }
