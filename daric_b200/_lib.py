@@ -72,6 +72,9 @@ SIGNATURES: dict[str, tuple] = {
         C.c_int, [_vp, C.c_int64, C.c_int64, C.c_int64, _i64p, _i64p, _i64p, _i64p, C.c_int, C.c_float,
                   _vp, C.c_int64, _i64p, C.c_int64, _vp, _vp, _vp, C.c_int64, _i64p, C.c_int, _vp]),
     "daric_attend_workspace": (C.c_int, [C.c_int, C.c_int64, C.POINTER(C.c_int64)]),
+    "daric_sparse_workspace": (
+        C.c_int, [C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                  C.POINTER(C.c_int64)]),
     "daric_copier_tree_attention": (
         C.c_int, [_vp, C.c_char_p, C.c_int, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
                   _vp, C.c_int64, C.c_int64, C.c_int64, _vp, _vp, _vp, C.c_int64, C.c_float,

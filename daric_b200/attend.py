@@ -100,20 +100,25 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _attend_workspace(dev: torch.device, head_dim: int, stream: int, kept: bool) -> torch.Tensor:
-    """Workspace of an attention call. Calls on one stream follow each other,
-    so they share one that is kept; a captured call has its own, which belongs
-    to its graph, and so has one on a stream given by its handle."""
+def _kept(key: tuple, kept: bool, dev: torch.device, size) -> torch.Tensor:
+    """Workspace of a call. Calls on one stream follow each other, so they
+    share one that is kept; a captured call has its own, which belongs to its
+    graph, and so has one on a stream given by its handle. ``size`` fills in
+    the bytes."""
     kept = kept and not _capturing()
-    key = (dev.index, head_dim, stream)
     ws = _workspaces.get(key) if kept else None
     if ws is None:
         v = C.c_int64(0)
-        check(_lib.load().daric_attend_workspace(dev.index, head_dim, C.byref(v)))
+        check(size(C.byref(v)))
         ws = torch.empty(v.value, dtype=torch.uint8, device=dev)
         if kept:
             _workspaces[key] = ws
     return ws
+
+
+def _attend_workspace(dev: torch.device, head_dim: int, stream: int, kept: bool) -> torch.Tensor:
+    return _kept((dev.index, head_dim, stream), kept, dev,
+                 lambda v: _lib.load().daric_attend_workspace(dev.index, head_dim, v))
 
 
 def _outputs(q, out, lse):
@@ -184,9 +189,9 @@ def sparse_attention(copier: CacheCopier, layer_name: str, q: torch.Tensor, page
 
     ``pages`` is int32 [rows, KV heads, k]: page numbers of the row's sequence
     (columns of its block table) as :func:`daric_b200.blocks.select_pages`
-    returns them; negative entries are empty, an entry past the block table is
-    skipped and sets a device error bit, and a page listed twice counts twice.
-    A row sees the listed positions up to its own. The rest is as in
+    returns them, ascending; negative entries are empty, an entry past the block
+    table is skipped and sets a device error bit, and one that repeats the entry
+    before it counts once. A row sees the listed positions up to its own. The rest is as in
     :func:`tree_attention` (without a mask)."""
     kv = layer_tensor(copier, layer_name)
     dev = kv.device
@@ -214,7 +219,12 @@ def _sparse(copier, layer_name, kv, q, pages, block_table, seq_lens, cu_q, n, sc
         return out, lse
     dev = kv.device
     s = _raw_stream(dev.index)
-    ws = _attend_workspace(dev, dim, s, kept)
+    # a shape of few rows needs what any such call does; lists of many rows
+    # have sizes of their own and are not kept
+    sizes = (rows, n, heads, pages.shape[1], pages.shape[2], block_table.shape[1])
+    few = rows * heads < 64 * n * pages.shape[1]
+    ws = _kept((dev.index, dim, s, "sparse"), kept and few, dev,
+               lambda v: _lib.load().daric_sparse_workspace(dev.index, dim, *sizes, v))
     check(_lib.load().daric_copier_sparse_attention(
         copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
         heads, dim, pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[2], block_table.data_ptr(),

@@ -71,7 +71,14 @@ struct AttendLaunch {
   float* part;                // workspace: partial outputs
   float2* part_ml;            // workspace: their maxima and sums
   int4* desc;                 // workspace: what the join of a CTA does
+  // listed pages on the tensor cores (workspace): per row tile of 128 pairs
+  // and KV head the pages that any of its rows lists
+  uint4* list;                // [lists, list_row]: page, rows that list it, block
+  int32_t* list_count;        // [lists], -1: no such row tile
+  int2* list_tile;            // [lists / heads]: sequence and its row tile
+  int32_t lists, list_row;
 };
+constexpr int kUnionPages = 48 * 1024;  // most pages of a sequence for that
 
 // Rows of query heads a CTA of the row-tile variant rg (1, 2, 4) holds.
 constexpr int attend_rows(int rg) { return 16 * rg; }

@@ -104,14 +104,33 @@ struct Variant {
 Variant variant_rg(int rg, int64_t dim) { return {rg, 0, attend_rows(rg), dim > 128 ? 1 : (rg == 1 ? 3 : 2)}; }
 Variant variant_mt(int mt) { return {0, mt, 128 * mt, 1}; }
 
-Variant attend_variant(const SeqBatch& b, const KvView& kv, bool sparse) {
-  const int64_t rows = sparse ? b.group : (int64_t)((b.num_rows + b.num_seqs - 1) / b.num_seqs) * b.group;
-  if (rows <= 16) return variant_rg(1, kv.head_dim);
-  if (rows <= 32 || sparse) return variant_rg(2, kv.head_dim);
+// k: pages listed per row (0: all of the sequence).
+Variant attend_variant(int64_t num_rows, int64_t num_seqs, int64_t group, int64_t head_dim, double layer_bytes, int64_t k,
+                       int64_t table_cols) {
+  const int64_t rows = k ? group : (num_rows + num_seqs - 1) / num_seqs * group;
   // the wide form keeps offsets in 32 bits of 16 bytes
-  if (kv.head_dim > 128 || (double)kv.num_pages * (double)kv.page_stride >= 60.0 * (1ll << 30))
-    return variant_rg(4, kv.head_dim);
+  const bool wide = head_dim <= 128 && layer_bytes < 60.0 * (1ll << 30);
+  // Listed pages: where a sequence has half a tile of pairs or more, and a
+  // tile no more than 32 rows (a bit each), the rows of a tile share one pass
+  // over the pages that any of them lists. They read each page once then,
+  // which is what bounds the row-by-row form (512 rows with 64 of 512 pages
+  // each, no two lists alike: 265 us row by row).
+  if (k && wide && group >= 4 && num_rows * group >= 64 * num_seqs && table_cols <= kUnionPages) return variant_mt(1);
+  if (rows <= 16) return variant_rg(1, head_dim);
+  if (rows <= 32 || k) return variant_rg(2, head_dim);
+  if (!wide) return variant_rg(4, head_dim);
   return variant_mt(rows <= 128 ? 1 : 2);
+}
+
+double layer_bytes(const KvView& kv) { return (double)kv.num_pages * (double)kv.page_stride; }
+
+// Lists of a wide call over listed pages.
+struct Lists {
+  int64_t lists, row;
+  int64_t bytes() const { return lists * row * 16 + (lists * 4 + 15) / 16 * 16 + (lists + 1) * 8; }
+};
+Lists list_room(int64_t num_rows, int64_t num_seqs, int64_t q_heads, int64_t kv_heads, int64_t k, int64_t table_cols) {
+  return {(num_rows * (q_heads / kv_heads) / 128 + num_seqs) * kv_heads, std::min<int64_t>(table_cols, 32 * k)};
 }
 
 size_t attend_bytes(int grid, int rows, int head_dim) {
@@ -141,6 +160,24 @@ int daric_attend_workspace(int device, int64_t head_dim, int64_t* out_bytes) {
     for (const Variant& v : {variant_rg(1, head_dim), variant_rg(2, head_dim), variant_rg(4, head_dim), variant_mt(2)})
       if (v.mt == 0 || head_dim <= 128) most = std::max(most, attend_bytes(sms * v.ctas, v.rows, (int)head_dim));
     *out_bytes = (int64_t)most;
+  });
+}
+
+int daric_sparse_workspace(int device, int64_t head_dim, int64_t num_rows, int64_t num_seqs, int64_t q_heads,
+                           int64_t kv_heads, int64_t k, int64_t table_cols, int64_t* out_bytes) {
+  return guard([&] {
+    DARIC_CHECK(out_bytes, "out_bytes is NULL");
+    DARIC_CHECK(head_dim > 0 && head_dim <= 256, "head dimension must be at most 256");
+    DARIC_CHECK(num_rows >= 0 && num_seqs >= 1 && kv_heads >= 1 && q_heads >= kv_heads && k >= 1 && table_cols >= 1,
+                "sizes must be positive");
+    const Variant v = attend_variant(num_rows, num_seqs, q_heads / kv_heads, head_dim, 0.0, k, table_cols);
+    int64_t most = (int64_t)attend_bytes(device_info(device).sm_count * v.ctas, v.rows, (int)head_dim);
+    for (int rg : {1, 2}) {  // a layer too large for the wide form
+      const Variant u = variant_rg(rg, head_dim);
+      most = std::max(most, (int64_t)attend_bytes(device_info(device).sm_count * u.ctas, u.rows, (int)head_dim));
+    }
+    if (v.mt) most = (most + 15) / 16 * 16 + list_room(num_rows, num_seqs, q_heads, kv_heads, k, table_cols).bytes();
+    *out_bytes = most;
   });
 }
 
@@ -178,7 +215,7 @@ int daric_copier_tree_attention(daric_copier* copier, const char* layer_name, in
     p.lse_row = lse_row;
     p.scale = scale;
     // tiles of the whole batch are counted in 32 bits
-    const Variant var = attend_variant(p.sq, L.kv, false);
+    const Variant var = attend_variant(num_rows, num_seqs, p.sq.group, head_dim, layer_bytes(L.kv), 0, table_cols);
     const int rows = var.rows;
     const double tiles = (double)L.kv.heads * ((double)num_rows * p.sq.group / rows + (double)num_seqs) *
                          ((double)table_cols * L.kv.page_size / 16.0 + 1.0);
@@ -227,15 +264,27 @@ int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, 
     p.pages_head = pages_head;
     p.k = (int32_t)k;
     p.scale = scale;
-    const Variant var = attend_variant(p.sq, L.kv, true);
-    const int rows = var.rows;
-    const double tiles = (double)L.kv.heads * (double)num_rows * ((double)p.sq.group / rows + 1.0) *
-                         ((double)k * L.kv.page_size / 16.0 + 1.0);
+    Variant var = attend_variant(num_rows, num_seqs, p.sq.group, head_dim, layer_bytes(L.kv), k, table_cols);
+    const Lists room = list_room(num_rows, num_seqs, q_heads, L.kv.heads, k, table_cols);
+    const double per_list = (double)std::max(k, room.row) * L.kv.page_size / 16.0 + 1.0;
+    const double tiles = (double)L.kv.heads * (double)num_rows * ((double)p.sq.group / 16 + 1.0) * per_list;
     DARIC_CHECK(tiles < 4.0e9, "sparse_attention: the batch has too many tiles for one call");
     const int grid = di.sm_count * var.ctas;
-    attend_workspace(p, grid, rows, workspace, workspace_bytes);
+    attend_workspace(p, grid, var.rows, workspace, workspace_bytes);
     OnDevice on(device);
-    launch_attend(p, kv_dtype, var.rg, grid, (cudaStream_t)stream);
+    if (var.mt) {
+      const int64_t at = ((int64_t)attend_bytes(grid, var.rows, (int)head_dim) + 15) / 16 * 16;
+      DARIC_CHECK(at + room.bytes() <= workspace_bytes, "workspace is too small");
+      uint8_t* w = (uint8_t*)workspace + at;
+      p.lists = (int32_t)room.lists;
+      p.list_row = (int32_t)room.row;
+      p.list = (uint4*)w;
+      p.list_count = (int32_t*)(w + room.lists * room.row * 16);
+      p.list_tile = (int2*)(w + room.lists * room.row * 16 + (room.lists * 4 + 15) / 16 * 16);
+      launch_wide(p, kv_dtype, 1, grid, (cudaStream_t)stream);
+    } else {
+      launch_attend(p, kv_dtype, var.rg, grid, (cudaStream_t)stream);
+    }
   });
 }
 

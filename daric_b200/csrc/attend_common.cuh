@@ -30,11 +30,12 @@ void allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
 __device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class K, class P>
-void launch_after(K kern, dim3 grid, int threads, cudaStream_t s, const P& p) {
+void launch_after(K kern, dim3 grid, int threads, cudaStream_t s, const P& p, int smem = 0) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.stream = s;
+  cfg.dynamicSmemBytes = (size_t)smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -74,6 +75,12 @@ __device__ __forceinline__ int32_t ld_ahead(const int32_t* p) {
   return v;
 }
 
+__device__ __forceinline__ int4 ld_ahead(const int4* p) {
+  int4 v;
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -109,6 +116,12 @@ struct Mma<__nv_bfloat16> {
     return *reinterpret_cast<uint32_t*>(&h);
   }
   __device__ __forceinline__ static float widen(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+  // both halves: a * 0 + b
+  __device__ __forceinline__ static uint32_t zero_sum(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&a), __nv_bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)),
+                                     *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
   static constexpr uint16_t kExpMask = 0x7f80;  // all ones: infinity or NaN
 };
 template <>
@@ -124,6 +137,11 @@ struct Mma<__half> {
     return *reinterpret_cast<uint32_t*>(&h);
   }
   __device__ __forceinline__ static float widen(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+  __device__ __forceinline__ static uint32_t zero_sum(uint32_t a, uint32_t b) {
+    const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), __half2(__ushort_as_half(0), __ushort_as_half(0)),
+                              *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
   static constexpr uint16_t kExpMask = 0x7c00;
 };
 

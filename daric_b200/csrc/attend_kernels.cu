@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
         int pg = e, left = sg.s.len - i;
         if (SPARSE) {
           pg = e < p.k && seq_id >= 0 ? ld_ahead(&prow[e]) : -1;
+          if (pg >= 0 && e > 0 && ld_ahead(&prow[e - 1]) == pg) pg = -1;  // a repeated page counts once
           if (pg >= p.sq.table_cols) {
             atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
             pg = -1;

@@ -46,12 +46,12 @@ constexpr int kKeys = 128;      // keys of a tile
 constexpr int kMaskRing = 8;    // tiles whose key masks are kept
 constexpr int kCopyThreads = 128;
 
-template <int D, int MT>
+template <int D, int MT, bool SPARSE>
 struct Wide {
   static constexpr int ROWS = 128 * MT;
   static constexpr int SLOT = kKeys * D * 2;
   static constexpr int QB = ROWS * D * 2;
-  static constexpr int NS = D == 64 ? 10 : (MT == 2 ? 5 : 6);
+  static constexpr int NS = D == 64 ? 10 : (MT == 2 || SPARSE ? 5 : 6);
   static constexpr int BEHIND = NS > 5 ? 3 : 2;  // slots copied but not reported yet
   static constexpr int THREADS = 512;  // the last three warps only lend their registers
   static constexpr int COPY_WARP = 8;
@@ -70,9 +70,13 @@ struct WideShared {
   int abort;               // a wait gave up: everyone leaves
   int poison[4];           // by count modulo 4: the segment if its drafted V rows hold infinities or NaN
 };
-template <int D, int MT>
+// SPARSE: which of a tile's (up to) 32 query rows see each of its keys.
+struct SparseShared {
+  uint32_t vis[kMaskRing][32][4];
+};
+template <int D, int MT, bool SPARSE>
 constexpr int wide_smem() {
-  return Wide<D, MT>::TILES + (int)sizeof(WideShared);
+  return Wide<D, MT, SPARSE>::TILES + (int)sizeof(WideShared) + (SPARSE ? (int)sizeof(SparseShared) : 0);
 }
 
 // The part of a segment that a CTA works on.
@@ -80,16 +84,19 @@ struct Part {
   int b, h, rt, tile0, n, ntiles;
   Seq s;
   int row_base, my_rows;  // first pair of the row tile, and pairs that exist
+  int listed;             // SPARSE: pages of the tile's list
+  const uint4* list;      // SPARSE: page, rows of the tile that see it, block
 };
 
-template <class T, int D, int MT>
-__global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __grid_constant__ AttendLaunch p) {
-  using W = Wide<D, MT>;
+template <class T, int D, int MT, bool SPARSE>
+__global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ AttendLaunch p) {
+  using W = Wide<D, MT, SPARSE>;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int HB = D / 64;          // 64-element halves of a row
   constexpr int HALF = kKeys * 128;   // bytes of such a half of a tile
   extern __shared__ __align__(1024) uint8_t base[];  // the only shared memory: it starts on 1024 bytes
   WideShared& sh = *reinterpret_cast<WideShared*>(base + W::TILES);
+  SparseShared& sp = *reinterpret_cast<SparseShared*>(base + W::TILES + sizeof(WideShared));
   uint8_t* q_tile = base;
   uint8_t* slots = base + W::QB;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -98,17 +105,28 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
 
   // ---- the line of tiles and this CTA's part of it (as in attend_kernels.cu)
   uint32_t* sums = reinterpret_cast<uint32_t*>(slots);  // before any copy
-  const int per = (p.sq.num_seqs + W::THREADS - 1) / W::THREADS;
+  // units of the line: sequences, or (SPARSE) the lists of a row tile and head
+  const int units = SPARSE ? p.lists : p.sq.num_seqs;
+  const int per = (units + W::THREADS - 1) / W::THREADS;
   auto tiles_of = [&](const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); };
+  auto list_tiles = [&](int i) {  // 0: no such row tile
+    const int n = p.list_count[i];
+    return n < 0 ? 0 : max((int)(((int64_t)n * p.kv.page_size + kKeys - 1) / kKeys), 1);
+  };
   auto tiles_seq = [&](const Seq& s) {
     return ((uint32_t)(s.rows * group) + W::ROWS - 1) / W::ROWS * (uint32_t)p.kv.heads * (uint32_t)tiles_of(s);
   };
   {
     uint32_t mine = 0;
-    for (int i = tid * per; i < min((tid + 1) * per, p.sq.num_seqs); ++i) {
-      Seq s = load_seq(p.sq, i);
-      clamp_len(p.sq, p.kv.page_size, s);
-      mine += tiles_seq(s);
+    if (SPARSE) grid_wait();  // the lists are there
+    for (int i = tid * per; i < min((tid + 1) * per, units); ++i) {
+      if (SPARSE) {
+        mine += (uint32_t)list_tiles(i);
+      } else {
+        Seq s = load_seq(p.sq, i);
+        clamp_len(p.sq, p.kv.page_size, s);
+        mine += tiles_seq(s);
+      }
     }
     sums[tid] = mine;
     __syncthreads();
@@ -173,6 +191,28 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
   };
   // Part of the line at tile t; false: none (lengths changed while the kernel ran).
   auto part_at = [&](uint32_t t, Part& g) {
+    if (SPARSE) {
+      for (;; ++b) {
+        if (b >= units) return false;
+        const uint32_t n = (uint32_t)list_tiles(b);
+        if (t < seg_at + n) break;
+        seg_at += (uint32_t)list_tiles(b);
+      }
+      const int2 where = p.list_tile[b / p.kv.heads];
+      g.b = where.x;
+      g.rt = where.y;
+      g.h = b % p.kv.heads;
+      g.s = load_seq(p.sq, g.b);
+      clamp_len(p.sq, p.kv.page_size, g.s);
+      g.ntiles = list_tiles(b);
+      g.listed = p.list_count[b];
+      g.list = p.list + (int64_t)b * p.list_row;
+      g.tile0 = (int)(t - seg_at);
+      g.n = (int)min((uint32_t)(g.ntiles - g.tile0), t1 - t);
+      g.row_base = g.rt * W::ROWS;
+      g.my_rows = min(W::ROWS, g.s.rows * group - g.row_base);
+      return true;
+    }
     for (;; ++b) {
       if (b >= p.sq.num_seqs) return false;
       g.s = load_seq(p.sq, b);
@@ -217,11 +257,43 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
     const int ct = tid - W::COPY_WARP * 32;
     uint32_t n_slot = 0, n_seg = 0, n_tile = 0;  // slots, segments, key tiles so far
     constexpr int BH = W::BEHIND;
+    constexpr int CH = D / 8, RPI = kCopyThreads / CH;  // vectors of a row, rows at a time
     uint64_t* pend[BH];                          // groups not reported yet, older first
+    int pend_v[BH], pend_seg[BH];                // SPARSE: their slot if it is a V tile, and the segment
 #pragma unroll
     for (int i = 0; i < BH; ++i) pend[i] = nullptr;
-    auto report = [&](uint64_t* bar) {
+    // V rows that some rows must not see: values without a finite size would
+    // reach them through 0 * inf. They are taken out here and added where
+    // they are seen, at the end of the segment.
+    auto take_out = [&](int st, uint32_t seg) {
+      const int c = ct % CH, r0 = ct / CH;
+      uint8_t* tile = slots + st * W::SLOT + (c >> 3) * HALF;
+      auto vec = [&](int k) {
+        const int r = r0 + k * RPI;
+        return reinterpret_cast<uint4*>(tile + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      };
+      // x * 0 summed up: 0, or NaN where some x is not finite
+      uint32_t sum = 0;
+#pragma unroll
+      for (int k0 = 0; k0 < kKeys / RPI; k0 += 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = *vec(k0 + k);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          sum = Mma<T>::zero_sum(x[k].x, Mma<T>::zero_sum(x[k].y, Mma<T>::zero_sum(x[k].z, Mma<T>::zero_sum(x[k].w, sum))));
+      }
+      if ((sum & 0x7fff7fffu) == 0) return;
+      for (int k = 0; k < kKeys / RPI; ++k) {
+        uint16_t* v = reinterpret_cast<uint16_t*>(vec(k));
+        for (int e = 0; e < 8; ++e)
+          if ((v[e] & Mma<T>::kExpMask) == Mma<T>::kExpMask) v[e] = 0;
+      }
+      *(volatile int*)&sh.poison[seg & 3] = (int)seg;
+    };
+    auto report = [&](uint64_t* bar, int v_slot_of, int seg) {
       if (!bar) return;
+      if (SPARSE && v_slot_of >= 0) take_out(v_slot_of, (uint32_t)seg);
       fence_proxy_async();
       mbar_arrive(bar);
     };
@@ -229,17 +301,23 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
       cp_wait<0>();
 #pragma unroll
       for (int i = 0; i < BH; ++i) {
-        report(pend[i]);
+        report(pend[i], pend_v[i], pend_seg[i]);
         pend[i] = nullptr;
       }
     };
-    auto push = [&](uint64_t* bar) {  // a group was issued: reports the one BH before it
+    auto push = [&](uint64_t* bar, int v) {  // a group was issued: reports the one BH before it
       cp_commit();
       cp_wait<BH>();
-      report(pend[0]);
+      report(pend[0], pend_v[0], pend_seg[0]);
 #pragma unroll
-      for (int i = 0; i + 1 < BH; ++i) pend[i] = pend[i + 1];
+      for (int i = 0; i + 1 < BH; ++i) {
+        pend[i] = pend[i + 1];
+        pend_v[i] = pend_v[i + 1];
+        pend_seg[i] = pend_seg[i + 1];
+      }
       pend[BH - 1] = bar;
+      pend_v[BH - 1] = v;
+      pend_seg[BH - 1] = (int)n_seg;
     };
     auto take = [&](uint64_t* bar, uint32_t parity) {  // what is reported late must not be waited for
       if (tc::mbar_test(bar, parity)) return true;
@@ -269,7 +347,6 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
       if (n_seg) ok = together(take(&sh.q_empty, (n_seg - 1) & 1));
       if (!ok) break;
       {
-        constexpr int CH = D / 8;
         for (int v = ct; v < W::ROWS * CH; v += kCopyThreads) {
           const int r = v / CH, c = v % CH, i = g.row_base + r;
           const bool in = r < g.my_rows;
@@ -281,16 +358,34 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
                                (((c & 7) ^ (r & 7)) << 4);
           cp16(dst, src, in);
         }
-        push(&sh.q_full);
+        push(&sh.q_full, -1);
       }
-      auto lookup = [&](int i) {  // block of this thread's key of tile i, -1: none
-        const int pos = (g.tile0 + i) * kKeys + ct;
-        if (i >= g.n || pos >= g.s.len) return -1;
-        return ld_ahead(&trow[fdiv((uint32_t)pos, p.kv.page_div)]);
+      // this thread's key of the next tile: block (-1: none), position, and
+      // (SPARSE) the rows of the tile that list its page
+      int blk = -1, pos = 0;
+      uint32_t rows_see = 0;
+      const int j_first = SPARSE ? (int)fdiv((uint32_t)g.row_base, p.sq.group_div) : 0;
+      auto lookup = [&](int i) {
+        const int k = (g.tile0 + i) * kKeys + ct;
+        blk = -1;
+        pos = 0x7fffffff;
+        if (i >= g.n) return;
+        if (SPARSE) {
+          const int e = (int)fdiv((uint32_t)k, p.kv.page_div);
+          rows_see = 0;
+          if (e < g.listed) {
+            const int4 x = ld_ahead(reinterpret_cast<const int4*>(g.list + e));
+            pos = x.x * p.kv.page_size + k - e * p.kv.page_size;
+            rows_see = (uint32_t)x.y;
+            blk = x.z;
+          }
+        } else {
+          pos = k;
+          if (k < g.s.len) blk = ld_ahead(&trow[fdiv((uint32_t)k, p.kv.page_div)]);
+        }
       };
-      int blk = lookup(0);
-      auto place = [&](int i) {  // offsets and mask of tile i; looks the next one up
-        const int pos = (g.tile0 + i) * kKeys + ct;
+      lookup(0);
+      auto place = [&](int i) {  // offsets and masks of tile i; looks the next one up
         bool in = pos < g.s.len;
         if (in && (blk < 0 || blk >= p.kv.num_pages)) {
           atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
@@ -301,10 +396,25 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
           const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
           off = (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride;
         }
-        const unsigned m = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) sh.vmask[(n_tile + i) % kMaskRing][ct >> 5] = m;
+        if (SPARSE) {
+          // rows at or behind the position see it; then turned over: a word of
+          // 32 keys for each row
+          const int before = pos - g.s.ctx - j_first;  // rows of the tile that stand before it
+          const uint32_t m = !in || before >= 32 ? 0u : (before <= 0 ? rows_see : rows_see & (0xffffffffu << before));
+          uint32_t mine = m;  // lane: key, bit: row; then lane: row, bit: key
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const uint32_t lo = o == 16 ? 0x0000ffffu : o == 8 ? 0x00ff00ffu : o == 4 ? 0x0f0f0f0fu : o == 2 ? 0x33333333u : 0x55555555u;
+            const uint32_t y = __shfl_xor_sync(0xffffffffu, mine, o);
+            mine = (lane & o) ? (mine & ~lo) | ((y >> o) & lo) : (mine & lo) | ((y << o) & ~lo);
+          }
+          sp.vis[(n_tile + i) % kMaskRing][lane][ct >> 5] = mine;
+        } else {
+          const unsigned m = __ballot_sync(0xffffffffu, in);
+          if (lane == 0) sh.vmask[(n_tile + i) % kMaskRing][ct >> 5] = m;
+        }
         sh.off[i % 3][ct] = in ? (uint32_t)(off >> 4) : 0xffffffffu;
-        blk = lookup(i + 1);
+        lookup(i + 1);
         // The offsets of the tile three before this one are read by now: its
         // last copies were issued before the meeting of the tile in between.
         ok = together(ok);
@@ -314,7 +424,6 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
         if (!ok) return;
         if (use) ok = take(&sh.empty[st], (use - 1) & 1);
         if (!ok) return;  // all stop at the next meeting
-        constexpr int CH = D / 8, RPI = kCopyThreads / CH;  // rows at a time
         const int c = ct % CH;
         const uint8_t* src = kv + (v_tile ? p.kv.v_off : 0) + c * 16;
         const uint32_t dst = smem_u32(slots) + st * W::SLOT + (c >> 3) * HALF;
@@ -329,31 +438,12 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
           const int r7 = (ct / CH + k * RPI) & 7;
           cp16(d0 + k * RPI * 128 + (((c & 7) ^ r7) << 4), src + (in ? (int64_t)o[k] * 16 : 0), in);
         }
-        if (v_tile && (g.tile0 + i + 1) * kKeys > see) {
-          // drafted V rows that some rows must not see: values without a
-          // finite size would reach them through 0 * inf. They are taken out
-          // here and added where they are seen, at the end of the segment.
+        if (!SPARSE && v_tile && (g.tile0 + i + 1) * kKeys > see) {
           cp_commit();
           cp_wait<0>();
-          uint8_t* tile = slots + st * W::SLOT + (c >> 3) * HALF;
-          bool bad = false;
-          for (int r = ct / CH; r < kKeys; r += RPI) {
-            uint4* w = reinterpret_cast<uint4*>(tile + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-            uint4 x = *w;
-            uint16_t* u = reinterpret_cast<uint16_t*>(&x);
-            bool here = false;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if ((u[e] & Mma<T>::kExpMask) == Mma<T>::kExpMask) {
-                u[e] = 0;
-                here = true;
-              }
-            if (here) *w = x;
-            bad = bad || here;
-          }
-          if (bad) *(volatile int*)&sh.poison[n_seg & 3] = (int)n_seg;
+          take_out((int)st, n_seg);
         }
-        push(&sh.full[st]);
+        push(&sh.full[st], v_tile ? (int)st : -1);
         ++n_slot;
       };
       if (MT == 2) {
@@ -550,7 +640,9 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
       const int row = g.s.row0 + j, head = g.h * group + pi - j * group;
       const int see = all_see(g);
       const int items = items_of(st, g.n);
-      float m = DARIC_NEG_INF, l0 = 0.f, l1 = 0.f;
+      // a row that does not exist has no maximum to wait for
+      float m = real ? DARIC_NEG_INF : 0.f, l0 = 0.f, l1 = 0.f;
+      const int jl = SPARSE ? j - (int)fdiv((uint32_t)g.row_base, p.sq.group_div) : 0;  // row of the tile
       for (int li = 0; li < items; ++li) {
         const uint32_t c = done + (uint32_t)li;
         const int i = MT == 2 ? li : 2 * li + st;  // key tile
@@ -558,11 +650,12 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc::fence_after();
         const int key0 = (g.tile0 + i) * kKeys;
-        const uint32_t* vm = sh.vmask[(n_tile + (uint32_t)i) % kMaskRing];
-        const bool draft = key0 + kKeys > see;
-        const bool masked = draft || (vm[0] & vm[1] & vm[2] & vm[3]) != 0xffffffffu;
+        const uint32_t* vm = SPARSE ? sp.vis[(n_tile + (uint32_t)i) % kMaskRing][real ? jl : 0]
+                                    : sh.vmask[(n_tile + (uint32_t)i) % kMaskRing];
+        const bool draft = !SPARSE && key0 + kKeys > see;
+        const bool masked = SPARSE || draft || (vm[0] & vm[1] & vm[2] & vm[3]) != 0xffffffffu;
         float mb = m * cexp;
-        bool careful = masked || __any_sync(0xffffffffu, m == DARIC_NEG_INF);
+        bool careful = (masked && !SPARSE) || __any_sync(0xffffffffu, m == DARIC_NEG_INF);
         if (!careful) {
           // one pass: weights by the maximum so far, kept in registers until
           // the maximum of this tile is known to be near enough
@@ -571,10 +664,15 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             uint32_t x[32];
+            const uint32_t see_w = SPARSE ? vm[w] : 0;
             tc::ld32(s_col + w * 32, x);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float u = __uint_as_float(x[2 * e]), v = __uint_as_float(x[2 * e + 1]);
+              float u = __uint_as_float(x[2 * e]), v = __uint_as_float(x[2 * e + 1]);
+              if (SPARSE) {
+                u = see_w & (1u << (2 * e)) ? u : DARIC_NEG_INF;
+                v = see_w & (2u << (2 * e)) ? v : DARIC_NEG_INF;
+              }
               mx = fmaxf(mx, fmaxf(u, v));
               const float a = exp2_fast(__fmaf_rn(u, cexp, -mb)), d = exp2_fast(__fmaf_rn(v, cexp, -mb));
               a0 += a;
@@ -715,16 +813,25 @@ __global__ void __launch_bounds__(Wide<D, MT>::THREADS, 1) wide_kernel(const __g
               x[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), a1, __uint_as_float(x[e]) * a0));
           }
           if (poison && real) {
-            const int d0 = max((g.tile0 * kKeys) - g.s.ctx, 0);
-            const int d1 = min((g.tile0 + g.n) * kKeys, g.s.len) - g.s.ctx;
-            for (int d = d0; d < d1; ++d) {
-              const int pos = g.s.ctx + d;
-              if (pos < 0 || !sees_draft(p.sq, row, j, d)) continue;
-              const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
-              const int blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
+            // positions of this part that this row sees beside rows that do not
+            const int k0 = SPARSE ? g.tile0 * kKeys : max(g.tile0 * kKeys, max(g.s.ctx, 0));
+            const int k1 = SPARSE ? min((g.tile0 + g.n) * kKeys, g.listed * p.kv.page_size)
+                                  : min((g.tile0 + g.n) * kKeys, g.s.len);
+            for (int k = k0; k < k1; ++k) {
+              int pg = (int)fdiv((uint32_t)k, p.kv.page_div), blk;
+              const int in = k - pg * p.kv.page_size;
+              if (SPARSE) {
+                const uint4 x = g.list[pg];
+                const int pos = (int)x.x * p.kv.page_size + in;
+                if (!((x.y >> jl) & 1u) || pos > g.s.ctx + j || pos >= g.s.len) continue;
+                blk = (int)x.z;
+              } else {
+                if (!sees_draft(p.sq, row, j, k - g.s.ctx)) continue;
+                blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
+              }
               if (blk < 0 || blk >= p.kv.num_pages) continue;
               const uint16_t* v = reinterpret_cast<const uint16_t*>(
-                  p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)(pos - pg * p.kv.page_size) * p.kv.tok_stride +
+                  p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)in * p.kv.tok_stride +
                   (int64_t)g.h * p.kv.head_stride + p.kv.v_off) + w * 32;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
@@ -836,20 +943,117 @@ __global__ void __launch_bounds__(256) wide_join_kernel(const __grid_constant__ 
   if (warp == 0 && p.lse) p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : __fmaf_rn(mm, p.scale, logf(ll));
 }
 
-template <class T, int D, int MT>
+// Lists of the SPARSE form, one per row tile (blockIdx.x) and KV head: the
+// pages that any of its rows lists, ascending, with the rows (bits) that do
+// and the page's block. A row's page behind its own position is left out.
+constexpr int kUnionThreads = 256;
+__global__ void __launch_bounds__(kUnionThreads) union_kernel(const __grid_constant__ AttendLaunch p) {
+  extern __shared__ uint32_t table[];  // rows that list each page of the sequence
+  __shared__ int s_where[2];
+  __shared__ int s_sum[kUnionThreads / 32];
+  grid_next();
+  const int tile = blockIdx.x, h = blockIdx.y, H = p.kv.heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = p.sq.group, bs = p.kv.page_size;
+  if (warp == 0) {  // the sequence of the row tile
+    int at = 0, found = -1, rt = 0;
+    for (int b0 = 0; b0 < p.sq.num_seqs && found < 0; b0 += 32) {
+      int n = 0;
+      if (b0 + lane < p.sq.num_seqs) n = (load_seq(p.sq, b0 + lane).rows * group + 127) / 128;
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const unsigned m = __ballot_sync(0xffffffffu, tile < at + x);
+      if (m) {
+        const int l = __ffs((int)m) - 1;
+        found = b0 + l;
+        rt = tile - at - __shfl_sync(0xffffffffu, x - n, l);
+      }
+      at += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) {
+      s_where[0] = found;
+      s_where[1] = rt;
+    }
+  }
+  for (int i = threadIdx.x; i < p.sq.table_cols; i += kUnionThreads) table[i] = 0;
+  __syncthreads();
+  const int b = s_where[0], rt = s_where[1], item = tile * H + h;
+  if (b < 0) {
+    if (threadIdx.x == 0) p.list_count[item] = -1;
+    return;
+  }
+  Seq s = load_seq(p.sq, b);
+  clamp_len(p.sq, bs, s);
+  const int j0 = rt * 128 / group, j1 = min(s.rows, (rt * 128 + 127) / group + 1);
+  for (int v = threadIdx.x; v < (j1 - j0) * p.k; v += kUnionThreads) {
+    const int jl = v / p.k, e = v - jl * p.k, j = j0 + jl;
+    const int pg = __ldg(&p.pages[(int64_t)(s.row0 + j) * p.pages_row + (int64_t)h * p.pages_head + e]);
+    if (pg >= p.sq.table_cols) {
+      atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
+    } else if (pg >= 0 && (int64_t)pg * bs <= s.ctx + j) {
+      atomicOr(&table[pg], 1u << jl);
+    }
+  }
+  __syncthreads();
+  // in order of the pages: a thread's run of them, then the runs before it
+  const int per = (p.sq.table_cols + kUnionThreads - 1) / kUnionThreads, first = threadIdx.x * per;
+  int n = 0;
+  for (int i = first; i < min(first + per, p.sq.table_cols); ++i) n += table[i] != 0;
+  int x = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) s_sum[warp] = x;
+  __syncthreads();
+  int at = x - n, total = 0;
+  for (int w = 0; w < kUnionThreads / 32; ++w) {
+    if (w < warp) at += s_sum[w];
+    total += s_sum[w];
+  }
+  uint4* list = p.list + (int64_t)item * p.list_row;
+  const int32_t* trow = p.sq.table + (int64_t)b * p.sq.table_ld;
+  for (int i = first; i < min(first + per, p.sq.table_cols); ++i)
+    if (table[i]) list[at++] = make_uint4((uint32_t)i, table[i], (uint32_t)__ldg(&trow[i]), 0);
+  if (threadIdx.x == 0) {
+    p.list_count[item] = total;
+    if (h == 0) p.list_tile[tile] = make_int2(b, rt);
+  }
+}
+
+template <class T, int D, int MT, bool SPARSE>
 void wide_one(const AttendLaunch& p, int grid, cudaStream_t s) {
+  using W = Wide<D, MT, SPARSE>;
+  constexpr int bytes = wide_smem<D, MT, SPARSE>();
+  static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
-  static_assert(wide_smem<D, MT>() <= 227 * 1024, "shared memory of a CTA");
-  allow_smem(wide_kernel<T, D, MT>, wide_smem<D, MT>(), done);
-  wide_kernel<T, D, MT><<<grid, Wide<D, MT>::THREADS, wide_smem<D, MT>(), s>>>(p);
-  DARIC_CUDA(cudaGetLastError());
+  allow_smem(wide_kernel<T, D, MT, SPARSE>, bytes, done);
+  if (SPARSE) {
+    static std::atomic<uint64_t> ready{0};
+    allow_smem(union_kernel, kUnionPages * 4, ready);
+    union_kernel<<<dim3((unsigned)(p.lists / p.kv.heads), (unsigned)p.kv.heads), kUnionThreads, p.sq.table_cols * 4, s>>>(p);
+    DARIC_CUDA(cudaGetLastError());
+    launch_after(wide_kernel<T, D, MT, SPARSE>, dim3((unsigned)grid), W::THREADS, s, p, bytes);
+  } else {
+    wide_kernel<T, D, MT, SPARSE><<<grid, W::THREADS, bytes, s>>>(p);
+    DARIC_CUDA(cudaGetLastError());
+  }
   launch_after(wide_join_kernel<T, D, MT>, dim3((unsigned)grid, 4 * MT, D / 32), 256, s, p);
+}
+
+template <class T, int D>
+void wide_d(const AttendLaunch& p, int mt, int grid, cudaStream_t s) {
+  if (p.pages) return wide_one<T, D, 1, true>(p, grid, s);
+  mt == 2 ? wide_one<T, D, 2, false>(p, grid, s) : wide_one<T, D, 1, false>(p, grid, s);
 }
 
 template <class T>
 void wide_t(const AttendLaunch& p, int mt, int grid, cudaStream_t s) {
-  if (p.kv.head_dim == 64) return mt == 2 ? wide_one<T, 64, 2>(p, grid, s) : wide_one<T, 64, 1>(p, grid, s);
-  mt == 2 ? wide_one<T, 128, 2>(p, grid, s) : wide_one<T, 128, 1>(p, grid, s);
+  p.kv.head_dim == 64 ? wide_d<T, 64>(p, mt, grid, s) : wide_d<T, 128>(p, mt, grid, s);
 }
 
 }  // namespace

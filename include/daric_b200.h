@@ -304,8 +304,11 @@ DARIC_API int daric_ptrs_to_slots(int64_t num_ranges, const int64_t* range_start
 /* 16-byte aligned. Workspaces belong to one call at a time.                 */
 /* ======================================================================== */
 
-/* Bytes of workspace of one tree_attention or sparse_attention call. */
+/* Bytes of workspace of one tree_attention call, and of one sparse_attention
+ * call of the given sizes. */
 DARIC_API int daric_attend_workspace(int device, int64_t head_dim, int64_t* out_bytes);
+DARIC_API int daric_sparse_workspace(int device, int64_t head_dim, int64_t num_rows, int64_t num_seqs, int64_t q_heads,
+                           int64_t kv_heads, int64_t k, int64_t table_cols, int64_t* out_bytes);
 
 /* Softmax attention of each query row over its sequence. Row j of a sequence
  * with T rows and length s sees positions < s - T and, of the last T, token i
@@ -323,8 +326,9 @@ DARIC_API int daric_copier_tree_attention(daric_copier* copier, const char* laye
 
 /* The same over listed pages: pages[n*pages_row + h*pages_head + e], e < k,
  * are page numbers (block-table columns) of query row n and KV head h;
- * negative entries are empty, one past the block table is skipped (bit 4), a
- * page listed twice counts twice. A row sees listed positions up to its own. */
+ * ascending; negative entries are empty, one past the block table is skipped
+ * (bit 4), one that repeats the entry before it counts once. A row sees listed
+ * positions up to its own. */
 DARIC_API int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, int kv_dtype, const void* q,
                                   int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads, int64_t head_dim,
                                   const int32_t* pages, int64_t pages_row, int64_t pages_head, int64_t k,
