@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 from typing import Optional
 
 import torch
@@ -24,7 +25,12 @@ from .cache_ops import CacheCopier, kv_dtype_code
 
 __all__ = ["tree_attention", "sparse_attention"]
 
-_workspaces: dict[tuple, torch.Tensor] = {}
+class _Workspaces(threading.local):
+    def __init__(self):
+        self.of: dict[tuple, torch.Tensor] = {}
+
+
+_workspaces = _Workspaces()
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _capturing = torch.cuda.is_current_stream_capturing
 
@@ -101,18 +107,19 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _kept(key: tuple, kept: bool, dev: torch.device, size) -> torch.Tensor:
-    """Workspace of a call. Calls on one stream follow each other, so they
-    share one that is kept; a captured call has its own, which belongs to its
-    graph, and so has one on a stream given by its handle. ``size`` fills in
-    the bytes."""
+    """Workspace of a call. The calls of one thread on one stream follow each
+    other, so they share one that is kept (a call is several launches, and
+    those of two threads may take turns on a stream); a captured call has its
+    own, which belongs to its graph, and so has one on a stream given by its
+    handle. ``size`` fills in the bytes."""
     kept = kept and not _capturing()
-    ws = _workspaces.get(key) if kept else None
+    ws = _workspaces.of.get(key) if kept else None
     if ws is None:
         v = C.c_int64(0)
         check(size(C.byref(v)))
         ws = torch.empty(v.value, dtype=torch.uint8, device=dev)
         if kept:
-            _workspaces[key] = ws
+            _workspaces.of[key] = ws
     return ws
 
 
@@ -146,7 +153,8 @@ def tree_attention(copier: CacheCopier, layer_name: str, q: torch.Tensor, block_
     sees the first ``s - T`` positions and, of the last ``T`` (the drafted
     tokens), token ``i`` where bit ``i % 64`` of ``tree_mask[row, i // 64]`` is
     set; without a mask the tokens up to its own. Without ``cu_q`` the rows
-    divide evenly over the sequences. ``scale`` defaults to 1 / sqrt(head_dim).
+    divide evenly over the sequences. ``scale`` (positive) defaults to
+    1 / sqrt(head_dim). Nothing is recorded for a backward pass.
 
     Returns (out [rows, heads, head_dim], lse [rows, heads] float32: natural
     log of the sum of exp of the scaled logits). A row that sees nothing gets

@@ -115,7 +115,9 @@ Variant attend_variant(int64_t num_rows, int64_t num_seqs, int64_t group, int64_
   // over the pages that any of them lists. They read each page once then,
   // which is what bounds the row-by-row form (512 rows with 64 of 512 pages
   // each, no two lists alike: 265 us row by row).
-  if (k && wide && group >= 4 && num_rows * group >= 64 * num_seqs && table_cols <= kUnionPages) return variant_mt(1);
+  // (A list of more entries than a table has pages holds repeats; it goes row by row.)
+  if (k && wide && group >= 4 && num_rows * group >= 64 * num_seqs && table_cols <= kUnionPages && k <= kUnionPages)
+    return variant_mt(1);
   if (rows <= 16) return variant_rg(1, head_dim);
   if (rows <= 32 || k) return variant_rg(2, head_dim);
   if (!wide) return variant_rg(4, head_dim);
@@ -198,7 +200,7 @@ int daric_copier_tree_attention(daric_copier* copier, const char* layer_name, in
                      L.kv.page_size);
     if (num_rows == 0) return;
     DARIC_CHECK(q && out, "NULL query or output");
-    DARIC_CHECK(!tree_mask || mask_words >= 1, "tree mask needs at least one word per row");
+    DARIC_CHECK(!tree_mask || (mask_words >= 1 && mask_words <= (1 << 25)), "tree mask needs 1 to 2^25 words per row");
     DARIC_CHECK(aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
     DARIC_CHECK(aligned(out, out_row * 2, out_head * 2, 16), "output rows must be 16-byte aligned");
     const DeviceInfo di = device_info(device);
@@ -269,6 +271,7 @@ int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, 
     const double per_list = (double)std::max(k, room.row) * L.kv.page_size / 16.0 + 1.0;
     const double tiles = (double)L.kv.heads * (double)num_rows * ((double)p.sq.group / 16 + 1.0) * per_list;
     DARIC_CHECK(tiles < 4.0e9, "sparse_attention: the batch has too many tiles for one call");
+    DARIC_CHECK(!var.mt || num_rows * p.sq.group / var.rows < (1 << 18), "sparse_attention: too many query rows");
     const int grid = di.sm_count * var.ctas;
     attend_workspace(p, grid, var.rows, workspace, workspace_bytes);
     OnDevice on(device);
@@ -394,7 +397,7 @@ int daric_copier_attention_scores(daric_copier* copier, const char* layer_name, 
     p.sq = seq_batch(block_table, table_ld, num_seqs, table_cols, seq_lens, cu_q, num_rows, q_heads, L.kv.heads,
                      L.kv.page_size);
     DARIC_CHECK(scores && col_off && (q || num_rows == 0), "NULL query, scores or column offsets");
-    DARIC_CHECK(!tree_mask || mask_words >= 1, "tree mask needs at least one word per row");
+    DARIC_CHECK(!tree_mask || (mask_words >= 1 && mask_words <= (1 << 25)), "tree mask needs 1 to 2^25 words per row");
     DARIC_CHECK(num_rows == 0 || aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
     DARIC_CHECK(scores_cols >= 0 && (scores_row >= scores_cols || L.kv.heads == 1), "score rows overlap");
     const int64_t splits = (table_cols * L.kv.page_size + kLseKeys - 1) / kLseKeys;

@@ -39,7 +39,7 @@ def attention_scores(copier: CacheCopier, layer_name: str, q: torch.Tensor, bloc
 
     ``scores`` is float32 [KV heads, columns] with unit column stride,
     ``col_off`` int64 [sequences] on the device (the ``seg_col_off`` of
-    ``score_select``). ``lse`` is what :func:`daric_b200.attend.tree_attention`
+    ``score_select``); the columns of two sequences must not overlap. ``lse`` is what :func:`daric_b200.attend.tree_attention`
     returned for the same rows and mask; without it the log-sums are computed
     here. Rows with lse -inf add nothing. The sums have one fixed order.
     Returns ``scores``."""
@@ -85,7 +85,9 @@ def compact(copier: CacheCopier, layer_names: Sequence[str], keep: Selection, bl
             dst_start: Optional[Sequence[int]] = None, mode="none", stream: int = 0) -> None:
     """Moves the kept tokens of every segment to positions ``dst_start[s]``,
     ``dst_start[s] + 1``, ... of its block table, K and V, in place, all layers
-    per launch. Tokens that are not overwritten stay as they are.
+    per launch. Tokens that are not overwritten stay as they are. A block that
+    is written must belong to one segment only (shared blocks are copied
+    first, or left in front of ``dst_start``).
 
     ``keep`` is a :class:`daric_b200.select.Selection` (or one like it) whose
     ``idx`` rows hold ascending positions: one row per layer, or one row for

@@ -1,0 +1,134 @@
+"""The paged-cache operators as they are used together, and calls at once."""
+import math
+import threading
+
+import pytest
+import torch
+
+from daric_b200 import _lib
+from daric_b200.attend import sparse_attention, tree_attention
+from daric_b200.blocks import new_bounds, page_bounds, select_pages
+from daric_b200.evict import attention_scores
+from attend_util import Batch, attend64, check_attend
+from test_gpu_attend import check_sparse, check_tree, random_pages, run_tree
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kvh,group,t,bs", [(1, 40, 1, 16), (1, 160, 1, 16), (2, 150, 2, 256), (1, 300, 3, 1024)])
+def test_large_groups_and_blocks(kvh, group, t, bs):
+    bt = Batch([1500, 33], [t, t], kvh=kvh, group=group, bs=bs, seed=group)
+    check_tree(bt, *run_tree(bt))
+    pages = random_pages(bt, 2, torch.Generator().manual_seed(group)).cuda()
+    out, lse = sparse_attention(bt.copier, "l", bt.q, pages, bt.table, bt.seq_lens, cu_q=bt.cu_q)
+    assert _lib.device_errors(0) == 0
+    check_sparse(bt, pages.cpu(), out, lse)
+
+
+@pytest.mark.parametrize("dtype,layout,t", [("bf16", "5d", 40), ("f16", "4d", 3)])
+def test_prompt_rows_then_decode_steps(dtype, layout, t):
+    """The last rows of two prompts select and read pages, then decode steps
+    refresh the bounds of the page they wrote and do the same."""
+    bt = Batch([900 + t, 333 + t], [t, t], kvh=2, group=4, layout=layout, dtype=dtype, seed=t)
+    k = 9
+    lens = bt.seq_lens.clone()
+    bounds = page_bounds(bt.copier, "l", bt.table, lens)
+
+    def step(start=None):
+        page_bounds(bt.copier, "l", bt.table, lens, bounds, start=start)
+        pages = select_pages(bt.q, bounds, bt.table, lens, k, bt.bs, cu_q=bt.cu_q)
+        out, lse = sparse_attention(bt.copier, "l", bt.q, pages, bt.table, lens, cu_q=bt.cu_q)
+        assert _lib.device_errors(0) == 0
+        check_sparse(bt, pages.cpu(), out, lse)
+        # every row lists its own page, the first one, and as many as there are up to k
+        for b in range(2):
+            for j in range(bt.rows[b]):
+                own = (bt.lens[b] - bt.rows[b] + j) // bt.bs
+                for h in range(bt.kvh):
+                    row = pages[bt.cu[b] + j, h].tolist()
+                    have = [x for x in row if x >= 0]
+                    assert have == sorted(set(have)) and have[0] == 0 and have[-1] == own
+                    assert len(have) == min(k, own + 1) and row[len(have):] == [-1] * (k - len(have))
+        return pages
+
+    step()
+    bt.rows, bt.cu, bt.n, bt.cu_q = [1, 1], [0, 1, 2], 2, None
+    gen = torch.Generator().manual_seed(1)
+    for _ in range(3):  # tables have room for one more page each
+        start = lens.clone()
+        lens += 1
+        bt.lens = [n + 1 for n in bt.lens]
+        pos = start.long()
+        for b in range(2):
+            if bt.lens[b] % bt.bs == 1:  # a new page, the one block that is free (of one sequence at most)
+                bt.table[b, int(pos[b]) // bt.bs] = 0
+        blk = bt.table.long()[torch.arange(2), pos // bt.bs]
+        new = torch.randn((2, bt.kvh, bt.d), generator=gen).to(bt.cache.dtype).cuda()
+        bt.k[blk, pos % bt.bs] = new
+        bt.v[blk, pos % bt.bs] = -new
+        bt.q = torch.randn((2, bt.kvh * bt.group, bt.d), generator=gen).to(bt.cache.dtype).cuda()
+        step(start)
+    fresh = new_bounds(bt.copier, "l")
+    page_bounds(bt.copier, "l", bt.table, lens, fresh)
+    for b in range(2):
+        ids = bt.table[b, :-(-bt.lens[b] // bt.bs)].long()
+        assert torch.equal(bounds[ids], fresh[ids])
+
+
+def test_two_threads_on_one_stream():
+    """Calls of two threads take turns on the default stream: neither's parts
+    are joined into the other's rows."""
+    bts = [Batch([6000, 1200], [2, 2], kvh=2, group=4, seed=50), Batch([3500, 4400], [30, 30], kvh=2, group=4, seed=51)]
+    pages = [random_pages(b, 40, torch.Generator().manual_seed(3)).cuda() for b in bts]
+
+    def once(i):
+        b = bts[i]
+        a = tree_attention(b.copier, "l", b.q, b.table, b.seq_lens, cu_q=b.cu_q)
+        s = sparse_attention(b.copier, "l", b.q, pages[i], b.table, b.seq_lens, cu_q=b.cu_q)
+        return (*a, *s)
+
+    expect = [once(i) for i in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def many(i):
+        got = [once(i) for _ in range(60)]
+        torch.cuda.synchronize()
+        wrong.extend(i for g in got if not all(torch.equal(x, y) for x, y in zip(g, expect[i])))
+
+    threads = [threading.Thread(target=many, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and _lib.device_errors(0) == 0
+
+
+def test_two_streams_at_once():
+    bt = Batch([5000, 700], [2, 2], kvh=2, group=4, seed=52)
+    expect = run_tree(bt)
+    scores = torch.zeros((2, 5700), device="cuda")
+    off = torch.tensor([0, 5000], device="cuda")
+    attention_scores(bt.copier, "l", bt.q, bt.table, bt.seq_lens, scores, off, cu_q=bt.cu_q)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                o, z = tree_attention(bt.copier, "l", bt.q, bt.table, bt.seq_lens, cu_q=bt.cu_q)
+                w = attention_scores(bt.copier, "l", bt.q, bt.table, bt.seq_lens, torch.zeros_like(scores), off, cu_q=bt.cu_q)
+                got.append((o, z, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, expect[0]) and torch.equal(z, expect[1]) and torch.equal(w, scores) for o, z, w in got)
+
+
+def test_lists_longer_than_any_table():
+    """A list of more entries than the many-row form takes goes row by row."""
+    bt = Batch([130], [40], kvh=1, group=4, seed=53)
+    few = random_pages(bt, 4, torch.Generator().manual_seed(4), holes=False).cuda()
+    long = torch.full((40, 1, 50000), -1, dtype=torch.int32, device="cuda")
+    long[:, :, 49996:] = few
+    out, lse = sparse_attention(bt.copier, "l", bt.q, long, bt.table, bt.seq_lens, cu_q=bt.cu_q)
+    assert _lib.device_errors(0) == 0
+    check_sparse(bt, few.cpu(), out, lse)
