@@ -35,7 +35,7 @@
 // landed, some slots behind the newest.
 //
 // Bound: the K and V bytes and their latency up to 128 pairs (64 of them, 8K
-// keys x 16 sequences: 4.4 TB/s of K and V); above, the chain of two products
+// keys x 16 sequences: 4.3 TB/s of K and V); above, the chain of two products
 // and a tile's exponentials per stream, of which exp2 is 16 a clock and SM.
 // Why tcgen05 and not the warp matrix instructions here: from 33 pairs on
 // those need more time per key than its bytes do.
