@@ -105,6 +105,7 @@ struct SelectPagesLaunch {
   int32_t num_pages, heads, head_dim, page_size;
   int32_t k, first, last;
   int32_t chunk, sm_count;  // pages a CTA scores
+  int32_t chunks, staged;   // such CTAs of an item; whether its keys fit shared memory when it selects
   uint32_t* keys;         // workspace: [N, heads, keys_row] ordered scores
   int32_t keys_row;       // table_cols, whole 16-byte vectors
   float* mags;            // workspace: [N, heads, chunks] largest sum of |q||bound| of a chunk of pages

@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D > 128 ? 2 : 4) page_score_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = blockIdx.x, h = blockIdx.z, chunk = blockIdx.y;
   const int g = lane >> 2, t = lane & 3;
+  grid_next();
   const RowView rv = row_view(p.sq, p.page_size, n);
   if (rv.pages <= p.k || chunk * p.chunk >= rv.pages) return;  // every page is taken, or none is here
   const int group = p.sq.group;
@@ -423,7 +424,7 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectPagesLaunch&
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant__ SelectPagesLaunch p, int chunks, int staged) {
+__global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant__ SelectPagesLaunch p) {
   extern __shared__ uint32_t dyn[];  // [bitmap words | staged keys]
   __shared__ uint32_t hist[kBins];
   __shared__ int sm[32];
@@ -433,6 +434,7 @@ __global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant
   __shared__ int near_page[kNear];
   __shared__ unsigned long long near_key[kNear];
   const int n = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  grid_wait();
   const RowView rv = row_view(p.sq, p.page_size, n);
   if (rv.seq < 0) return;  // a row behind the last sequence
   int32_t* out = p.out + ((int64_t)n * p.heads + h) * p.k;
@@ -452,13 +454,13 @@ __global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant
   const int kk = p.k - p.first - p.last;
   if (tid == 0) s_near = s_in = 0;
   float mag = 0.f;
-  for (int i = tid; i < (P + p.chunk - 1) / p.chunk; i += blockDim.x) mag = fmaxf(mag, p.mags[item * chunks + i]);
+  for (int i = tid; i < (P + p.chunk - 1) / p.chunk; i += blockDim.x) mag = fmaxf(mag, p.mags[item * p.chunks + i]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
   if (lane == 0) sm[warp] = __float_as_int(mag);
-  if (staged)  // rows of keys are whole 16-byte vectors
+  if (p.staged)  // rows of keys are whole 16-byte vectors
     for (int i = tid; i < (P + 3) / 4; i += blockDim.x)
-      reinterpret_cast<uint4*>(skeys)[i] = __ldg(reinterpret_cast<const uint4*>(gkeys) + i);
+      reinterpret_cast<uint4*>(skeys)[i] = __ldcg(reinterpret_cast<const uint4*>(gkeys) + i);
   for (int i = tid; i < words; i += blockDim.x) taken[i] = 0;
   __syncthreads();
   if (tid == 0) {
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant
     s_e = mag * 6.103515625e-05f;  // E = 2^-14 of the largest magnitude
   }
   __syncthreads();
-  auto key_at = [&](int i) { return staged ? skeys[i] : gkeys[i]; };
+  auto key_at = [&](int i) { return p.staged ? skeys[i] : gkeys[i]; };
   const float E = s_e;
 
   if (kk > 0) {
@@ -687,25 +689,24 @@ void select_d(const SelectPagesLaunch& p0, cudaStream_t s) {
   while (p.chunk > kScoreChunk &&
          (int64_t)(p.sq.table_cols + p.chunk - 1) / p.chunk * p.sq.num_rows * p.heads < 4 * (int64_t)p.sm_count)
     p.chunk /= 2;
-  const int chunks = (p.sq.table_cols + p.chunk - 1) / p.chunk;
+  p.chunks = (p.sq.table_cols + p.chunk - 1) / p.chunk;
   if (p.sq.table_cols > p.k) {
     constexpr int bytes = kScoreStages * 2 * (D / 32) * kScoreWarps * 32 * 16;
     static std::atomic<uint64_t> ready{0};
     allow_smem(page_score_kernel<T, D>, bytes, ready);
     page_score_kernel<T, D>
-        <<<dim3((unsigned)p.sq.num_rows, (unsigned)chunks, (unsigned)p.heads), kScoreWarps * 32, bytes, s>>>(p);
+        <<<dim3((unsigned)p.sq.num_rows, (unsigned)p.chunks, (unsigned)p.heads), kScoreWarps * 32, bytes, s>>>(p);
     DARIC_CUDA(cudaGetLastError());
   }
   // keys are staged in shared memory while they fit
   const int words = ((p.sq.table_cols + 31) / 32 + 3) / 4 * 4;
-  const int staged = p.sq.table_cols <= 40960;
-  const int bytes = (words + (staged ? p.keys_row : 0)) * 4;
+  p.staged = p.sq.table_cols <= 40960;
+  const int bytes = (words + (p.staged ? p.keys_row : 0)) * 4;
   // a thread per eight keys, so that short tables keep many CTAs on an SM
   const int threads = std::min(1024, std::max(128, (p.sq.table_cols / 8 + 31) / 32 * 32));
   static std::atomic<uint64_t> done{0};
   allow_smem(page_select_kernel<T, D>, 190 * 1024, done);
-  page_select_kernel<T, D><<<dim3((unsigned)p.sq.num_rows, (unsigned)p.heads), threads, bytes, s>>>(p, chunks, staged);
-  DARIC_CUDA(cudaGetLastError());
+  launch_after(page_select_kernel<T, D>, dim3((unsigned)p.sq.num_rows, (unsigned)p.heads), threads, s, p, bytes);
 }
 
 }  // namespace

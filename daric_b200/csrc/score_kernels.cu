@@ -296,7 +296,7 @@ struct QueryBlock {
     if (threadIdx.x < kBlockRows) {
       const int pi = i0 + threadIdx.x, j = (int)fdiv((uint32_t)pi, p.sq.group_div);
       row[threadIdx.x] = s.row0 + j;
-      z[threadIdx.x] = pi < pairs && p.lse ? __ldg(&p.lse[(int64_t)(s.row0 + j) * p.lse_row + h * group + pi - j * group])
+      z[threadIdx.x] = pi < pairs && p.lse ? __ldcg(&p.lse[(int64_t)(s.row0 + j) * p.lse_row + h * group + pi - j * group])
                                            : DARIC_NEG_INF;
     }
     __syncthreads();
@@ -338,15 +338,17 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) weight_bloc
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int64_t col = __ldg(&p.col_off[b]);
-  if (col < 0 || col + s.len > p.scores_cols) {
-    if (threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
-    return;
-  }
+  const bool outside = col < 0 || col + s.len > p.scores_cols;
+  if (outside && threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
   const int pairs = s.rows * p.sq.group;
   const int key0 = ((int)blockIdx.y * kBlockWarps + warp) * KEYS;
-  if ((int)blockIdx.y * kBlockWarps * KEYS >= s.len) return;
+  if (outside || (int)blockIdx.y * kBlockWarps * KEYS >= s.len) {
+    grid_wait();  // none of a grid that was launched ahead ends before the one that it follows
+    return;
+  }
   KeyTile<D, M> kt;
-  kt.load(p, s, b, h, key0);
+  kt.load(p, s, b, h, key0);  // beside the log-sums, where those are computed here
+  grid_wait();
   const bool draft = key0 + KEYS > s.ctx;
   float sum[2 * M];  // keys g, g + 8, ...
 #pragma unroll
@@ -533,6 +535,7 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) lse_kernel(
 // lse of each query row and head from its parts (one warp each).
 __global__ void __launch_bounds__(256) lse_join_kernel(const __grid_constant__ ScoresLaunch p) {
   const int64_t items = (int64_t)p.sq.num_rows * p.kv.heads * p.sq.group;
+  grid_next();
   grid_wait();
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -592,7 +595,9 @@ void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
   if (pairs <= 16) return stream_n<T, D, 2>(p, s);
   constexpr int M = D > 128 ? 1 : 2;
   const unsigned tiles = (unsigned)((cap + kBlockWarps * 16 * M - 1) / (kBlockWarps * 16 * M));
-  weight_block_kernel<T, D, M><<<dim3((unsigned)p.kv.heads, tiles, (unsigned)p.sq.num_seqs), kBlockWarps * 32, 0, s>>>(p);
+  const dim3 grid((unsigned)p.kv.heads, tiles, (unsigned)p.sq.num_seqs);
+  if (!p0.lse) return launch_after(weight_block_kernel<T, D, M>, grid, kBlockWarps * 32, s, p);
+  weight_block_kernel<T, D, M><<<grid, kBlockWarps * 32, 0, s>>>(p);
   DARIC_CUDA(cudaGetLastError());
 }
 
