@@ -140,14 +140,42 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
   const int reps = turn && BYHEAD ? 1 : min(turn ? U : kMoveVecs, kMoveBatch / rows);  // tokens of a thread
   const int batch = rows * reps;                         // tokens of a batch
 
-  // Places of the next chunk of tokens, [ready, ready + kMoveTokens / 2).
-  int ready = 0;
+  // Places of the next chunk of tokens, [ready, ready + kMoveTokens / 2), in
+  // three steps, each a batch after the one before, so that no load is waited
+  // for: list entries, block ids, places.
+  constexpr int CT = kMoveTokens / 2 / kMoveThreads;  // tokens of a thread in a chunk
+  constexpr int kNoTable = -0x7fffffff - 1;           // a block id of no table entry
+  int ready = 0, step = 0;
+  int from_of[CT], prev_of[CT], blk_of[CT][2];
+  auto entries_of = [&]() {
+#pragma unroll
+    for (int k = 0; k < CT; ++k) {
+      const int i = ready + (int)threadIdx.x + k * kMoveThreads;
+      from_of[k] = i < count ? ld_ahead(&idx[i]) : 0;
+      prev_of[k] = i < count && i > 0 ? ld_ahead(&idx[i - 1]) : -1;
+    }
+  };
+  auto blocks_of = [&]() {
+#pragma unroll
+    for (int k = 0; k < CT; ++k) {
+      const int i = ready + (int)threadIdx.x + k * kMoveThreads, to = sg.dst + i;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int pos = e ? to : from_of[k];
+        const int64_t at = sg.blk_off + (int)fdiv((uint32_t)pos, p.page_div);
+        blk_of[k][e] = i < count && from_of[k] > to && at < p.table_numel ? ld_ahead(&p.block_table[at]) : kNoTable;
+      }
+    }
+  };
   auto places = [&]() {
-    for (int i = ready + (int)threadIdx.x; i < min(ready + kMoveTokens / 2, count); i += kMoveThreads) {
-      const int from = __ldg(&idx[i]), to = sg.dst + i;
+#pragma unroll
+    for (int k = 0; k < CT; ++k) {
+      const int i = ready + (int)threadIdx.x + k * kMoveThreads;
+      if (i >= count) break;
+      const int from = from_of[k], to = sg.dst + i;
       uint2 pl = make_uint2(kStays, 0);
       // a list that does not ascend, or would move a token up, is not moved in place
-      if (from < to || (i > 0 && __ldg(&idx[i - 1]) >= from)) {
+      if (from < to || prev_of[k] >= from) {
         atomicOr(p.err, DEV_ERR_INDEX_RANGE);
       } else if (from != to) {
         int64_t off[2] = {-1, -1};
@@ -155,11 +183,11 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
         for (int e = 0; e < 2; ++e) {
           const int pos = e ? to : from;
           const int pg = (int)fdiv((uint32_t)pos, p.page_div);
-          if (sg.blk_off + pg >= p.table_numel) {
+          const int blk = blk_of[k][e];
+          if (blk == kNoTable && sg.blk_off + pg >= p.table_numel) {
             atomicOr(p.err, DEV_ERR_INDEX_RANGE);
             continue;
           }
-          const int blk = __ldg(&p.block_table[sg.blk_off + pg]);
           if (blk < 0 || blk >= p.num_pages) {
             atomicOr(p.err, DEV_ERR_BLOCK_RANGE);
             continue;
@@ -217,13 +245,28 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
     if (turn && BYHEAD && place(w, 0).x != kStays)
       te.load(L.table, p.table_row, p.half_rot, s_from[i % kMoveTokens], sg.dst + i, c * NF);
   };
+  entries_of();
+  blocks_of();
   places();
 #pragma unroll
   for (int k = 0; k < ST - 1; ++k) load(k * batch, k);
   entries(0);
   int stage = 0;
   for (int w = 0; w < count; w += batch) {
-    if (w + ST * batch > ready && ready < count) places();
+    if (ready < count) {
+      if (step == 0 && w + (ST + 2) * batch > ready) {
+        entries_of();
+        step = 1;
+      } else if (step == 1) {
+        blocks_of();
+        step = 2;
+      }
+      if (w + ST * batch > ready) {  // a short way, where the first batches already reach here
+        if (step == 1) blocks_of();
+        places();
+        step = 0;
+      }
+    }
     load(w + (ST - 1) * batch, stage == 0 ? ST - 1 : stage - 1);
     cp_wait<ST - 1>();
     // Every load of this batch is done before its stores; the sources of
