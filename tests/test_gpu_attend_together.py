@@ -132,3 +132,45 @@ def test_lists_longer_than_any_table():
     out, lse = sparse_attention(bt.copier, "l", bt.q, long, bt.table, bt.seq_lens, cu_q=bt.cu_q)
     assert _lib.device_errors(0) == 0
     check_sparse(bt, few.cpu(), out, lse)
+
+
+FORMS = [(1, 4, 1), (1, 4, 5), (2, 4, 16), (1, 8, 33)]  # KV heads, group, rows: each form of the kernels
+
+
+@pytest.mark.parametrize("kvh,group,t", FORMS)
+@pytest.mark.parametrize("bs", [16, 24, 128])
+@pytest.mark.parametrize("layout", ["5d", "4d"])
+def test_slots_behind_the_length_do_not_matter(kvh, group, t, bs, layout):
+    """Whatever stands in the rest of the last page and in other blocks, NaN too."""
+    bt = Batch([300, 77, 129], [t, t, t], kvh=kvh, group=group, bs=bs, layout=layout, seed=t)
+    pages = random_pages(bt, 2, torch.Generator().manual_seed(t)).cuda()
+
+    def both():
+        return (*run_tree(bt), *sparse_attention(bt.copier, "l", bt.q, pages, bt.table, bt.seq_lens, cu_q=bt.cu_q))
+
+    used = torch.zeros((bt.nb, bs), dtype=torch.bool, device="cuda")
+    for b, n in enumerate(bt.lens):
+        pos = torch.arange(n, device="cuda")
+        used[bt.table[b].long()[pos // bs], pos % bs] = True
+    expect = both()
+    for x in (bt.k, bt.v):
+        x[~used] = math.nan
+    assert all(torch.equal(a, b) for a, b in zip(both(), expect))
+    assert _lib.device_errors(0) == 0
+
+
+@pytest.mark.parametrize("kvh,group,t", FORMS)
+@pytest.mark.parametrize("bs", [16, 24])
+def test_bad_blocks_in_every_form(kvh, group, t, bs):
+    """Keys of a block that is not there are keys that do not exist."""
+    bt = Batch([400, 200], [t, t], kvh=kvh, group=group, bs=bs, seed=t + bs)
+    clean = bt.table.clone()
+    bt.table[0, 2] = -5
+    bt.table[1, 4] = 1 << 30
+    out, lse = tree_attention(bt.copier, "l", bt.q, bt.table, bt.seq_lens, cu_q=bt.cu_q)
+    assert _lib.device_errors(0) == 1
+    bt.table = clean
+    for b, page in ((0, 2), (1, 4)):
+        k, v = bt.kv64(b)
+        ok = bt.sees(b) & (torch.arange(bt.lens[b], device="cuda") // bs != page)
+        check_attend(bt, out, lse, b, *attend64(bt.q64(b), k, v, ok.repeat(group, 1)[None], 1 / math.sqrt(bt.d)))
