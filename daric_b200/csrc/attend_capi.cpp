@@ -114,7 +114,7 @@ Variant attend_variant(int64_t num_rows, int64_t num_seqs, int64_t group, int64_
   // tile no more than 32 rows (a bit each), the rows of a tile share one pass
   // over the pages that any of them lists. They read each page once then,
   // which is what bounds the row-by-row form (512 rows with 64 of 512 pages
-  // each, no two lists alike: 265 us row by row, 158 us shared).
+  // each, no two lists alike: 265 us row by row, 190 us shared).
   // (A list of more entries than a table has pages holds repeats; it goes row by row.)
   if (k && wide && group >= 4 && num_rows * group >= 64 * num_seqs && table_cols <= kUnionPages && k <= kUnionPages)
     return variant_mt(1);

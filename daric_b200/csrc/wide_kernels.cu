@@ -16,33 +16,18 @@
 // Two streams of (scores, weights, output) take turns, so that one is
 // multiplied while the other is exponentiated: with MT = 2 the two row tiles,
 // with MT = 1 the even and the odd key tiles, whose two outputs are joined at
-// the end of a segment. A copy slot is a K or a V tile in the 128-byte
-// swizzle, and the slots form one ring.
+// the end of a segment. Warps: four of softmax per stream, one thread a row;
+// four that copy; one that issues the matrix instructions. A copy slot is a K
+// or a V tile (16-byte cp.async, a page table lookup per key, into the
+// 128-byte swizzle); each copying thread reports a slot when its own copies of
+// it have landed, some slots behind the newest.
 //
-// Warps: eight of softmax, four a stream, one thread a row; one or two that
-// issue the matrix instructions; the others copy, in one of two ways:
-// * MT = 1 where pages are boxes of a tensor map (TMA): one warp has K copied
-//   by cp.async.bulk.tensor (a box of up to 128 tokens x 64 dimensions of a
-//   page), four copy V by 16-byte cp.async, one the query rows. A box of a
-//   16-token page costs the SM's copy unit some 100 clocks whatever its 2 KB,
-//   so that K and V both by boxes, or both by 16-byte copies, leave the rest
-//   waiting (128 pairs a tile, 512 rows with 64 of 512 pages each: 189, 190
-//   and, split, 177 us; 16 x 16 drafted rows at 8K: 120, 116, 108 us).
-// * else (other page sizes, and MT = 2, where a tile serves twice the rows and
-//   copies are not what is waited for: 105 us split, 99 so, 512 pairs at 32K
-//   keys) four warps copy both, a page table lookup per key.
-// A thread that copies reports a slot when its own 16-byte copies of it have
-// landed, some slots behind the newest.
-//
-// Bound: the K and V bytes and their latency up to 128 pairs (64 of them, 8K
-// keys x 16 sequences: 4.3 TB/s of K and V); above, the chain of two products
-// and a tile's exponentials per stream, of which exp2 is 16 a clock and SM.
-// Why tcgen05 and not the warp matrix instructions here: from 33 pairs on
-// those need more time per key than its bytes do.
+// Bound: the K and V bytes up to about 256 pairs; above, exp2 (16 a clock and
+// SM) and the matrix rate together. Why tcgen05 and not the warp matrix
+// instructions here: from 33 pairs on those need more time per key than its
+// bytes do.
 #include "attend_common.cuh"
 #include "tensor_common.cuh"
-
-#include <cuda.h>  // types of the tensor map; its encoder is looked up at run time
 
 #include <algorithm>
 #include <type_traits>
@@ -52,7 +37,6 @@ namespace {
 using namespace att;
 using bulk::fence_proxy_async;
 using bulk::mbar_arrive;
-using bulk::mbar_arrive_expect_tx;
 using bulk::mbar_init;
 using bulk::mbar_init_fence;
 using bulk::mbar_try_wait;
@@ -71,9 +55,7 @@ struct Wide {
   static constexpr int BEHIND = NS > 5 ? 3 : 2;  // slots copied but not reported yet
   static constexpr int THREADS = 512;  // the last three warps only lend their registers
   static constexpr int COPY_WARP = 8;
-  static constexpr int MMA_WARP = 12;    // MT = 1: of the first stream; 13: of the second
-  static constexpr int V_WARP = 14;      // TMA: copies V with the warps 9 to 11
-  static constexpr int QUERY_WARP = 15;  // TMA: copies query rows
+  static constexpr int MMA_WARP = 12;
   static constexpr int TILES = QB + NS * SLOT;
 };
 
@@ -94,54 +76,7 @@ struct SparseShared {
 };
 template <int D, int MT, bool SPARSE>
 constexpr int wide_smem() {
-  static_assert(sizeof(WideShared) % 16 == 0, "the masks behind it are read as vectors");
   return Wide<D, MT, SPARSE>::TILES + (int)sizeof(WideShared) + (SPARSE ? (int)sizeof(SparseShared) : 0);
-}
-
-// TMA: a page of one head (128 tokens of it at most) is a box of a tensor map
-// of the layer, (dimension, token, head, block, K or V), for each 64 dimensions.
-struct WideLaunch : AttendLaunch {
-  alignas(64) CUtensorMap map;
-  int32_t box_log;  // tokens of a box: 8 to 128
-};
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int blk, int kv,
-                                         uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
-      "[%7];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(tok), "r"(head), "r"(blk), "r"(kv), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
-}
-
-// Two fp32 values in one register pair, and the larger of three.
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // The part of a segment that a CTA works on.
@@ -153,8 +88,8 @@ struct Part {
   const uint4* list;      // SPARSE: page, rows of the tile that see it, block
 };
 
-template <class T, int D, int MT, bool SPARSE, bool TMA>
-__global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ WideLaunch p) {
+template <class T, int D, int MT, bool SPARSE>
+__global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ AttendLaunch p) {
   using W = Wide<D, MT, SPARSE>;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int HB = D / 64;          // 64-element halves of a row
@@ -229,15 +164,14 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
       mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.o_empty[i], 128);
     }
-    mbar_init(&sh.q_full, TMA ? 32 : kCopyThreads);
-    mbar_init(&sh.q_empty, MT == 2 ? 1 : 2);
+    mbar_init(&sh.q_full, kCopyThreads);
+    mbar_init(&sh.q_empty, 1);
     mbar_init(&sh.ml_full, 128);
     mbar_init_fence();
     sh.abort = 0;
     for (int i = 0; i < 4; ++i) sh.poison[i] = -1;
   }
-  if (TMA) fence_proxy_async();  // the copies that follow are written over the sums
-  __syncthreads();               // sums are read, barriers are ready
+  __syncthreads();  // sums are read, barriers are ready
   if (t0 >= t1 || (smem_u32(base) & 1023)) return;
   if (warp == W::MMA_WARP) tc::alloc512(&sh.tmem);
   tc::fence_before();
@@ -312,298 +246,50 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
   auto k_slot = [&](int i) { return MT == 2 ? 2 * i : (i == 0 ? 0 : 2 * i - 1); };
   auto v_slot = [&](int i, int n) { return MT == 2 ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
 
-  constexpr int CH = D / 8, RPI = kCopyThreads / CH;  // vectors of a row, rows that 128 threads take at a time
-  // V rows that some rows must not see: values without a finite size would
-  // reach them through 0 * inf. They are taken out here and added where
-  // they are seen, at the end of the segment.
-  auto take_out_rows = [&](int st, uint32_t seg, int c, int r0, auto step, auto count) {  // vector c of the rows r0 + k step
-    constexpr int ST = decltype(step)::value, N = decltype(count)::value;
-    uint8_t* tile = slots + st * W::SLOT + (c >> 3) * HALF;
-    auto vec = [&](int k) {
-      const int r = r0 + k * ST;
-      return reinterpret_cast<uint4*>(tile + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-    };
-    // x * 0 summed up: 0, or NaN where some x is not finite
-    uint32_t sum = 0;
-#pragma unroll
-    for (int k0 = 0; k0 < N; k0 += 8) {
-      uint4 x[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = *vec(k0 + k);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        sum = Mma<T>::zero_sum(x[k].x, Mma<T>::zero_sum(x[k].y, Mma<T>::zero_sum(x[k].z, Mma<T>::zero_sum(x[k].w, sum))));
-    }
-    if ((sum & 0x7fff7fffu) == 0) return;
-    for (int k = 0; k < N; ++k) {
-      uint16_t* v = reinterpret_cast<uint16_t*>(vec(k));
-      for (int e = 0; e < 8; ++e)
-        if ((v[e] & Mma<T>::kExpMask) == Mma<T>::kExpMask) v[e] = 0;
-    }
-    *(volatile int*)&sh.poison[seg & 3] = (int)seg;
-  };
-  // query rows of a part, by the thread ct of n
-  auto copy_queries = [&](const Part& g, int ct, int n) {
-    for (int v = ct; v < W::ROWS * CH; v += n) {
-      const int r = v / CH, c = v % CH, i = g.row_base + r;
-      const bool in = r < g.my_rows;
-      const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
-      const uint8_t* src = in ? p.q + (int64_t)(g.s.row0 + j) * p.q_row + (int64_t)(g.h * group + i - j * group) * p.q_head + c * 16
-                              : p.q;
-      const uint32_t dst = smem_u32(q_tile) + (r >> 7) * (HB * HALF) + (c >> 3) * HALF + (r & 127) * 128 +
-                           (((c & 7) ^ (r & 7)) << 4);
-      cp16(dst, src, in);
-    }
-  };
-  if (TMA) {  // the first part's by all threads, before the roles part
-    Part g;
-    if (part_at(t0, g)) copy_queries(g, tid, W::THREADS);
-    cp_commit();
-    cp_wait<0>();
-    fence_proxy_async();
-    __syncthreads();
-  }
-  // whether a V tile goes through take_out (SPARSE: always; else where not
-  // every row sees every key, the sequence's last tile among them)
-  auto mended = [&](const Part& g, int i, int see) { return SPARSE || (g.tile0 + i + 1) * kKeys > see; };
-
   // items of stream s in a part of n key tiles, and the key tile of its local item
   auto items_of = [&](int s, int n) { return MT == 2 ? n : (n + 1 - s) / 2; };
 
-  // Registers: 512 threads start with 128 each, 65536 in all; 256 x 176 of
-  // softmax + 256 x 80 of the others = 65536.
-  if (warp >= W::COPY_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  if (TMA && warp == W::COPY_WARP) {
-    // -------------------------------------------------------- copies of K --
-    const int np = kKeys >> p.box_log, bt = 1 << p.box_log;  // boxes of a tile and half, their tokens
-    uint32_t n_slot = 0, n_tile = 0, last = 0;
-    uint32_t t = t0;
-    bool ok = true;
-    while (ok && t < t1) {
-      Part g;
-      if (!part_at(t, g)) break;
-      const int32_t* trow = p.sq.table + (int64_t)g.b * p.sq.table_ld;
-      const int my_pos = SPARSE ? g.s.ctx + (int)fdiv((uint32_t)g.row_base, p.sq.group_div) + lane : 0;  // of row `lane`
-      // a lane is a box of the next tile: its block, first token of it,
-      // position, and (SPARSE) the rows that list it
-      int nxt_blk, nxt_tok, nxt_pos;
-      uint32_t nxt_rows;
-      auto lookup = [&](int i) {
-        nxt_blk = -1;
-        nxt_tok = 0;
-        nxt_pos = 0x7fffffff;
-        nxt_rows = 0;
-        if (i >= g.n || lane >= np) return;
-        const int k = (g.tile0 + i) * kKeys + lane * bt;
-        const int e = (int)fdiv((uint32_t)k, p.kv.page_div);
-        nxt_tok = k - e * p.kv.page_size;
-        if (SPARSE) {
-          if (e < g.listed) {
-            const int4 x = ld_ahead(reinterpret_cast<const int4*>(g.list + e));
-            nxt_pos = x.x * p.kv.page_size + nxt_tok;
-            nxt_rows = (uint32_t)x.y;
-            nxt_blk = x.z;
-          }
-        } else {
-          nxt_pos = k;
-          if (k < g.s.len) nxt_blk = ld_ahead(&trow[e]);
-        }
-      };
-      int blk = 0, tok = 0;  // of the tile
-      auto place = [&](int i) {  // boxes and masks of tile i; looks the next one up
-        bool in = nxt_pos < g.s.len;
-        if (in && (nxt_blk < 0 || nxt_blk >= p.kv.num_pages)) {
-          atomicOr(p.sq.err, DEV_ERR_BLOCK_RANGE);
-          in = false;
-        }
-        blk = in ? nxt_blk : p.kv.num_pages;  // a block that is not there reads as zeros
-        tok = nxt_tok;
-        if (SPARSE) {
-          // lane: a row of the tile; bits: the keys it sees, of pages that
-          // list it up to its own position
-          uint32_t see_w[4];
-          const uint32_t rows = in ? nxt_rows : 0;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            see_w[w] = 0;
-            for (int s = 0; s < 32; s += bt) {
-              const int e = (w * 32 + s) >> p.box_log, off = (w * 32 + s) & (bt - 1);
-              const uint32_t r = __shfl_sync(0xffffffffu, rows, e);
-              const int pos0 = __shfl_sync(0xffffffffu, nxt_pos, e);
-              const int c = (r >> lane) & 1u ? min(max(my_pos - pos0 - off + 1, 0), min(bt, 32)) : 0;
-              see_w[w] |= (c == 32 ? 0xffffffffu : (1u << c) - 1u) << s;
-            }
-          }
-          *reinterpret_cast<uint4*>(sp.vis[(n_tile + i) % kMaskRing][lane]) = make_uint4(see_w[0], see_w[1], see_w[2], see_w[3]);
-        } else {
-          const int have = in ? min(bt, g.s.len - nxt_pos) : 0;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int k = w * 32 + lane;
-            const int n = __shfl_sync(0xffffffffu, have, k >> p.box_log);
-            const unsigned m = __ballot_sync(0xffffffffu, (k & (bt - 1)) < n);
-            if (lane == 0) sh.vmask[(n_tile + i) % kMaskRing][w] = m;
-          }
-        }
-        lookup(i + 1);
-        __syncwarp();
-      };
-      lookup(0);
-      for (int i = 0; i < g.n; ++i) {
-        place(i);
-        const uint32_t x = n_slot + (uint32_t)k_slot(i), st = x % W::NS, use = x / W::NS;
-        if (use) ok = __all_sync(0xffffffffu, wait(&sh.empty[st], (use - 1) & 1));
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&sh.full[st], W::SLOT);
-          mbar_arrive_n(&sh.full[st], kCopyThreads - 1);
-        }
-        __syncwarp();
-        if (lane < np) {
-          const uint32_t dst = smem_u32(slots) + st * W::SLOT + ((uint32_t)lane << p.box_log) * 128;
-#pragma unroll
-          for (int hf = 0; hf < HB; ++hf) load_box(dst + hf * HALF, &p.map, hf * 64, tok, g.h, blk, 0, &sh.full[st]);
-        }
-        __syncwarp();
-        last = x + 1;
-      }
-      n_slot += 2 * (uint32_t)g.n;
-      n_tile += (uint32_t)g.n;
-      t += (uint32_t)g.n;
-    }
-    // A wait gave up: no box may land after the block has ended. (Else every
-    // slot was waited for by the products.)
-    if (!ok)
-      for (uint32_t k = last > (uint32_t)W::NS ? last - W::NS : 0; k < last; ++k)
-        mbar_wait(&sh.full[k % W::NS], (k / W::NS) & 1);
-    __syncwarp();
-  } else if (TMA && ((warp > W::COPY_WARP && warp < W::MMA_WARP) || warp == W::V_WARP)) {
-    // -------------------------------------------------------- copies of V --
-    // The boxes of K keep the copy unit of the SM busy; V goes by 16-byte
-    // copies beside it, 32 keys a warp, each reported by the thread that made
-    // it once it has landed, some tiles behind the newest.
-    constexpr int VB = W::NS > 5 ? 2 : 1, RPW = 32 / CH;
-    const int key0 = (warp == W::V_WARP ? 0 : warp - W::COPY_WARP) * 32;
-    const int c = lane % CH, r0 = key0 + lane / CH;
-    const uint32_t at0 = smem_u32(slots) + (c >> 3) * HALF + r0 * 128;
-    uint32_t n_slot = 0, n_seg = 0;
-    int pend[VB];       // slots not reported yet, older first; -1: none
-    uint32_t pend_seg[VB];
-    bool pend_mend[VB];
-#pragma unroll
-    for (int k = 0; k < VB; ++k) {
-      pend[k] = -1;
-      pend_seg[k] = 0;
-      pend_mend[k] = false;
-    }
-    auto report = [&](int k) {
-      if (pend[k] < 0) return;
-      if (pend_mend[k]) take_out_rows(pend[k], pend_seg[k], c, r0, std::integral_constant<int, RPW>(), std::integral_constant<int, 32 / RPW>());
-      fence_proxy_async();
-      mbar_arrive(&sh.full[pend[k]]);
-      pend[k] = -1;
-    };
-    auto flush = [&]() {
-      cp_wait<0>();
-#pragma unroll
-      for (int k = 0; k < VB; ++k) report(k);
-    };
-    uint32_t t = t0;
-    bool ok = true;
-    while (ok && t < t1) {
-      Part g;
-      if (!part_at(t, g)) break;
-      const int32_t* trow = p.sq.table + (int64_t)g.b * p.sq.table_ld;
-      const uint8_t* src = p.kv.base + (int64_t)g.h * p.kv.head_stride + p.kv.v_off + c * 16;
-      const int see = all_see(g);
-      int blk, in_page, pos;  // of this lane's key of the next tile
-      auto lookup = [&](int i) {
-        blk = -1;
-        in_page = 0;
-        pos = 0x7fffffff;
-        if (i >= g.n) return;
-        const int k = (g.tile0 + i) * kKeys + key0 + lane;
-        const int e = (int)fdiv((uint32_t)k, p.kv.page_div);
-        in_page = k - e * p.kv.page_size;
-        if (SPARSE) {
-          if (e < g.listed) {
-            const int4 x = ld_ahead(reinterpret_cast<const int4*>(g.list + e));
-            pos = x.x * p.kv.page_size + in_page;
-            blk = x.z;
-          }
-        } else {
-          pos = k;
-          if (k < g.s.len) blk = ld_ahead(&trow[e]);
-        }
-      };
-      lookup(0);
-      for (int i = 0; i < g.n; ++i) {
-        const bool in = pos < g.s.len && blk >= 0 && blk < p.kv.num_pages;  // K's copies report a bad block
-        const uint32_t off = in ? (uint32_t)(((int64_t)blk * p.kv.page_stride + (int64_t)in_page * p.kv.tok_stride) >> 4)
-                                : 0xffffffffu;
-        lookup(i + 1);
-        const uint32_t x = n_slot + (uint32_t)v_slot(i, g.n), st = x % W::NS, use = x / W::NS;
-        if (use && !__all_sync(0xffffffffu, tc::mbar_test(&sh.empty[st], (use - 1) & 1))) {
-          flush();  // what is reported late must not be waited for
-          ok = __all_sync(0xffffffffu, wait(&sh.empty[st], (use - 1) & 1));
-          if (!ok) break;
-        }
-#pragma unroll
-        for (int k = 0; k < 32 / RPW; ++k) {
-          const uint32_t o = __shfl_sync(0xffffffffu, off, k * RPW + lane / CH);
-          const int r7 = (r0 + k * RPW) & 7;
-          cp16(at0 + st * W::SLOT + k * RPW * 128 + (((c & 7) ^ r7) << 4), src + (o != 0xffffffffu ? (int64_t)o * 16 : 0),
-               o != 0xffffffffu);
-        }
-        cp_commit();
-        cp_wait<VB>();
-        report(0);
-#pragma unroll
-        for (int k = 0; k + 1 < VB; ++k) {
-          pend[k] = pend[k + 1];
-          pend_seg[k] = pend_seg[k + 1];
-          pend_mend[k] = pend_mend[k + 1];
-        }
-        pend[VB - 1] = (int)st;
-        pend_seg[VB - 1] = n_seg;
-        pend_mend[VB - 1] = mended(g, i, see);
-      }
-      n_slot += 2 * (uint32_t)g.n;
-      ++n_seg;
-      t += (uint32_t)g.n;
-    }
-    flush();
-    __syncwarp();
-  } else if (TMA && warp >= W::QUERY_WARP) {
-    // ---------------------------------------------------------- query rows --
-    uint32_t n_seg = 0;
-    uint32_t t = t0;
-    while (t < t1) {
-      Part g;
-      if (!part_at(t, g)) break;
-      if (n_seg) {
-        if (!__all_sync(0xffffffffu, wait(&sh.q_empty, (n_seg - 1) & 1))) break;
-        copy_queries(g, lane, 32);
-        cp_commit();
-        cp_wait<0>();
-        fence_proxy_async();
-        mbar_arrive(&sh.q_full);
-      }
-      ++n_seg;
-      t += (uint32_t)g.n;
-    }
-    __syncwarp();
-  } else if (!TMA && warp >= W::COPY_WARP && warp < W::MMA_WARP) {
+  if (warp >= W::COPY_WARP && warp < W::MMA_WARP) {
     // ------------------------------------------------------------ copies --
+    // Registers: 512 threads start with 128 each, 65536 in all; 256 x 176 of
+    // softmax + 128 x 80 here + 128 x 80 = 65536.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int ct = tid - W::COPY_WARP * 32;
     uint32_t n_slot = 0, n_seg = 0, n_tile = 0;  // slots, segments, key tiles so far
     constexpr int BH = W::BEHIND;
+    constexpr int CH = D / 8, RPI = kCopyThreads / CH;  // vectors of a row, rows at a time
     uint64_t* pend[BH];                          // groups not reported yet, older first
     int pend_v[BH], pend_seg[BH];                // SPARSE: their slot if it is a V tile, and the segment
 #pragma unroll
     for (int i = 0; i < BH; ++i) pend[i] = nullptr;
+    // V rows that some rows must not see: values without a finite size would
+    // reach them through 0 * inf. They are taken out here and added where
+    // they are seen, at the end of the segment.
     auto take_out = [&](int st, uint32_t seg) {
-      take_out_rows(st, seg, ct % CH, ct / CH, std::integral_constant<int, RPI>(), std::integral_constant<int, kKeys / RPI>());
+      const int c = ct % CH, r0 = ct / CH;
+      uint8_t* tile = slots + st * W::SLOT + (c >> 3) * HALF;
+      auto vec = [&](int k) {
+        const int r = r0 + k * RPI;
+        return reinterpret_cast<uint4*>(tile + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      };
+      // x * 0 summed up: 0, or NaN where some x is not finite
+      uint32_t sum = 0;
+#pragma unroll
+      for (int k0 = 0; k0 < kKeys / RPI; k0 += 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = *vec(k0 + k);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          sum = Mma<T>::zero_sum(x[k].x, Mma<T>::zero_sum(x[k].y, Mma<T>::zero_sum(x[k].z, Mma<T>::zero_sum(x[k].w, sum))));
+      }
+      if ((sum & 0x7fff7fffu) == 0) return;
+      for (int k = 0; k < kKeys / RPI; ++k) {
+        uint16_t* v = reinterpret_cast<uint16_t*>(vec(k));
+        for (int e = 0; e < 8; ++e)
+          if ((v[e] & Mma<T>::kExpMask) == Mma<T>::kExpMask) v[e] = 0;
+      }
+      *(volatile int*)&sh.poison[seg & 3] = (int)seg;
     };
     auto report = [&](uint64_t* bar, int v_slot_of, int seg) {
       if (!bar) return;
@@ -661,7 +347,17 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
       if (n_seg) ok = together(take(&sh.q_empty, (n_seg - 1) & 1));
       if (!ok) break;
       {
-        copy_queries(g, ct, kCopyThreads);
+        for (int v = ct; v < W::ROWS * CH; v += kCopyThreads) {
+          const int r = v / CH, c = v % CH, i = g.row_base + r;
+          const bool in = r < g.my_rows;
+          const int j = (int)fdiv((uint32_t)i, p.sq.group_div);
+          const uint8_t* src = in ? p.q + (int64_t)(g.s.row0 + j) * p.q_row +
+                                        (int64_t)(g.h * group + i - j * group) * p.q_head + c * 16
+                                  : p.q;
+          const uint32_t dst = smem_u32(q_tile) + (r >> 7) * (HB * HALF) + (c >> 3) * HALF + (r & 127) * 128 +
+                               (((c & 7) ^ (r & 7)) << 4);
+          cp16(dst, src, in);
+        }
         push(&sh.q_full, -1);
       }
       // this thread's key of the next tile: block (-1: none), position, and
@@ -742,7 +438,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
           const int r7 = (ct / CH + k * RPI) & 7;
           cp16(d0 + k * RPI * 128 + (((c & 7) ^ r7) << 4), src + (in ? (int64_t)o[k] * 16 : 0), in);
         }
-        if (!SPARSE && v_tile && mended(g, i, see)) {
+        if (!SPARSE && v_tile && (g.tile0 + i + 1) * kKeys > see) {
           cp_commit();
           cp_wait<0>();
           take_out((int)st, n_seg);
@@ -777,26 +473,28 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
     cp_wait<0>();
   } else if (warp >= W::MMA_WARP) {
     // ---------------------------------------------------------- products --
-    // MT = 2: one warp issues the products of both streams in turn, which
-    // keeps them half a tile apart, so that one is exponentiated while the
-    // other is multiplied (two warps: 98 -> 118 us for 512 pairs at 32K keys).
-    // MT = 1: each stream waits for its own key tiles and has its own warp.
-    if (warp < W::MMA_WARP + (MT == 2 ? 1 : 2)) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == W::MMA_WARP) {
       constexpr uint32_t id_qk = tc::instr_desc(BF, false, 128, kKeys), id_pv = tc::instr_desc(BF, true, 128, D);
-      const uint32_t own = tc::uniform((uint32_t)(warp - W::MMA_WARP)), tm = tc::uniform(tmem);
+      // The tensor pipe runs dry while this warp does anything else, so the
+      // loop is kept short: ring places move by addition, a slot is waited
+      // for once.
+      uint32_t at = 0, at_par = 0;  // slot of the segment's first tile and its parity
+      uint32_t n_seg = 0;
+      uint32_t p_par[2] = {0, 0}, o_par[2] = {0, 0}, o_used = 0;
       const uint64_t q_desc = tc::smem_desc(smem_u32(q_tile), 16), k_desc = tc::smem_desc(smem_u32(slots), 16),
                      v_desc = tc::smem_desc(smem_u32(slots), HALF);
-      uint32_t at = 0, at_par = 0;  // slot of the segment's first tile and its parity
-      uint32_t n_seg = 0, p_par = 0, o_par = 0, o_used = 0;  // the last three: a bit for each stream
-      auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+      const uint32_t tm = tc::uniform(tmem);
+      auto commit = [&](uint64_t* bar) {
+        if (tc::elect()) tc::commit(bar);
+      };
       uint32_t t = t0;
       bool ok = true;
       while (ok && t < t1) {
         Part g;
         if (!part_at(t, g)) break;
         const int n = (int)tc::uniform((uint32_t)g.n);
-        // a place of the ring: slot and parity of its use, which move by
-        // addition: nothing but the products may keep the tensor pipe waiting
+        // a place of the ring: slot and the parity of its use
         struct Place {
           uint32_t st, par;
         };
@@ -807,108 +505,113 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
             x.par ^= 1;
           }
         };
-        auto full = [&](const Place& x) { return all_wait(&sh.full[x.st], x.par); };
-        // scores of stream s; done: the slot's last reader, last: and the queries'
-        auto qk = [&](uint32_t s, const Place& x, bool done, bool last) {
+        Place first{at, at_par};
+        auto full = [&](const Place& x) { return __all_sync(0xffffffffu, wait(&sh.full[x.st], x.par)) != 0; };
+        auto qk = [&](uint32_t s, const Place& k) {  // scores of stream s with the K tile of a place
           const uint64_t qa = q_desc + (MT == 2 ? s * (uint32_t)(HB * HALF >> 4) : 0u);
-          const uint64_t ka = k_desc + tc::uniform(x.st) * (uint32_t)(W::SLOT >> 4);
+          const uint64_t ka = k_desc + tc::uniform(k.st) * (uint32_t)(W::SLOT >> 4);
           if (tc::elect()) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const int o = (k >> 2) * (HALF >> 4) + (k & 3) * (32 >> 4);
-              tc::mma_ss(tm + s * kKeys, qa + o, ka + o, id_qk, k > 0);
+            for (int i = 0; i < D / 16; ++i) {
+              const int o = (i >> 2) * (HALF >> 4) + (i & 3) * (32 >> 4);
+              tc::mma_ss(tm + s * kKeys, qa + o, ka + o, id_qk, i > 0);
             }
             tc::commit(&sh.s_full[s]);
-            if (done) tc::commit(&sh.empty[x.st]);
-            if (last) tc::commit(&sh.q_empty);
           }
         };
-        // output of stream s, added to what is there
-        auto pv = [&](uint32_t s, const Place& x, bool add, bool done) {
-          const uint64_t va = v_desc + tc::uniform(x.st) * (uint32_t)(W::SLOT >> 4);
+        auto pv = [&](uint32_t s, const Place& v, bool add) {
+          const uint64_t va = v_desc + tc::uniform(v.st) * (uint32_t)(W::SLOT >> 4);
           if (tc::elect()) {
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              tc::mma_ts(tm + 2 * kKeys + s * D, tm + s * kKeys + k * 8, va + k * (2048 >> 4), id_pv, add || k > 0);
+            for (int i = 0; i < kKeys / 16; ++i)
+              tc::mma_ts(tm + 2 * kKeys + s * D, tm + s * kKeys + i * 8, va + i * (2048 >> 4), id_pv, add || i > 0);
             tc::commit(&sh.pv_done[s]);
-            if (done) tc::commit(&sh.empty[x.st]);
           }
         };
         // weights of a stream are there, and before a segment's first product
         // its output has been read
-        auto weights = [&](uint32_t s, bool first) {
-          if (first) {
-            if ((o_used >> s) & 1) {
-              if (!all_wait(&sh.o_empty[s], (o_par >> s) & 1)) return false;
-              o_par ^= 1u << s;
-            }
-            o_used |= 1u << s;
+        auto weights = [&](uint32_t s, bool first_item) {
+          if (first_item && ((o_used >> s) & 1)) {
+            if (!__all_sync(0xffffffffu, wait(&sh.o_empty[s], o_par[s]))) return false;
+            o_par[s] ^= 1;
           }
-          if (!all_wait(&sh.p_full[s], (p_par >> s) & 1)) return false;
-          p_par ^= 1u << s;
+          if (!__all_sync(0xffffffffu, wait(&sh.p_full[s], p_par[s]))) return false;
+          p_par[s] ^= 1;
           tc::fence_after();
           return true;
         };
-        if (!TMA || n_seg) ok = all_wait(&sh.q_full, (TMA ? n_seg - 1 : n_seg) & 1);
+        ok = __all_sync(0xffffffffu, wait(&sh.q_full, n_seg & 1)) && full(first);
         if (!ok) break;
-        Place k{at, at_par}, v = k;
-        if (MT == 2) {  // K0 V0 K1 V1 ...
-          ok = full(k);
-          if (!ok) break;
-          tc::fence_after();
+        tc::fence_after();
+        if (MT == 2) {
+          Place k = first, v = first;
           step(v, 1);
-          qk(0, k, false, false);
-          qk(1, k, true, n == 1);
+          qk(0, k);
+          qk(1, k);
+          commit(&sh.empty[k.st]);
+          if (n == 1) commit(&sh.q_empty);
           for (int i = 0; i < n; ++i) {
             const bool more = i + 1 < n;
             step(k, 2);
             ok = full(v) && weights(0, i == 0);
             if (!ok) break;
-            pv(0, v, i > 0, false);
+            pv(0, v, i > 0);
             if (more) {
               ok = full(k);
               if (!ok) break;
-              qk(0, k, false, false);
+              qk(0, k);
             }
             ok = weights(1, i == 0);
             if (!ok) break;
-            pv(1, v, i > 0, true);
-            if (more) qk(1, k, true, i + 2 == n);
+            pv(1, v, i > 0);
+            commit(&sh.empty[v.st]);
+            if (more) {
+              qk(1, k);
+              commit(&sh.empty[k.st]);
+              if (i + 2 == n) commit(&sh.q_empty);
+            }
             step(v, 2);
           }
-        } else {  // K0 K1 V0 K2 V1 ... V(n-1)
-          const int i0 = (int)own;
-          if (i0 < n) {
-            step(k, own);
+        } else {
+          // K0 K1 V0 K2 V1 ... V(n-1)
+          Place k = first, v = first;
+          qk(0, k);
+          commit(&sh.empty[k.st]);
+          if (n > 1) {
+            step(k, 1);
             ok = full(k);
             if (!ok) break;
-            tc::fence_after();
-            qk(own, k, true, i0 + 2 >= n);
-            if (i0 == 0) step(v, n == 1 ? 1 : 2);
-            else step(v, n == 2 ? 3 : 4);
-            for (int i = i0; i < n; i += 2) {
-              ok = full(v) && weights(own, i == i0);
-              if (!ok) break;
-              pv(own, v, i > i0, true);
-              if (i + 2 >= n) break;
-              step(k, i == 0 ? 3 : 4);
+            qk(1, k);
+            commit(&sh.empty[k.st]);
+          }
+          if (n <= 2) commit(&sh.q_empty);
+          step(v, n > 1 ? 2 : 1);
+          for (int i = 0; i < n; ++i) {
+            const uint32_t s = i & 1;
+            ok = full(v) && weights(s, i < 2);
+            if (!ok) break;
+            pv(s, v, i > 1);
+            commit(&sh.empty[v.st]);
+            if (i + 2 < n) {
+              step(k, 2);
               ok = full(k);
               if (!ok) break;
-              qk(own, k, true, i + 4 >= n);
-              step(v, i + 3 == n ? 3 : 4);
+              qk(s, k);
+              commit(&sh.empty[k.st]);
+              if (i + 3 == n) commit(&sh.q_empty);
             }
-          } else if (tc::elect()) {
-            mbar_arrive(&sh.q_empty);
+            step(v, i + 2 < n ? 2 : 1);
           }
         }
+        o_used |= MT == 2 || n > 1 ? 3u : 1u;
+        Place nx{at, at_par};
         for (uint32_t left = 2 * (uint32_t)n; left > 0;) {  // 2 n places on
           const uint32_t by = min(left, (uint32_t)W::NS);
-          Place x{at, at_par};
-          step(x, by);
-          at = x.st;
-          at_par = x.par;
+          step(nx, by);
           left -= by;
         }
+        at = nx.st;
+        at_par = nx.par;
         ++n_seg;
         t += (uint32_t)n;
       }
@@ -955,51 +658,32 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ Wi
         bool careful = (masked && !SPARSE) || __any_sync(0xffffffffu, m == DARIC_NEG_INF);
         if (!careful) {
           // one pass: weights by the maximum so far, kept in registers until
-          // the maximum of this tile is known to be near enough; the next
-          // columns are on their way meanwhile. With the selects of SPARSE
-          // the paired fp32 instructions are the faster form (177 -> 158 us
-          // in the case above), without them the single ones (99 against 104
-          // us with MT = 2).
-          uint32_t y[64], x[2][32];
-          float mx = DARIC_NEG_INF;
-          float a0 = 0.f, a1 = 0.f;
-          uint64_t sum = pair_of(0.f, 0.f);
-          const uint64_t c2 = pair_of(cexp, cexp), b2 = pair_of(-mb, -mb);
-          tc::ld32_ahead(s_col, x[0]);
+          // the maximum of this tile is known to be near enough
+          uint32_t y[64];
+          float mx = DARIC_NEG_INF, a0 = 0.f, a1 = 0.f;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            tc::ld32_there(x[w & 1]);
-            if (w < 3) tc::ld32_ahead(s_col + (w + 1) * 32, x[(w + 1) & 1]);
+            uint32_t x[32];
             const uint32_t see_w = SPARSE ? vm[w] : 0;
+            tc::ld32(s_col + w * 32, x);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              float u = __uint_as_float(x[w & 1][2 * e]), v = __uint_as_float(x[w & 1][2 * e + 1]);
+              float u = __uint_as_float(x[2 * e]), v = __uint_as_float(x[2 * e + 1]);
               if (SPARSE) {
                 u = see_w & (1u << (2 * e)) ? u : DARIC_NEG_INF;
                 v = see_w & (2u << (2 * e)) ? v : DARIC_NEG_INF;
               }
-              float a, d;
-              if (SPARSE) {
-                mx = max3(mx, u, v);
-                const float2 z = unpair(fma_pair(pair_of(u, v), c2, b2));
-                a = exp2_fast(z.x);
-                d = exp2_fast(z.y);
-                sum = add_pair(sum, pair_of(a, d));
-              } else {
-                mx = fmaxf(mx, fmaxf(u, v));
-                a = exp2_fast(__fmaf_rn(u, cexp, -mb));
-                d = exp2_fast(__fmaf_rn(v, cexp, -mb));
-                a0 += a;
-                a1 += d;
-              }
+              mx = fmaxf(mx, fmaxf(u, v));
+              const float a = exp2_fast(__fmaf_rn(u, cexp, -mb)), d = exp2_fast(__fmaf_rn(v, cexp, -mb));
+              a0 += a;
+              a1 += d;
               y[w * 16 + e] = Mma<T>::pack(a, d);
             }
           }
-          const float2 a01 = SPARSE ? unpair(sum) : make_float2(a0, a1);
           careful = __any_sync(0xffffffffu, (mx - m) * cexp > 8.f);
           if (!careful) {
-            l0 += a01.x;
-            l1 += a01.y;
+            l0 += a0;
+            l1 += a1;
 #pragma unroll
             for (int w = 0; w < 2; ++w) tc::st32(s_col + w * 32, *reinterpret_cast<const uint32_t(*)[32]>(&y[w * 32]));
           }
@@ -1341,80 +1025,35 @@ __global__ void __launch_bounds__(kUnionThreads) union_kernel(const __grid_const
   }
 }
 
-// Encoder of tensor maps, a function of the driver.
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encoder() {
-  static const EncodeTiled f = [] {
-    void* at = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &at, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      at = nullptr;
-    }
-    return (EncodeTiled)at;
-  }();
-  return f;
-}
-
-// Whether a layer's pages can be boxes: whole pages in a tile of 128 keys or
-// whole tiles in a page, and 8 tokens or more (a swizzle pattern is 8 rows).
-bool make_map(WideLaunch& w) {
-  const KvView& kv = w.kv;
-  if (kv.page_size % 8 || (kv.page_size < kKeys ? kKeys % kv.page_size : kv.page_size % kKeys)) return false;
-  const int bt = std::min(kv.page_size, kKeys);
-  w.box_log = 0;
-  while ((1 << w.box_log) < bt) ++w.box_log;
-  const cuuint64_t dims[5] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.heads,
-                              (cuuint64_t)kv.num_pages, 2};
-  const cuuint64_t strides[4] = {(cuuint64_t)kv.tok_stride, (cuuint64_t)kv.head_stride, (cuuint64_t)kv.page_stride,
-                                 (cuuint64_t)kv.v_off};
-  for (cuuint64_t st : strides)
-    if (st == 0 || st >= (1ull << 40)) return false;
-  const cuuint32_t box[5] = {64, (cuuint32_t)bt, 1, 1, 1}, step[5] = {1, 1, 1, 1, 1};
-  const EncodeTiled f = encoder();
-  return f && f(&w.map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, kv.base, dims, strides, box, step,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <class T, int D, int MT, bool SPARSE, bool TMA>
-void wide_one(const WideLaunch& p, int grid, cudaStream_t s) {
+template <class T, int D, int MT, bool SPARSE>
+void wide_one(const AttendLaunch& p, int grid, cudaStream_t s) {
   using W = Wide<D, MT, SPARSE>;
   constexpr int bytes = wide_smem<D, MT, SPARSE>();
   static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
-  allow_smem(wide_kernel<T, D, MT, SPARSE, TMA>, bytes, done);
+  allow_smem(wide_kernel<T, D, MT, SPARSE>, bytes, done);
   if (SPARSE) {
     static std::atomic<uint64_t> ready{0};
     allow_smem(union_kernel, kUnionPages * 4, ready);
-    union_kernel<<<dim3((unsigned)(p.lists / p.kv.heads), (unsigned)p.kv.heads), kUnionThreads, p.sq.table_cols * 4, s>>>(
-        static_cast<const AttendLaunch&>(p));
+    union_kernel<<<dim3((unsigned)(p.lists / p.kv.heads), (unsigned)p.kv.heads), kUnionThreads, p.sq.table_cols * 4, s>>>(p);
     DARIC_CUDA(cudaGetLastError());
-    launch_after(wide_kernel<T, D, MT, SPARSE, TMA>, dim3((unsigned)grid), W::THREADS, s, p, bytes);
+    launch_after(wide_kernel<T, D, MT, SPARSE>, dim3((unsigned)grid), W::THREADS, s, p, bytes);
   } else {
-    wide_kernel<T, D, MT, SPARSE, TMA><<<grid, W::THREADS, bytes, s>>>(p);
+    wide_kernel<T, D, MT, SPARSE><<<grid, W::THREADS, bytes, s>>>(p);
     DARIC_CUDA(cudaGetLastError());
   }
-  launch_after(wide_join_kernel<T, D, MT>, dim3((unsigned)grid, 4 * MT, D / 32), 256, s, static_cast<const AttendLaunch&>(p));
+  launch_after(wide_join_kernel<T, D, MT>, dim3((unsigned)grid, 4 * MT, D / 32), 256, s, p);
 }
 
-template <class T, int D, bool TMA>
-void wide_d(const WideLaunch& p, int mt, int grid, cudaStream_t s) {
-  if (p.pages) return wide_one<T, D, 1, true, TMA>(p, grid, s);
-  // MT = 2 copies without boxes (the top of this file says why)
-  mt == 2 ? wide_one<T, D, 2, false, false>(p, grid, s) : wide_one<T, D, 1, false, TMA>(p, grid, s);
+template <class T, int D>
+void wide_d(const AttendLaunch& p, int mt, int grid, cudaStream_t s) {
+  if (p.pages) return wide_one<T, D, 1, true>(p, grid, s);
+  mt == 2 ? wide_one<T, D, 2, false>(p, grid, s) : wide_one<T, D, 1, false>(p, grid, s);
 }
 
 template <class T>
-void wide_t(const AttendLaunch& a, int mt, int grid, cudaStream_t s) {
-  WideLaunch p{};
-  static_cast<AttendLaunch&>(p) = a;
-  const bool boxes = make_map(p);
-  if (a.kv.head_dim == 64) return boxes ? wide_d<T, 64, true>(p, mt, grid, s) : wide_d<T, 64, false>(p, mt, grid, s);
-  boxes ? wide_d<T, 128, true>(p, mt, grid, s) : wide_d<T, 128, false>(p, mt, grid, s);
+void wide_t(const AttendLaunch& p, int mt, int grid, cudaStream_t s) {
+  p.kv.head_dim == 64 ? wide_d<T, 64>(p, mt, grid, s) : wide_d<T, 128>(p, mt, grid, s);
 }
 
 }  // namespace
