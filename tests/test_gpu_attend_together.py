@@ -174,3 +174,22 @@ def test_bad_blocks_in_every_form(kvh, group, t, bs):
         k, v = bt.kv64(b)
         ok = bt.sees(b) & (torch.arange(bt.lens[b], device="cuda") // bs != page)
         check_attend(bt, out, lse, b, *attend64(bt.q64(b), k, v, ok.repeat(group, 1)[None], 1 / math.sqrt(bt.d)))
+
+
+@pytest.mark.parametrize("seqs,length", [(12, 2048), (60, 150), (100, 61)])
+@pytest.mark.parametrize("t", [16, 40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_segments_on_a_block(seqs, length, t, d):
+    """A block of the many-row forms goes through several whole and cut segments."""
+    lens = [length + 3 * (b % 7) for b in range(seqs)]
+    bt = Batch(lens, [t] * seqs, kvh=8, group=4, d=d, seed=seqs + t)
+    first = run_tree(bt)
+    check_tree(bt, *first)
+    pages = random_pages(bt, 3 if length < 1000 else 40, torch.Generator().manual_seed(t)).cuda()
+    out, lse = sparse_attention(bt.copier, "l", bt.q, pages, bt.table, bt.seq_lens, cu_q=bt.cu_q)
+    check_sparse(bt, pages.cpu(), out, lse)
+    for _ in range(10):
+        again = run_tree(bt)
+        o, z = sparse_attention(bt.copier, "l", bt.q, pages, bt.table, bt.seq_lens, cu_q=bt.cu_q)
+        assert all(torch.equal(x, y) for x, y in zip((*first, out, lse), (*again, o, z)))
+    assert _lib.device_errors(0) == 0
