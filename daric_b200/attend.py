@@ -230,7 +230,7 @@ def _sparse(copier, layer_name, kv, q, pages, block_table, seq_lens, cu_q, n, sc
     # a shape of few rows needs what any such call does; lists of many rows
     # have sizes of their own and are not kept
     sizes = (rows, n, heads, pages.shape[1], pages.shape[2], block_table.shape[1])
-    few = rows * heads < 64 * n * pages.shape[1]
+    few = rows * heads < 128 * n * pages.shape[1]
     ws = _kept((dev.index, dim, s, "sparse"), kept and few, dev,
                lambda v: _lib.load().daric_sparse_workspace(dev.index, dim, *sizes, v))
     check(_lib.load().daric_copier_sparse_attention(

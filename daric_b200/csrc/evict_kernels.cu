@@ -9,7 +9,10 @@
 // (new - old): C = nc oc + ns os, S = ns oc - nc os from the table rows of both
 // positions, in fp32 (a product and a fused multiply-add each), and the turned
 // key is rounded once to the cache's type.
-// Bound: the bytes of the tokens that move, read and written once.
+// Bound: the bytes of the tokens that move, read and written once (32 layers,
+// 8 KV heads of 128, bf16, 40 % of 8192 tokens, keys turned: 175 us, 5.0 TB/s;
+// few short lists: the chain of a segment's batches, one layer of 6001 tokens
+// in 27 us).
 #include "attend_common.cuh"
 #include "device_common.cuh"
 
