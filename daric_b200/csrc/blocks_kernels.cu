@@ -511,13 +511,19 @@ __global__ void __launch_bounds__(1024) page_select_kernel(const __grid_constant
       __syncthreads();
       find_digit(hist, kBins, rem, &s_digit, &s_above, sm);
       const int bin = s_digit, left = rem - s_above;
-      if (hist[bin] <= (uint32_t)kNear) {
+      const uint32_t in_bin = hist[bin];
+      // every thread has read the bin's count before the digits below clear
+      // the histogram: the threads take one way together
+      __syncthreads();
+      if (in_bin <= (uint32_t)kNear) {
         for (int i = e0 + tid; i < e1; i += blockDim.x) {
           const uint32_t k = key_at(i);
-          if (bin_of(value_of(k)) == bin) near_key[atomicAdd(&s_count, 1)] = k;
+          if (bin_of(value_of(k)) != bin) continue;
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kNear) near_key[at] = k;
         }
         __syncthreads();
-        const int n = s_count;
+        const int n = min(s_count, kNear);
         for (int i = tid; i < n; i += blockDim.x) {  // ties do not matter: one value is wanted
           int above = 0, same = 0;
           for (int j = 0; j < n; ++j) {

@@ -125,6 +125,29 @@ def test_ties_go_to_the_lower_page():
     check_select(bt, b, 50)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_alike_pages_of_long_tables(rows):
+    """The widest CTAs with more pages in the bin of the k-th score than are
+    ranked at once: all alike, and one page far above that leaves the others in
+    a few bins. Again and again: the answer does not depend on timing."""
+    bt = Batch([8 * 9000] * 2, [1] * 2, kvh=1, group=2, d=64, bs=8, seed=9)
+    q = bt.q[:1].expand(2 * rows, -1, -1).contiguous()
+    b = torch.zeros_like(new_bounds(bt.copier, "l"))
+    b[:, :, 0], b[:, :, 1] = -1.0, 1.0
+    cu = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device="cuda")
+    far = 5000
+    for first in (list(range(19)), sorted([*range(18), far])):  # of sequence 0
+        if far in first:
+            b[bt.table[0, far].long(), :, 1] = 2.0 ** 40
+            b[bt.table[0, far].long(), :, 0] = -2.0 ** 40
+        expect = torch.tensor([[*(first if s == 0 else range(19)), (8 * 9000 - rows + j) // 8]
+                               for s in range(2) for j in range(rows)], dtype=torch.int32)
+        for _ in range(25):
+            got = select_pages(q, b, bt.table, bt.seq_lens, 20, bt.bs, cu_q=cu)
+            assert torch.equal(got[:, 0].cpu(), expect)
+    assert _lib.device_errors(0) == 0
+
+
 def test_scores_closer_than_fp32_tells():
     """Pages whose scores differ by less than an fp32 sum resolves."""
     bt = Batch([16 * 300], [1], kvh=1, group=1, d=128, seed=5)
