@@ -818,8 +818,9 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
               x[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), a1, __uint_as_float(x[e]) * a0));
           }
           if (poison && real) {
-            // positions of this part that this row sees beside rows that do not
-            const int k0 = SPARSE ? g.tile0 * kKeys : max(g.tile0 * kKeys, max(g.s.ctx, 0));
+            // positions of the tiles that values were taken out of: whole
+            // tiles, with context in front of the drafted tokens
+            const int k0 = SPARSE ? g.tile0 * kKeys : max(g.tile0 * kKeys, max(see, 0) / kKeys * kKeys);
             const int k1 = SPARSE ? min((g.tile0 + g.n) * kKeys, g.listed * p.kv.page_size)
                                   : min((g.tile0 + g.n) * kKeys, g.s.len);
             for (int k = k0; k < k1; ++k) {
@@ -831,7 +832,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
                 if (!((x.y >> jl) & 1u) || pos > g.s.ctx + j || pos >= g.s.len) continue;
                 blk = (int)x.z;
               } else {
-                if (!sees_draft(p.sq, row, j, k - g.s.ctx)) continue;
+                if (k >= g.s.ctx && !sees_draft(p.sq, row, j, k - g.s.ctx)) continue;
                 blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
               }
               if (blk < 0 || blk >= p.kv.num_pages) continue;

@@ -150,6 +150,25 @@ def test_nonfinite_values_stay_where_they_are_seen(dtype, group):
     assert (out[3, :group, 5] == math.inf).all() and torch.isnan(out[3, group:]).all()
 
 
+@pytest.mark.parametrize("kvh,group,t", [(1, 4, 1), (1, 4, 5), (2, 4, 16), (1, 8, 33), (1, 20, 6), (1, 20, 16), (1, 4, 200)])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("at", ["last", "tile"])
+def test_nonfinite_values_of_the_context_reach_every_row(kvh, group, t, masked, at):
+    """At the last position before the drafted tokens, and at the first one of
+    the 128 keys that hold it, in every form."""
+    bt = Batch([900, 300 + t], [t, t], kvh=kvh, group=group, seed=6)
+    mask = tree_masks(bt.rows, -(-t // 64), torch.Generator().manual_seed(9)) if masked else None
+    for b in range(2):
+        ctx = bt.lens[b] - t
+        pos = ctx - 1 if at == "last" else ctx // 128 * 128
+        blk = int(bt.table[b, pos // 16])
+        bt.v[blk, pos % 16, 0, 5] = math.inf
+        bt.v[blk, pos % 16, kvh - 1, 70] = math.nan
+    out, lse = run_tree(bt, mask)
+    check_tree(bt, out, lse, mask)
+    assert (out[:, :group, 5] == math.inf).all() and torch.isnan(out[:, -group:, 70]).all()
+
+
 def test_lowest_values_and_large_logits():
     bt = Batch([90, 200], [2, 2], seed=12, spread=30.0)
     bt.k[int(bt.table[0, 0]), 3] = torch.finfo(torch.bfloat16).min / 1e30
