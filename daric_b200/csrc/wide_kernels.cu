@@ -50,6 +50,11 @@ using bulk::mbar_wait;
 constexpr int kKeys = 128;      // keys of a tile
 constexpr int kMaskRing = 8;    // tiles whose key masks are kept
 constexpr int kCopyThreads = 128;
+// A wait gives up after five seconds, not the copy kernels' 200 ms: the other
+// roles wait while the softmax warps put values back that are not finite, which
+// takes as long as there are such values.
+constexpr uint64_t kLongWaitNs = 5000000000ull;
+static_assert(kLongWaitNs >= bulk::kWaitNs, "mbar_wait polls as often as it does for its default limit");
 
 template <int D, int MT, bool SPARSE>
 struct Wide {
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
-    if (mbar_wait(bar, parity)) return true;
+    if (mbar_wait(bar, parity, kLongWaitNs)) return true;
     *abort = 1;
     atomicOr(p.sq.err, DEV_ERR_TIMEOUT);
     return false;
@@ -817,33 +822,61 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
             for (int e = 0; e < 32; ++e)
               x[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), a1, __uint_as_float(x[e]) * a0));
           }
-          if (poison && real) {
+          if (poison) {
             // positions of the tiles that values were taken out of: whole
-            // tiles, with context in front of the drafted tokens
+            // tiles, with context in front of the drafted tokens. Each lane
+            // looks at one of 32; what is not finite is then added by the rows
+            // that see it, position by position.
             const int k0 = SPARSE ? g.tile0 * kKeys : max(g.tile0 * kKeys, max(see, 0) / kKeys * kKeys);
             const int k1 = SPARSE ? min((g.tile0 + g.n) * kKeys, g.listed * p.kv.page_size)
                                   : min((g.tile0 + g.n) * kKeys, g.s.len);
-            for (int k = k0; k < k1; ++k) {
-              int pg = (int)fdiv((uint32_t)k, p.kv.page_div), blk;
-              const int in = k - pg * p.kv.page_size;
-              if (SPARSE) {
-                const uint4 x = g.list[pg];
-                const int pos = (int)x.x * p.kv.page_size + in;
-                if (!((x.y >> jl) & 1u) || pos > g.s.ctx + j || pos >= g.s.len) continue;
-                blk = (int)x.z;
-              } else {
-                if (k >= g.s.ctx && !sees_draft(p.sq, row, j, k - g.s.ctx)) continue;
-                blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
+            for (int kk = k0; kk < k1; kk += 32) {
+              int pos = kk + lane, tok = 0, blk = -1;
+              uint32_t rows_see = 0xffffffffu;
+              if (pos < k1) {
+                const int pg = (int)fdiv((uint32_t)pos, p.kv.page_div);
+                tok = pos - pg * p.kv.page_size;
+                if (SPARSE) {
+                  const uint4 e = g.list[pg];
+                  pos = (int)e.x * p.kv.page_size + tok;
+                  rows_see = e.y;
+                  if (pos < g.s.len) blk = (int)e.z;
+                } else {
+                  blk = __ldg(&p.sq.table[(int64_t)g.b * p.sq.table_ld + pg]);
+                }
               }
-              if (blk < 0 || blk >= p.kv.num_pages) continue;
-              const uint16_t* v = reinterpret_cast<const uint16_t*>(
-                  p.kv.base + (int64_t)blk * p.kv.page_stride + (int64_t)in * p.kv.tok_stride +
-                  (int64_t)g.h * p.kv.head_stride + p.kv.v_off) + w * 32;
+              auto row_of = [&](int block, int token) {  // its 32 columns of V
+                return reinterpret_cast<const uint16_t*>(p.kv.base + (int64_t)block * p.kv.page_stride +
+                                                         (int64_t)token * p.kv.tok_stride +
+                                                         (int64_t)g.h * p.kv.head_stride + p.kv.v_off) + w * 32;
+              };
+              bool bad = false;
+              if (blk >= 0 && blk < p.kv.num_pages) {
+                const uint4* v = reinterpret_cast<const uint4*>(row_of(blk, tok));
+                uint32_t sum = 0;  // x * 0 summed up, as in take_out
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const uint16_t u = v[e];
-                if ((u & Mma<T>::kExpMask) == Mma<T>::kExpMask)
-                  x[e] = __float_as_uint(__uint_as_float(x[e]) + Mma<T>::widen(u));
+                for (int e = 0; e < 4; ++e) {
+                  const uint4 u = v[e];
+                  sum = Mma<T>::zero_sum(u.x, Mma<T>::zero_sum(u.y, Mma<T>::zero_sum(u.z, Mma<T>::zero_sum(u.w, sum))));
+                }
+                bad = (sum & 0x7fff7fffu) != 0;
+              }
+              for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
+                const int from = __ffs((int)left) - 1;
+                const int at = __shfl_sync(0xffffffffu, pos, from);
+                const uint32_t who = __shfl_sync(0xffffffffu, rows_see, from);
+                const uint16_t* v = row_of(__shfl_sync(0xffffffffu, blk, from), __shfl_sync(0xffffffffu, tok, from));
+                const bool seen = real && (SPARSE ? ((who >> jl) & 1u) && at <= g.s.ctx + j
+                                                  : at < g.s.ctx || sees_draft(p.sq, row, j, at - g.s.ctx));
+                if (seen) {
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) {
+                    const uint16_t u = v[e];
+                    if ((u & Mma<T>::kExpMask) == Mma<T>::kExpMask)
+                      x[e] = __float_as_uint(__uint_as_float(x[e]) + Mma<T>::widen(u));
+                  }
+                }
+                __syncwarp();
               }
             }
           }

@@ -396,6 +396,28 @@ def test_sparse_nonfinite_values_stay_where_they_are_listed():
             assert (out[r, :, 5] == math.inf).all() and torch.isnan(out[r, :, 70]).all()
 
 
+@pytest.mark.parametrize("every", [1, 40])
+def test_sparse_nonfinite_values_in_many_pages(every):
+    """Long lists with an infinity in every page, or in every 40th: put back for
+    the rows that list it and for no other."""
+    t, k = 128, 40
+    bt = Batch([16 * 500], [t], kvh=2, group=4, seed=63)
+    pages = random_pages(bt, k, torch.Generator().manual_seed(7), holes=False)
+    call = lambda: sparse_attention(bt.copier, "l", bt.q, pages.cuda(), bt.table, bt.seq_lens)
+    finite, lse = call()
+    marked = torch.arange(0, 500, every)
+    bt.v[bt.table[0, marked.cuda()].long(), 3, :, 5] = math.inf  # token 3: a row may stand before it in its own page
+    own = (bt.lens[0] - t + torch.arange(t)) // 16
+    tok = (bt.lens[0] - t + torch.arange(t)) % 16
+    hit = torch.isin(pages, marked.int()) & ((pages != own[:, None, None]) | (tok >= 3)[:, None, None])
+    hit = hit.any(-1).repeat_interleave(bt.group, 1).cuda()
+    out, lse2 = call()
+    assert _lib.device_errors(0) == 0 and torch.equal(lse, lse2)
+    assert torch.equal(out[..., 5] == math.inf, hit)
+    out[..., 5] = finite[..., 5]
+    assert torch.equal(out, finite)
+
+
 def test_sparse_of_every_page_is_full_attention():
     bt = Batch([257, 64], [1, 1], seed=23)
     full, full_lse = run_tree(bt)
