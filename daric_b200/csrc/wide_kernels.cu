@@ -73,6 +73,7 @@ struct WideShared {
   uint64_t full[10], empty[10];
   uint64_t s_full[2], p_full[2], pv_done[2], o_empty[2];
   uint64_t q_full, q_empty, ml_full;
+  uint64_t drained;        // every product that was issued has completed
   float2 ml[128];          // MT = 1: maximum and sum of the odd key tiles
   uint32_t vmask[kMaskRing][4];
   uint32_t off[3][kKeys];  // row offsets of three key tiles, 16-byte units of the layer
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
     mbar_init(&sh.q_full, kCopyThreads);
     mbar_init(&sh.q_empty, 1);
     mbar_init(&sh.ml_full, 128);
+    mbar_init(&sh.drained, 1);
     mbar_init_fence();
     sh.abort = 0;
     for (int i = 0; i < 4; ++i) sh.poison[i] = -1;
@@ -625,6 +627,11 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
         ++n_seg;
         t += (uint32_t)n;
       }
+      // Where a wait gave up the softmax leaves without having waited for the
+      // last products: they read shared memory and write tensor memory, so
+      // this warp stays for them (for a bounded time, too).
+      commit(&sh.drained);
+      if (!mbar_wait(&sh.drained, 0, kLongWaitNs)) atomicOr(p.sq.err, DEV_ERR_TIMEOUT);
     }
     __syncwarp();
   } else {
@@ -919,7 +926,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
     }
   }
   // Nothing of this CTA is under way any more: every product was waited for
-  // by the softmax, every copy by its thread.
+  // by the warp that issued it, every copy by its thread.
   __syncthreads();
   if (warp == W::MMA_WARP) {
     __syncwarp();
