@@ -78,9 +78,9 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     A row sees the pages up to the one of its own position. The first ``first``
     and the last ``last`` (at least 1) of them are always listed; the others by
     ``max over the group's query heads of sum_d max(q_d min_d, q_d max_d)``,
-    highest first, ties to the lower page. The order is that of the score in
-    exact arithmetic, whatever the rounding of the fast pass. NaN ranks
-    highest. Rows outside every sequence are not written."""
+    highest first, ties to the lower page. The order is that of the score
+    summed up in 64 bits, whatever the rounding of the fast pass. NaN (0 times
+    an infinite bound among them) ranks highest. Rows outside every sequence are not written."""
     dev = q.device
     if not q.is_cuda:
         raise RuntimeError("q must be a CUDA tensor")

@@ -9,17 +9,18 @@
 // instructions per 16 bytes.
 //
 // select_pages: for query row n, KV head h and page g
-//   u = max over the heads of h's group of  sum_d max(q_d, 0) mx_d + min(q_d, 0) mn_d,
-// an upper bound of q . k over the page's keys. This is a matrix product of
-// (max(q, 0), min(q, 0)) with the stored (mx, mn) rows, so the bounds go from
+//   u = max over the heads of h's group of  sum_d max(q_d mn_d, q_d mx_d),
+// an upper bound of q . k over the page's keys. For finite bounds this is a
+// matrix product of (max(q, 0), min(q, 0)) with the stored (mx, mn) rows (where
+// some are infinite or NaN all pages are scored in 64 bits, as below), so the bounds go from
 // global memory straight into matrix fragments (16 bytes a thread; the order
 // of the summed dimension is the same for both operands, so any order is
 // right) and no shared memory, unpacking or shuffle stands beside the loads.
 // Bound: the bytes of the bounds (8 rows over 8192 pages each, 8 KV heads: 49
 // us, 4.8 TB/s), then the selection's barriers (12 to 17 us).
 //
-// The k pages of highest u are those of exact arithmetic, ties to the lower
-// page: |fp32 result - exact| <= E = 2^-14 * max over pages of
+// The k pages of highest u are those of sums in 64 bits, ties to the lower page:
+// |fp32 result - exact| <= E = 2^-14 * max over pages of
 // sum |q_d| |bound_d| (256 * 2 products of one sum, each addition off by at
 // most 2^-23 of the largest partial sum; the products are exact in fp32). A page whose
 // fp32 score is over 2E above the k-th is in, one 2E below it is out, and the
@@ -407,8 +408,10 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectPagesLaunch&
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const double qv = (double)Mma<T>::widen(qw[e][k]);
-        u[e] += (qv > 0.0 ? qv : 0.0) * m + (qv < 0.0 ? qv : 0.0) * l;
-        if (qv != qv) u[e] = qv;
+        // max(q mn, q mx), NaN where either is: an infinite bound that the
+        // sign of q does not meet says nothing
+        const double a = qv * l, b = qv * m;
+        u[e] += a != a || b != b ? a + b : fmax(a, b);
       }
     }
 #pragma unroll

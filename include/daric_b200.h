@@ -351,7 +351,7 @@ DARIC_API int daric_select_pages_workspace(int64_t num_rows, int64_t kv_heads, i
  * of the pages up to the row's own position the first `first` and the last
  * `last` (>= 1), then those of highest
  *   max over the head's query heads of sum_d max(q_d min_d, q_d max_d),
- * in the order of exact arithmetic, ties to the lower page, NaN highest. */
+ * in the order of sums in 64 bits, ties to the lower page, NaN highest. */
 DARIC_API int daric_select_pages(const void* q, int kv_dtype, int64_t q_row, int64_t q_head, int64_t num_rows, int64_t q_heads,
                        int64_t head_dim, const void* bounds, int64_t num_pages, int64_t kv_heads,
                        const int32_t* block_table, int64_t table_ld, int64_t num_seqs, int64_t table_cols,

@@ -170,6 +170,31 @@ def test_nan_and_infinite_bounds_rank_first():
     assert 77 in got[0, 0].tolist()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("low,high", [(-math.inf, 0.5), (-0.5, math.inf), (-math.inf, math.inf), (math.inf, math.inf),
+                                      (-math.inf, -math.inf), (math.nan, 0.5)])
+def test_infinite_bounds_by_the_definition(dtype, low, high):
+    """max(q min, q max) of a dimension whose bounds are infinite, where q is
+    positive, negative and 0: 0 times infinity is NaN, which ranks highest."""
+    bt = Batch([16 * 200], [1], kvh=2, group=3, d=64, dtype=dtype, seed=6)
+    b = page_bounds(bt.copier, "l", bt.table, bt.seq_lens)
+    b[int(bt.table[0, 99]), :, 0, 3], b[int(bt.table[0, 99]), :, 1, 3] = low, high
+    b[int(bt.table[0, 55]), 1, 0, 9], b[int(bt.table[0, 55]), 1, 1, 9] = low, high
+    for sign in (1.0, -1.0, 0.0):
+        bt.q[..., 3] = bt.q[..., 3].abs() * sign
+        bt.q[:, :3, 9] = bt.q[:, :3, 9].abs() * sign
+        got = select_pages(bt.q, b, bt.table, bt.seq_lens, 10, bt.bs)
+        near = b[bt.table[0, :200].long()].double()
+        for h in range(2):
+            q = bt.q[0].double().view(2, 3, 1, 64)[h]
+            u = torch.maximum(q * near[:, h, 0], q * near[:, h, 1]).sum(-1)  # [group, page]
+            nan = torch.isnan(u).any(0)
+            score = torch.where(nan, 0.0, u.nan_to_num(0.0, math.inf, -math.inf).amax(0)).tolist()
+            rest = sorted(range(1, 199), key=lambda i: (-int(nan[i]), -score[i], i))
+            assert got[0, h].tolist() == sorted([0, 199, *rest[:8]]), (sign, h)
+    assert _lib.device_errors(0) == 0
+
+
 def test_strides_padding_streams_and_graphs():
     bt = Batch([800, 700], [1, 1], kvh=2, group=4, seed=7)
     b = page_bounds(bt.copier, "l", bt.table, bt.seq_lens)
