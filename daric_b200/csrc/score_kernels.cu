@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, D > 128 ? 2 : 4) weight_str
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int64_t col = __ldg(&p.col_off[b]);
-  if (col < 0 || col + s.len > p.scores_cols) {
+  if (col < 0 || col > p.scores_cols - s.len) {
     if (threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
     return;
   }
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) weight_bloc
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int64_t col = __ldg(&p.col_off[b]);
-  const bool outside = col < 0 || col + s.len > p.scores_cols;
+  const bool outside = col < 0 || col > p.scores_cols - s.len;
   if (outside && threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
   const int pairs = s.rows * p.sq.group;
   const int key0 = ((int)blockIdx.y * kBlockWarps + warp) * KEYS;

@@ -138,6 +138,18 @@ def test_score_bits_streams_graphs():
             call(**args)
 
 
+@pytest.mark.parametrize("rows", [1, 9])
+@pytest.mark.parametrize("col", [-1, -(1 << 63), (1 << 63) - 1, (1 << 63) - 100, 1 << 40, 701])
+def test_score_columns_outside_are_left_out(rows, col):
+    """Offsets whose sum with a length passes 64 bits, too; a sequence of length 0 has no columns."""
+    bt = Batch([300, 600, 0], [rows, rows, 0], kvh=2, group=4, seed=rows)
+    scores = torch.full((2, 1300), 5.0, device="cuda")
+    off = torch.tensor([0, col, 1300], device="cuda")
+    attention_scores(bt.copier, "l", bt.q, bt.table, bt.seq_lens, scores, off, cu_q=bt.cu_q, accumulate=False)
+    assert _lib.device_errors(0) == 4
+    assert (scores[:, 300:] == 5.0).all() and (scores[:, :300] != 5.0).all()
+
+
 # ------------------------------------------------------------ compact --
 KV = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "fp8": torch.uint8}
 
