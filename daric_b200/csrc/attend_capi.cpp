@@ -339,7 +339,7 @@ int daric_select_pages(const void* q, int kv_dtype, int64_t q_row, int64_t q_hea
                 "select_pages: head dimension must be 64, 128 or 256, got " + std::to_string(head_dim));
     DARIC_CHECK(kv_heads >= 1 && kv_heads < 4096 && num_pages >= 1 && num_pages <= INT32_MAX, "bounds sizes out of range");
     DARIC_CHECK(block_size >= 1 && block_size <= 1024, "block size must be in [1, 1024]");
-    DARIC_CHECK(first >= 0 && last >= 1 && k >= 1 && first + last <= k && k <= INT32_MAX,
+    DARIC_CHECK(first >= 0 && last >= 1 && k >= 1 && first <= k - last && k <= INT32_MAX,
                 "select_pages: k must hold the first and last pages that are always taken (last >= 1)");
     DARIC_CHECK(table_cols <= (1 << 20), "select_pages: at most 1048576 pages per sequence");
     SelectPagesLaunch p{};
@@ -494,8 +494,6 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
     p.block_table = block_table;
     p.table_numel = block_table_numel;
     DARIC_CHECK((int64_t)A.kv.head_dim * es <= 4096, "compact: rows of at most 4096 bytes");
-    const DeviceInfo di = device_info(device);
-    p.err = di.err;
     p.num_pages = A.kv.num_pages;
     p.page_size = A.kv.page_size;
     p.heads = A.kv.heads;
@@ -511,9 +509,12 @@ int daric_copier_compact(daric_copier* copier, int64_t num_layers, const char* c
     for (int64_t s = 0; s < num_segs; ++s) {
       DARIC_CHECK(out_off[s] >= 0 && seg_cap[s] >= 0 && (!seg_blk_off || seg_blk_off[s] >= 0) && (!dst_start || dst_start[s] >= 0),
                   "negative segment field at segment " + std::to_string(s));
-      DARIC_CHECK(out_off[s] + seg_cap[s] <= idx_row || lists == 1, "segment " + std::to_string(s) + " exceeds the selection's row");
-      DARIC_CHECK(seg_cap[s] + (dst_start ? dst_start[s] : 0) <= INT32_MAX, "positions exceed int32");
+      // (differences of what is not negative: no sum that could pass 64 bits)
+      DARIC_CHECK(out_off[s] <= idx_row - seg_cap[s] || lists == 1, "segment " + std::to_string(s) + " exceeds the selection's row");
+      DARIC_CHECK(seg_cap[s] <= INT32_MAX - (dst_start ? dst_start[s] : 0), "positions exceed int32");
     }
+    const DeviceInfo di = device_info(device);
+    p.err = di.err;
     OnDevice on(device);
     for (int64_t l0 = 0; l0 < num_layers; l0 += kCompactLayers) {
       p.layer0 = (int32_t)l0;

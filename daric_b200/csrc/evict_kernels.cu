@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
   // for: list entries, block ids, places.
   constexpr int CT = kMoveTokens / 2 / kMoveThreads;  // tokens of a thread in a chunk
   constexpr int kNoTable = -0x7fffffff - 1;           // a block id of no table entry
+  const int64_t table_len = p.table_numel - sg.blk_off;  // entries of this segment's table: the offset may be any
   int ready = 0, step = 0;
   int from_of[CT], prev_of[CT], blk_of[CT][2];
   auto entries_of = [&]() {
@@ -165,8 +166,8 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int pos = e ? to : from_of[k];
-        const int64_t at = sg.blk_off + (int)fdiv((uint32_t)pos, p.page_div);
-        blk_of[k][e] = i < count && from_of[k] > to && at < p.table_numel ? ld_ahead(&p.block_table[at]) : kNoTable;
+        const int pg = (int)fdiv((uint32_t)pos, p.page_div);
+        blk_of[k][e] = i < count && from_of[k] > to && pg < table_len ? ld_ahead(&p.block_table[sg.blk_off + pg]) : kNoTable;
       }
     }
   };
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kMoveThreads, 1) compact_kernel(const __grid_c
           const int pos = e ? to : from;
           const int pg = (int)fdiv((uint32_t)pos, p.page_div);
           const int blk = blk_of[k][e];
-          if (blk == kNoTable && sg.blk_off + pg >= p.table_numel) {
+          if (blk == kNoTable && pg >= table_len) {
             atomicOr(p.err, DEV_ERR_INDEX_RANGE);
             continue;
           }

@@ -186,3 +186,15 @@ def test_workspace_sizes(calls):
     refused(calls, lib.daric_sparse_workspace(0, 128, 4, 0, 8, 2, 3, 4, C.byref(v)), "positive")
     refused(calls, lib.daric_sparse_workspace(0, 128, 4, 2, 8, 2, 0, 4, C.byref(v)), "positive")
     refused(calls, lib.daric_sparse_workspace(0, 512, 4, 2, 8, 2, 3, 4, C.byref(v)), "head dimension")
+
+
+BIG = (1 << 63) - 1
+
+
+@pytest.mark.parametrize("entry,kw,match", [
+    ("select", dict(first=1 << 62, last=1 << 62), "k must hold"), ("select", dict(first=BIG, last=BIG), "k must hold"),
+    ("compact", dict(dst=(0, BIG)), "exceed int32"), ("compact", dict(dst=(0, BIG - 3)), "exceed int32"),
+    ("compact", dict(off=(0, BIG)), "exceeds the selection's row"), ("compact", dict(cap=(3, BIG)), "exceeds the selection's row"),
+    ("compact", dict(dst=(0, (1 << 31) - 4)), "exceed int32")])
+def test_values_whose_sums_pass_64_bits(calls, entry, kw, match):
+    refused(calls, getattr(calls, entry)(**kw), match)

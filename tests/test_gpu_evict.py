@@ -329,6 +329,23 @@ def test_compact_counts_bound_the_lists_and_bad_entries_are_left_out():
     assert k is not None
 
 
+@pytest.mark.parametrize("off", [13, 14, 1 << 40, (1 << 63) - 1])
+def test_compact_tables_that_start_behind_the_end(off):
+    """A segment whose block table lies outside moves nothing, the others do."""
+    copier, names, sel, table, kw, caches, expect, chk = compact_case(1, [100, 60], [30, 20], seed=15)
+    assert table.numel() == 12
+    table = torch.cat([table, table[:1]])
+    start = caches[0].clone()
+    part = dict(kw, seg_blk_off=[kw["seg_blk_off"][0], off])
+    compact(copier, names, sel, table, **part)
+    assert _lib.device_errors(0) == 4
+    own = table[kw["seg_blk_off"][1]:12].long()
+    assert torch.equal(caches[0][:, own], start[:, own])
+    rest = torch.ones(caches[0].shape[1], dtype=torch.bool)
+    rest[own.cpu()] = False
+    assert torch.equal(caches[0].cpu()[:, rest], expect[0][:, rest])
+
+
 def test_compact_in_a_graph_and_on_a_stream():
     copier, names, sel, table, kw, caches, expect, chk = compact_case(2, [300], [100], seed=10, mode="flexible")
     start = [c.clone() for c in caches]
