@@ -388,7 +388,9 @@ void launch_compact(CompactLaunch& p, int kv_dtype, int tab_dtype, int elem, int
     }
   const int groups = (p.heads + p.move_heads - 1) / p.move_heads;
   p.vecs = row / 16;
-  p.rot_vecs = p.rotate ? half / 16 * (p.neox ? 1 : 2) : 0;
+  // NeoX pairs the two halves (whole vectors each); GPT-J neighbours, so there
+  // the halves together are whole vectors
+  p.rot_vecs = !p.rotate ? 0 : (p.neox ? half / 16 : 2 * half / 16);
   p.tail0 = p.rotate ? 2 * half / 16 : 0;
   const dim3 grid((unsigned)(p.turn_pieces + planes * groups * p.slices), (unsigned)p.num_segs, (unsigned)p.num_layers);
   if (!p.rotate) {  // bytes only: one kernel for every dtype

@@ -281,6 +281,16 @@ def test_compact_turns_keys(layout, dtype, neox, rot, tab):
     check_compact(2, [500, 33], [250, 20], layout=layout, dtype=dtype, mode="flexible", neox=neox, rot=rot, tab=tab, seed=2)
 
 
+@pytest.mark.parametrize("dtype,d,rot,tab", [("bf16", 64, 24, torch.float32), ("bf16", 128, 8, torch.float32), ("f16", 128, 40, torch.float32),
+                                             ("fp8", 64, 16, torch.bfloat16), ("fp8", 128, 48, torch.float16),
+                                             ("f32", 64, 8, torch.float32), ("f32", 64, 24, torch.float32)])
+@pytest.mark.parametrize("per_head", [False, True])
+def test_compact_turns_an_odd_number_of_vectors(dtype, d, rot, tab, per_head):
+    """GPT-J style: the turned part is whole 16-byte vectors, its half need not be."""
+    check_compact(2, [500, 33], [250, 20], kvh=3, d=d, dtype=dtype, mode="flexible", neox=False, rot=rot, tab=tab,
+                  per_head=per_head, seed=2)
+
+
 @pytest.mark.parametrize("lens,keep", [([1], [1]), ([1], [0]), ([17, 16, 15], [17, 0, 1]), ([5000], [4900]), ([5000], [3]),
                                        ([700] * 40, [333] * 40)])
 def test_compact_lengths(lens, keep):
