@@ -123,6 +123,7 @@ struct Mma<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&r);
   }
   static constexpr uint16_t kExpMask = 0x7f80;  // all ones: infinity or NaN
+  static constexpr int kLift = 0;
 };
 template <>
 struct Mma<__half> {
@@ -143,7 +144,23 @@ struct Mma<__half> {
     return *reinterpret_cast<const uint32_t*>(&r);
   }
   static constexpr uint16_t kExpMask = 0x7c00;
+  // The largest weight of a row is stored as 2^kLift (bf16: 1): fp16 has full
+  // precision down to 2^-14 only, and many keys of small weights count together.
+  static constexpr int kLift = 15;
 };
+
+// Exponent of a weight, x c, with the type's factor.
+template <class T>
+__device__ __forceinline__ float lifted(float x, float c) {
+  if constexpr (Mma<T>::kLift == 0) return x * c;
+  else return __fmaf_rn(x, c, (float)Mma<T>::kLift);
+}
+// Log-sum of a row: its maximum m before the scale, its sum l of weights that
+// carry a factor of 2^LIFT.
+template <int LIFT>
+__device__ __forceinline__ float lse_of(float m, float scale, float l) {
+  return __fmaf_rn(m, scale, logf(l * (1.f / (float)(1 << LIFT))));
+}
 
 // ------------------------------------------------------------ sequences --
 struct Seq {

@@ -6,8 +6,11 @@
 //   l = a l + sum p,  O = a O + p V,       c = scale * log2(e),
 // and O / l at the end; parts of one row over different keys join the same
 // way. m, l, O and x are fp32; p is rounded to the cache's type for the
-// second product (relative 2^-9 bf16, 2^-12 fp16 per weight, of either sign),
-// while l sums the unrounded p.
+// second product, which takes both operands in 16 bits (half a step: relative
+// 2^-8 bf16, 2^-11 fp16 per weight, of either sign; a second product with what
+// the rounding left would double that work), while l sums the unrounded p. With
+// fp16 all weights carry a factor of 2^15, which cancels in O / l: they keep
+// their precision down to 2^-29 of the largest and vanish below 2^-40.
 //
 // Bound: the K and V bytes of the cache while group * rows stays small (64
 // sequences of 131 to 8192 tokens, 4 KV heads of 7, fp16: 104 us of kernel, 5.3
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
         for (int u = 0; u < 2; ++u) {
           float(&y)[4] = x[2 * j + u];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = exp2_fast((y[e] - base[e >> 1]) * cexp);
+          for (int e = 0; e < 4; ++e) y[e] = exp2_fast(lifted<T>(y[e] - base[e >> 1], cexp));
           l[0] += y[0] + y[1];
           l[1] += y[2] + y[3];
           a[2 * u] = Mma<T>::pack(y[0], y[1]);
@@ -490,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
         if (starts && ends) {
           if (p.lse)
             p.lse[(int64_t)pair_row(i) * p.lse_row + pair_head(i)] =
-                ll == 0.f ? DARIC_NEG_INF : __fmaf_rn(mm, p.scale, logf(ll));
+                ll == 0.f ? DARIC_NEG_INF : lse_of<Mma<T>::kLift>(mm, p.scale, ll);
         } else {
           p.part_ml[(int64_t)slot * G::ROWS + i] = make_float2(mm, ll);
         }
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Atten
     *reinterpret_cast<uint32_t*>(p.out + row * p.out_row + (int64_t)head * p.out_head + (v * 64 + lane * 2) * 2) =
         Mma<T>::pack(o[v].x * inv, o[v].y * inv);
   if (lane == 0 && p.lse)
-    p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : __fmaf_rn(mm, p.scale, logf(ll));
+    p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : lse_of<Mma<T>::kLift>(mm, p.scale, ll);
 }
 
 template <class T, int D, int RG, bool SPARSE>

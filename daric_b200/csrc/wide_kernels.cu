@@ -5,13 +5,15 @@
 // one KV head and passes tiles of 128 keys by them:
 //   S = Q K^T   tcgen05.mma, Q and K from shared memory, S in tensor memory
 //   P = 2^((S - m) c) by one thread per row, rounded to the cache's type and
-//       written over S in tensor memory (relative 2^-9 bf16, 2^-12 fp16 per
-//       weight; l sums the unrounded values)
+//       written over S in tensor memory (half a step: relative 2^-8 bf16, 2^-11
+//       fp16 per weight; l sums the unrounded values; fp16 weights carry a
+//       factor of 2^7, which cancels at the end, so that they keep their
+//       precision down to 2^-21 and vanish below 2^-32)
 //   O += P V    tcgen05.mma, P from tensor memory, V from shared memory in the
 //       layout it was copied in (its rows are the summed dimension)
 // m is the maximum when it was last moved: it moves, and O and l are rescaled,
 // only when the running maximum is over 2^8 times ahead, so that O is rarely
-// read back. m, l, S and O are fp32.
+// read back (weights are 2^8 at most, times the factor 2^15). m, l, S and O are fp32.
 //
 // Two streams of (scores, weights, output) take turns, so that one is
 // multiplied while the other is exponentiated: with MT = 2 the two row tiles,
@@ -90,6 +92,11 @@ constexpr int wide_smem() {
   return Wide<D, MT, SPARSE>::TILES + (int)sizeof(WideShared) + (SPARSE ? (int)sizeof(SparseShared) : 0);
 }
 
+// Weights may be 2^kLag: how far a row's maximum may run ahead of m.
+constexpr float kLag = 8.f;
+template <class T>
+constexpr int kWideLift = Mma<T>::kLift ? Mma<T>::kLift - (int)kLag : 0;
+
 // The part of a segment that a CTA works on.
 struct Part {
   int b, h, rt, tile0, n, ntiles;
@@ -105,6 +112,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   constexpr int HB = D / 64;          // 64-element halves of a row
   constexpr int HALF = kKeys * 128;   // bytes of such a half of a tile
+  constexpr int LIFT = kWideLift<T>;
   extern __shared__ __align__(1024) uint8_t base[];  // the only shared memory: it starts on 1024 bytes
   WideShared& sh = *reinterpret_cast<WideShared*>(base + W::TILES);
   SparseShared& sp = *reinterpret_cast<SparseShared*>(base + W::TILES + sizeof(WideShared));
@@ -671,7 +679,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
                                     : sh.vmask[(n_tile + (uint32_t)i) % kMaskRing];
         const bool draft = !SPARSE && key0 + kKeys > see;
         const bool masked = SPARSE || draft || (vm[0] & vm[1] & vm[2] & vm[3]) != 0xffffffffu;
-        float mb = m * cexp;
+        float mb = m * cexp - (float)LIFT;
         bool careful = (masked && !SPARSE) || __any_sync(0xffffffffu, m == DARIC_NEG_INF);
         if (!careful) {
           // one pass: weights by the maximum so far, kept in registers until
@@ -697,7 +705,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
               y[w * 16 + e] = Mma<T>::pack(a, d);
             }
           }
-          careful = __any_sync(0xffffffffu, (mx - m) * cexp > 8.f);
+          careful = __any_sync(0xffffffffu, (mx - m) * cexp > kLag);
           if (!careful) {
             l0 += a0;
             l1 += a1;
@@ -740,7 +748,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
             for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (vis[w] >> e) & 1u ? __uint_as_float(x[e]) : DARIC_NEG_INF);
           }
           // the maximum moves when it is over 2^8 ahead (or was none)
-          const bool move = mx > m && (m == DARIC_NEG_INF || (mx - m) * cexp > 8.f);
+          const bool move = mx > m && (m == DARIC_NEG_INF || (mx - m) * cexp > kLag);
           const bool scale_o = move && m != DARIC_NEG_INF;
           if (__any_sync(0xffffffffu, scale_o)) {
             ok = wait(&sh.pv_done[st], (c - 1) & 1);
@@ -760,7 +768,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
             tc::wait_st();
           }
           if (move) m = mx;
-          mb = m == DARIC_NEG_INF ? 0.f : m * cexp;
+          mb = m == DARIC_NEG_INF ? 0.f : m * cexp - (float)LIFT;
           // weights, over the scores they came from (64 scores become 32 columns)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -910,7 +918,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
         if (pair) mbar_arrive(&sh.o_empty[1]);
         if (real) {
           if (starts && ends) {
-            if (p.lse) p.lse[(int64_t)row * p.lse_row + head] = l == 0.f ? DARIC_NEG_INF : __fmaf_rn(m, p.scale, logf(l));
+            if (p.lse) p.lse[(int64_t)row * p.lse_row + head] = l == 0.f ? DARIC_NEG_INF : lse_of<LIFT>(m, p.scale, l);
           } else {
             p.part_ml[(int64_t)slot * W::ROWS + i_pair] = make_float2(m, l);
           }
@@ -986,7 +994,7 @@ __global__ void __launch_bounds__(256) wide_join_kernel(const __grid_constant__ 
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
   *reinterpret_cast<uint2*>(p.out + row * p.out_row + (int64_t)head * p.out_head + warp * 8) =
       make_uint2(Mma<T>::pack(o.x * inv, o.y * inv), Mma<T>::pack(o.z * inv, o.w * inv));
-  if (warp == 0 && p.lse) p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : __fmaf_rn(mm, p.scale, logf(ll));
+  if (warp == 0 && p.lse) p.lse[row * p.lse_row + head] = ll == 0.f ? DARIC_NEG_INF : lse_of<kWideLift<T>>(mm, p.scale, ll);
 }
 
 // Lists of the SPARSE form, one per row tile (blockIdx.x) and KV head: the

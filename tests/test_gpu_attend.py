@@ -169,6 +169,28 @@ def test_nonfinite_values_of_the_context_reach_every_row(kvh, group, t, masked, 
     assert (out[:, :group, 5] == math.inf).all() and torch.isnan(out[:, -group:, 70]).all()
 
 
+@pytest.mark.parametrize("kvh,group,t", [(1, 4, 1), (1, 4, 5), (2, 4, 16), (1, 8, 33), (1, 20, 16)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("logit", [12.0, 18.0, 20.0])
+def test_many_small_weights_count_together(kvh, group, t, dtype, logit):
+    """One key far above thousands of others: the output is what those sum to
+    (weights of 2^-17, 2^-26 and 2^-29; fp16 itself ends at 2^-24)."""
+    bt = Batch([5000], [t], kvh=kvh, group=group, dtype=dtype, seed=3)
+    bt.q.zero_()
+    bt.q[..., 0] = 1.0
+    bt.k.zero_()
+    bt.v.fill_(1.0)
+    blk = int(bt.table[0, 0])
+    bt.k[blk, 0, :, 0] = logit
+    bt.v[blk, 0] = 0.0
+    out, lse = run_tree(bt, scale=1.0)
+    check_tree(bt, out, lse, scale=1.0)
+    if t == 1:
+        pages = torch.arange(bt.table.shape[1], dtype=torch.int32).expand(1, kvh, -1)
+        out, lse = sparse_attention(bt.copier, "l", bt.q, pages.cuda(), bt.table.clamp(min=1), bt.seq_lens, scale=1.0)
+        check_tree(bt, out, lse, scale=1.0)
+
+
 def test_lowest_values_and_large_logits():
     bt = Batch([90, 200], [2, 2], seed=12, spread=30.0)
     bt.k[int(bt.table[0, 0]), 3] = torch.finfo(torch.bfloat16).min / 1e30
