@@ -335,15 +335,16 @@ __global__ void __launch_bounds__(kBlockWarps * 32, D > 128 ? 1 : 2) weight_bloc
   constexpr int KEYS = 16 * M;
   __shared__ __align__(16) QueryBlock<D> qb;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.z, h = blockIdx.x;
+  // heads and tiles share grid x (y ends at 65535): the heads of a tile are neighbours
+  const int b = blockIdx.z, tile = (int)(blockIdx.x / (unsigned)p.kv.heads), h = (int)blockIdx.x - tile * p.kv.heads;
   Seq s = load_seq(p.sq, b);
   clamp_len(p.sq, p.kv.page_size, s);
   const int64_t col = __ldg(&p.col_off[b]);
   const bool outside = col < 0 || col > p.scores_cols - s.len;
   if (outside && threadIdx.x == 0) atomicOr(p.sq.err, DEV_ERR_INDEX_RANGE);
   const int pairs = s.rows * p.sq.group;
-  const int key0 = ((int)blockIdx.y * kBlockWarps + warp) * KEYS;
-  if (outside || (int)blockIdx.y * kBlockWarps * KEYS >= s.len) {
+  const int key0 = (tile * kBlockWarps + warp) * KEYS;
+  if (outside || tile * kBlockWarps * KEYS >= s.len) {
     grid_wait();  // none of a grid that was launched ahead ends before the one that it follows
     return;
   }
@@ -595,8 +596,8 @@ void scores_d(const ScoresLaunch& p0, cudaStream_t s) {
   if (pairs <= 8) return stream_n<T, D, 1>(p, s);
   if (pairs <= 16) return stream_n<T, D, 2>(p, s);
   constexpr int M = D > 128 ? 1 : 2;
-  const unsigned tiles = (unsigned)((cap + kBlockWarps * 16 * M - 1) / (kBlockWarps * 16 * M));
-  const dim3 grid((unsigned)p.kv.heads, tiles, (unsigned)p.sq.num_seqs);
+  const int64_t tiles = (cap + kBlockWarps * 16 * M - 1) / (kBlockWarps * 16 * M);  // 2^17 at most: times 4095 heads, 2^29
+  const dim3 grid((unsigned)(tiles * p.kv.heads), 1, (unsigned)p.sq.num_seqs);
   if (!p0.lse) return launch_after(weight_block_kernel<T, D, M>, grid, kBlockWarps * 32, s, p);
   weight_block_kernel<T, D, M><<<grid, kBlockWarps * 32, 0, s>>>(p);
   DARIC_CUDA(cudaGetLastError());

@@ -78,6 +78,20 @@ def test_score_lengths(lens, rows):
     check_scores(Batch(lens, rows, kvh=1, group=4, d=64, seed=len(lens)))
 
 
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("rows,d,cols", [(17, 256, 8200), (17, 256, 16383), (17, 128, 16383), (1, 256, 16383)])
+def test_scores_of_the_widest_tables(given, rows, d, cols):
+    """Tables for up to 16.7M positions: the lengths are the GPU's to know."""
+    bt = Batch([100], [rows], kvh=2, group=1, d=d, bs=1024, seed=1)
+    table = torch.zeros((1, cols), dtype=torch.int32, device="cuda")
+    table[:, :1] = bt.table[:, :1]
+    lse = tree_attention(bt.copier, "l", bt.q, bt.table, bt.seq_lens)[1] if given else None
+    off = torch.zeros(1, dtype=torch.int64, device="cuda")
+    call = lambda t: attention_scores(bt.copier, "l", bt.q, t, bt.seq_lens, torch.zeros((2, 100), device="cuda"), off, lse=lse)
+    assert torch.equal(call(table), call(bt.table))
+    assert _lib.device_errors(0) == 0
+
+
 def test_scores_of_a_tree_sum_to_its_rows():
     bt = Batch([100, 300], [9, 12], kvh=2, group=4, seed=3)
     mask = tree_masks(bt.rows, 1, torch.Generator().manual_seed(1))
