@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kBoundWarps * 32) bounds_kernel(const __grid_c
   clamp_len(p.sq, bs, s);
   const int start = p.start ? max(__ldg(&p.start[b]), 0) : 0;
   const int p0 = (int)fdiv((uint32_t)start, p.kv.page_div);
-  const int pages = (s.len + bs - 1) / bs - p0;
+  const int pages = start < s.len ? (s.len + bs - 1) / bs - p0 : 0;
   const int c = lane % CH, t0 = lane / CH;
   const int32_t* trow = p.sq.table + (int64_t)b * p.sq.table_ld + p0;
   const int64_t items = (int64_t)pages * H, stride = (int64_t)gridDim.x * kBoundWarps;

@@ -57,6 +57,18 @@ def test_bounds_from_a_position_and_nan():
     assert (b == 7).all() and _lib.device_errors(0) == 0
 
 
+@pytest.mark.parametrize("start,touched", [((99, 46), True), ((100, 47), False), ((111, 48), False), ((1 << 31) - 1, False),
+                                           (-5, True)])
+def test_bounds_from_the_end_on(start, touched):
+    """A start at the length or behind it, inside the last page, too, changes nothing."""
+    bt = Batch([100, 47], [0, 0], seed=2)
+    b = torch.full_like(new_bounds(bt.copier, "l"), 7.0)
+    start = torch.tensor(start if isinstance(start, tuple) else (start, start), dtype=torch.int32, device="cuda")
+    page_bounds(bt.copier, "l", bt.table, bt.seq_lens, b, start=start)
+    last = [int(bt.table[0, 6]), int(bt.table[1, 2])]
+    assert ((b[last] != 7).any() if touched else (b == 7).all()) and _lib.device_errors(0) == 0
+
+
 def select_ref(bt, bounds, k, first=1, last=1):
     out = torch.full((bt.n, bt.kvh, k), -1, dtype=torch.int32)
     for b, t in enumerate(bt.rows):
