@@ -207,12 +207,13 @@ __device__ __forceinline__ bool sees_draft(const SeqBatch& sq, int row, int j, i
   return (__ldg(&sq.mask[(int64_t)row * sq.mask_words + (i >> 6)]) >> (i & 63)) & 1;
 }
 
-// Sequence whose rows hold `row` (warp-wide search over cu_q, all lanes call it), -1 if none.
+// The sequence that starts last at or before `row` (warp-wide search over cu_q, all lanes call
+// it), -1 if none; whether its rows hold the row is the caller's to see.
 __device__ __forceinline__ int find_seq(const SeqBatch& sq, int row) {
   if (!sq.cu_q) return row / sq.rows_each;
   const int lane = threadIdx.x & 31;
   int lo = 0, n = sq.num_seqs;  // the answer is in [lo, lo + n)
-  if (row < __ldg(&sq.cu_q[0]) || row >= __ldg(&sq.cu_q[n])) return -1;
+  if (row < __ldg(&sq.cu_q[0])) return -1;
   while (n > 1) {  // the last sequence that starts at or before the row
     const int step = (n + 31) / 32;
     const int at = lo + lane * step;

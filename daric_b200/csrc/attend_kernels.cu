@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : (RG == 1 ? 3 : 2)) att
         sg.s = load_seq(p.sq, seq_id);
         clamp_len(p.sq, p.kv.page_size, sg.s);
         qpos = sg.s.ctx + (b - sg.s.row0);
+        if (b - sg.s.row0 >= sg.s.rows) seq_id = -1;  // behind its last row, or its offsets are bad
       } else {
         sg.s = Seq{};
       }

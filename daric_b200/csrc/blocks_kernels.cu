@@ -160,6 +160,7 @@ __device__ __forceinline__ RowView row_view(const SeqBatch& sq, int page_size, i
   if (v.seq < 0) return v;
   Seq s = load_seq(sq, v.seq);
   clamp_len(sq, page_size, s);
+  if (n - s.row0 >= s.rows) return RowView{-1, 0};  // behind its last row, or its offsets are bad
   const int pos = s.ctx + (n - s.row0);
   v.pages = pos < 0 || pos >= s.len ? 0 : pos / page_size + 1;
   return v;

@@ -193,3 +193,24 @@ def test_many_segments_on_a_block(seqs, length, t, d):
         o, z = sparse_attention(bt.copier, "l", bt.q, pages, bt.table, bt.seq_lens, cu_q=bt.cu_q)
         assert all(torch.equal(x, y) for x, y in zip((*first, out, lse), (*again, o, z)))
     assert _lib.device_errors(0) == 0
+
+
+@pytest.mark.parametrize("cu,kept", [([0, 1, 99], [True, False, False]), ([0, 3, 1], [True] * 3), ([0, 2, 99], [True, True, False]),
+                                     ([-1, 1, 2], [False, True, False])])
+def test_sequences_with_bad_offsets_have_no_rows(cu, kept):
+    """Every call leaves their rows as they were and sets the error bit (a call
+    that goes from rows to sequences sees only the sequences that rows lead to)."""
+    bt = Batch([270, 233], [2, 1], kvh=2, group=4, seed=54)
+    bounds = page_bounds(bt.copier, "l", bt.table, bt.seq_lens)
+    cu_q = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    pages = torch.zeros((3, bt.kvh, 1), dtype=torch.int32, device="cuda")
+    for call in (tree_attention, lambda c, n, q, *a, **k: sparse_attention(c, n, q, pages, *a, **k)):
+        out, lse = torch.full_like(bt.q, 55.0), torch.full(bt.q.shape[:2], 55.0, device="cuda")
+        call(bt.copier, "l", bt.q, bt.table, bt.seq_lens, cu_q=cu_q, out=out, lse=lse)
+        assert _lib.device_errors(0) == (4 if call is tree_attention or cu != [0, 3, 1] else 0)
+        for r in range(3):
+            assert (out[r] != 55).any().item() == (lse[r] != 55).any().item() == kept[r]
+    got = torch.full((3, bt.kvh, 5), 55, dtype=torch.int32, device="cuda")
+    select_pages(bt.q, bounds, bt.table, bt.seq_lens, 5, bt.bs, cu_q=cu_q, out=got)
+    assert _lib.device_errors(0) == (4 if cu != [0, 3, 1] else 0)
+    assert [(got[r] != 55).any().item() for r in range(3)] == kept
