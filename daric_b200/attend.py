@@ -106,13 +106,24 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _stays(dev: torch.device, stream: int) -> bool:
+    """Whether the current stream of ``dev``, of the given handle, is one of
+    torch's own, which live as long as the process (the handle of any other may
+    come back as another stream), and captures nothing (which is asked of the
+    current device's stream)."""
+    return (stream == 0 or torch._C._cuda_getCurrentStream(dev.index)[0] != stream) and \
+        torch.cuda.current_device() == dev.index and not _capturing()
+
+
 def _kept(key: tuple, kept: bool, dev: torch.device, size) -> torch.Tensor:
     """Workspace of a call. The calls of one thread on one stream follow each
     other, so they share one that is kept (a call is several launches, and
     those of two threads may take turns on a stream); a captured call has its
-    own, which belongs to its graph, and so has one on a stream given by its
-    handle. ``size`` fills in the bytes."""
-    kept = kept and not _capturing()
+    own, which belongs to its graph, and so has one on a stream that is not
+    torch's. ``key`` starts with the device's index, head_dim and the stream;
+    ``size`` fills in the bytes (39 MB for head_dim 128, 20 MB for 64 and
+    256)."""
+    kept = kept and _stays(dev, key[2])
     ws = _workspaces.of.get(key) if kept else None
     if ws is None:
         v = C.c_int64(0)

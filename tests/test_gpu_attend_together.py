@@ -5,7 +5,7 @@ import threading
 import pytest
 import torch
 
-from daric_b200 import _lib
+from daric_b200 import _lib, attend
 from daric_b200.attend import sparse_attention, tree_attention
 from daric_b200.blocks import new_bounds, page_bounds, select_pages
 from daric_b200.evict import attention_scores
@@ -214,3 +214,39 @@ def test_sequences_with_bad_offsets_have_no_rows(cu, kept):
     select_pages(bt.q, bounds, bt.table, bt.seq_lens, 5, bt.bs, cu_q=cu_q, out=got)
     assert _lib.device_errors(0) == (4 if cu != [0, 3, 1] else 0)
     assert [(got[r] != 55).any().item() for r in range(3)] == kept
+
+
+def test_workspaces_are_kept_for_torchs_streams_only(monkeypatch):
+    """Not where the handle of a stream may come back as another one, where the
+    call is captured, or where that cannot be told."""
+    bt = Batch([5000, 700], [2, 2], kvh=2, group=4, seed=55)
+    pages = random_pages(bt, 40, torch.Generator().manual_seed(3)).cuda()
+    kept = attend._workspaces.of
+
+    def both():
+        return (*tree_attention(bt.copier, "l", bt.q, bt.table, bt.seq_lens, cu_q=bt.cu_q),
+                *sparse_attention(bt.copier, "l", bt.q, pages, bt.table, bt.seq_lens, cu_q=bt.cu_q))
+
+    kept.clear()
+    expect = both()
+    assert len(kept) == 2
+    both()
+    assert len(kept) == 2
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream, more in ((torch.cuda.ExternalStream(side.cuda_stream), 0), (side, 2)):
+        kept.clear()
+        with torch.cuda.stream(stream):
+            got = both()
+        side.synchronize()
+        assert len(kept) == more and all(torch.equal(a, b) for a, b in zip(got, expect))
+    kept.clear()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = both()
+    g.replay()
+    assert not kept and all(torch.equal(a, b) for a, b in zip(got, expect))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    got = both()
+    assert not kept and all(torch.equal(a, b) for a, b in zip(got, expect))
+
