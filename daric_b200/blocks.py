@@ -8,6 +8,7 @@ Batches are described as in :mod:`daric_b200.attend`.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional
 
 import torch
@@ -103,11 +104,12 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tenso
     if n == 0 or rows == 0:
         return out
     cols = block_table.shape[1]
-    words = rows * kv_heads * ((cols + 3) // 4 * 4 + (cols + 63) // 64)
-    ws = q.new_empty(max(words, 1), dtype=torch.int32)
+    size = C.c_int64(0)
+    check(_lib.load().daric_select_pages_workspace(rows, kv_heads, cols, C.byref(size)))
+    ws = q.new_empty(size.value, dtype=torch.uint8)
     check(_lib.load().daric_select_pages(
         q.data_ptr(), kv_dtype_code(q.dtype), q.stride(0), q.stride(1), rows, heads, dim, bounds.data_ptr(), nb,
         kv_heads, block_table.data_ptr(), block_table.stride(0), n, cols, seq_lens.data_ptr(), _ptr(cu_q),
-        int(block_size), k, int(first), int(last), out.data_ptr(), ws.data_ptr(), words * 4, dev.index,
+        int(block_size), k, int(first), int(last), out.data_ptr(), ws.data_ptr(), size.value, dev.index,
         _raw_stream(dev.index)))
     return out

@@ -68,9 +68,10 @@ def attention_scores(copier: CacheCopier, layer_name: str, q: torch.Tensor, bloc
         return scores
     ws, ws_bytes = None, 0
     if lse is None and rows:
-        splits = (cols * kv.shape[2] + 255) // 256
-        ws = q.new_empty(rows * heads * (splits * 2 + 1) + 4, dtype=torch.float32)
-        ws_bytes = ws.numel() * 4
+        size = C.c_int64(0)
+        check(_lib.load().daric_scores_workspace(rows, heads, cols, kv.shape[2], C.byref(size)))
+        ws_bytes = size.value
+        ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     check(_lib.load().daric_copier_attention_scores(
         copier._h, layer_name.encode(), kv_dtype_code(kv.dtype), q.data_ptr(), q.stride(0), q.stride(1), rows,
         heads, dim, block_table.data_ptr(), block_table.stride(0), n, cols, seq_lens.data_ptr(), _ptr(cu_q),
