@@ -55,13 +55,14 @@ SeqBatch seq_batch(const int32_t* table, int64_t table_ld, int64_t num_seqs, int
   SeqBatch b{};
   DARIC_CHECK(num_seqs >= 1 && num_rows >= 0 && table_cols >= 1, "batch sizes must be positive");
   DARIC_CHECK(num_seqs <= 65535, "at most 65535 sequences per call");
-  DARIC_CHECK(table_cols * page_size <= INT32_MAX, "block table reaches past int32 positions");
+  // (a tile of up to 1024 keys past the end is still counted in 32 bits)
+  DARIC_CHECK(table_cols <= (INT32_MAX - 1024) / page_size, "block table reaches past int32 positions");
   DARIC_CHECK(table && seq_lens, "NULL block table or lengths");
   DARIC_CHECK(table_ld >= table_cols || num_seqs == 1, "block table rows overlap");
   DARIC_CHECK(q_heads >= kv_heads && q_heads % kv_heads == 0,
               "query heads (" + std::to_string(q_heads) + ") must be a multiple of KV heads (" +
                   std::to_string(kv_heads) + ")");
-  DARIC_CHECK(num_rows * q_heads <= INT32_MAX, "too many query rows");
+  DARIC_CHECK(num_rows <= INT32_MAX / q_heads, "too many query rows");
   DARIC_CHECK(cu_q || num_rows % num_seqs == 0, "query rows must divide evenly over the sequences without cu_q");
   b.table = table;
   b.table_ld = table_ld;
@@ -254,7 +255,8 @@ int daric_copier_sparse_attention(daric_copier* copier, const char* layer_name, 
                      L.kv.page_size);
     if (num_rows == 0) return;
     DARIC_CHECK(q && out && pages, "NULL query, output or page list");
-    DARIC_CHECK(k >= 1 && k * L.kv.page_size <= INT32_MAX, "sparse_attention: page lists must have at least one entry");
+    DARIC_CHECK(k >= 1 && k <= (INT32_MAX - 1024) / L.kv.page_size,
+                "sparse_attention: page lists must have at least one entry, and less than 2^31 - 1024 positions");
     DARIC_CHECK(aligned(q, q_row * 2, q_head * 2, 16), "query rows must be 16-byte aligned");
     DARIC_CHECK(aligned(out, out_row * 2, out_head * 2, 16), "output rows must be 16-byte aligned");
     const DeviceInfo di = device_info(device);

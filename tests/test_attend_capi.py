@@ -198,3 +198,16 @@ BIG = (1 << 63) - 1
     ("compact", dict(dst=(0, (1 << 31) - 4)), "exceed int32")])
 def test_values_whose_sums_pass_64_bits(calls, entry, kw, match):
     refused(calls, getattr(calls, entry)(**kw), match)
+
+
+@pytest.mark.parametrize("entry", ["tree", "sparse", "bounds", "select", "scores"])
+@pytest.mark.parametrize("cols", [(1 << 27) - 1, (1 << 27) - 64, BIG // 16 + 1, BIG])
+def test_tables_that_end_beside_2_to_31(calls, entry, cols):
+    """Positions behind the last one are counted in 32 bits, too."""
+    refused(calls, getattr(calls, entry)(cols=cols, ld=cols), "1048576" if entry == "select" else "int32 positions")
+
+
+@pytest.mark.parametrize("kw,match", [(dict(k=(1 << 27) - 1), "positions"), (dict(k=BIG // 16 + 1), "positions"), (dict(k=BIG), "positions"),
+                                      (dict(rows=BIG - 1), "too many query rows"), (dict(rows=1 << 61), "too many query rows")])
+def test_lists_and_rows_that_pass_their_range(calls, kw, match):
+    refused(calls, calls.sparse(**kw), match)
