@@ -94,11 +94,14 @@ void check_scale(float scale) {
 // How the query heads of one KV head times the rows of a sequence (their
 // mean: the lengths are on the device) are tiled: up to 16 and 32 pairs as row
 // groups of 16 (attend_kernels.cu, memory-bound there); from 33 on as 128 or
-// 256 rows on the tensor cores (wide_kernels.cu). 256-wide heads do not fit
-// those and take four row groups. (us for 16 sequences of 8192 keys, 8 KV
-// heads of 128, bf16, by pairs: 16: one row group 104, two 105, tensor cores
-// 120; 20: 186, 107, 120; 32: 188, 111, 121; 36: two row groups 184, one tile
-// of 128 124, two 156; 128: 362, 133, 164; 132: 445, 216, 166.)
+// 256 rows on the tensor cores (wide_kernels.cu). That form's tiles of 128 keys
+// leave no room for 256-wide heads (tiles of 64 would, and are not built), which
+// take four row groups (8 sequences of 8192 keys, 8 KV heads of 4, bf16, 256
+// wide: 16 rows 223 us, 64 rows 770 us, 178 TFLOP/s; 128 wide: 84 and 104). (us
+// for 16 sequences of 8192 keys, 8 KV heads of 128, bf16, by pairs: 16: one row
+// group 104, two 105, tensor cores 120; 20: 186, 107, 120; 32: 188, 111, 121;
+// 36: two row groups 184, one tile of 128 124, two 156; 128: 362, 133, 164; 132:
+// 445, 216, 166.)
 struct Variant {
   int rg;    // row groups of 16, or 0
   int mt;    // tiles of 128 rows, or 0
@@ -115,14 +118,15 @@ Variant attend_variant(int64_t num_rows, int64_t num_seqs, int64_t group, int64_
   // the wide form keeps offsets in 32 bits of 16 bytes
   const bool wide = head_dim <= 128 && layer_bytes < 60.0 * (1ll << 30);
   // Listed pages: where a sequence fills a tile of pairs, and the tile has no
-  // more than 32 rows (a bit each), the rows of a tile share one pass over the
-  // pages that any of them lists; that many rows one by one read each page
-  // many times. (us for 64 of 512 pages, 8 KV heads of 4; shared where all
+  // more than 32 rows (a bit each: four or more query heads per KV head), the
+  // rows of a tile share one pass over the pages that any of them lists; that
+  // many rows one by one read each page many times. (us for 64 of 512 pages, 8 KV heads of 4; shared where all
   // rows list the same pages, shared where no two lists are alike, row by row:
   // 1 x 16 rows 27, 39, 23; 1 x 128 rows 33, 77, 82; 1 x 512 rows 62, 185, 274;
   // 16 x 16 rows 60, 173, 163; 16 x 32 rows 67, 204, 309. Lists of 16 pages,
-  // 16 x 32 rows: 30, 182, 116.)
-  // (A list of more entries than a table has pages holds repeats; it goes row by row.)
+  // 16 x 32 rows: 30, 182, 116. How alike the lists are only the GPU knows: short
+  // lists with little in common lose by the rule, long ones win.) The merge takes
+  // repeats and padding as they come, so lists may be longer than the table.
   if (k && wide && group >= 4 && num_rows * group >= 128 * num_seqs && table_cols <= kUnionPages && k <= kUnionPages)
     return variant_mt(1);
   if (rows <= 16) return variant_rg(1, head_dim);

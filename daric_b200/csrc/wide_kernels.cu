@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
   };
   // Part of the line at tile t; false: none (lengths changed while the kernel ran).
   auto part_at = [&](uint32_t t, Part& g) {
-    if (SPARSE) {
+    if constexpr (SPARSE) {
       for (;; ++b) {
         if (b >= units) return false;
         const uint32_t n = (uint32_t)list_tiles(b);
@@ -228,27 +228,24 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
       g.listed = p.list_count[b];
       g.list = p.list + (int64_t)b * p.list_row;
       g.tile0 = (int)(t - seg_at);
-      g.n = (int)min((uint32_t)(g.ntiles - g.tile0), t1 - t);
-      g.row_base = g.rt * W::ROWS;
-      g.my_rows = min(W::ROWS, g.s.rows * group - g.row_base);
-      return true;
+    } else {
+      for (;; ++b) {
+        if (b >= p.sq.num_seqs) return false;
+        g.s = load_seq(p.sq, b);
+        clamp_len(p.sq, p.kv.page_size, g.s);
+        const uint32_t n = tiles_seq(g.s);
+        if (t < seg_at + n) break;
+        seg_at += n;
+      }
+      uint32_t x = t - seg_at;
+      g.ntiles = tiles_of(g.s);
+      g.tile0 = (int)(x % (uint32_t)g.ntiles);
+      x /= (uint32_t)g.ntiles;
+      const int rts = (g.s.rows * group + W::ROWS - 1) / W::ROWS;
+      g.rt = (int)(x % (uint32_t)rts);
+      g.h = (int)(x / (uint32_t)rts);
+      g.b = b;
     }
-    for (;; ++b) {
-      if (b >= p.sq.num_seqs) return false;
-      g.s = load_seq(p.sq, b);
-      clamp_len(p.sq, p.kv.page_size, g.s);
-      const uint32_t n = tiles_seq(g.s);
-      if (t < seg_at + n) break;
-      seg_at += n;
-    }
-    uint32_t x = t - seg_at;
-    g.ntiles = tiles_of(g.s);
-    g.tile0 = (int)(x % (uint32_t)g.ntiles);
-    x /= (uint32_t)g.ntiles;
-    const int rts = (g.s.rows * group + W::ROWS - 1) / W::ROWS;
-    g.rt = (int)(x % (uint32_t)rts);
-    g.h = (int)(x / (uint32_t)rts);
-    g.b = b;
     g.n = (int)min((uint32_t)(g.ntiles - g.tile0), t1 - t);
     g.row_base = g.rt * W::ROWS;
     g.my_rows = min(W::ROWS, g.s.rows * group - g.row_base);
@@ -260,12 +257,6 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
     if (p.sq.mask) return g.s.ctx;
     return g.s.ctx + (int)fdiv((uint32_t)g.row_base, p.sq.group_div) + 1;
   };
-  // order in which the slots of a part are filled: MT = 2: K0 V0 K1 V1 ...;
-  // MT = 1: K0 K1 V0 K2 V1 ... (the next scores are under way while a tile is
-  // exponentiated)
-  auto k_slot = [&](int i) { return MT == 2 ? 2 * i : (i == 0 ? 0 : 2 * i - 1); };
-  auto v_slot = [&](int i, int n) { return MT == 2 ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
-
   // items of stream s in a part of n key tiles, and the key tile of its local item
   auto items_of = [&](int s, int n) { return MT == 2 ? n : (n + 1 - s) / 2; };
 
@@ -466,6 +457,8 @@ __global__ void __launch_bounds__(512, 1) wide_kernel(const __grid_constant__ At
         push(&sh.full[st], v_tile ? (int)st : -1);
         ++n_slot;
       };
+      // Order of the slots: K0 V0 K1 V1 ..., with one row tile K0 K1 V0 K2 V1
+      // ... (the next scores are under way while a tile is exponentiated).
       if (MT == 2) {
         for (int i = 0; i < g.n; ++i) {
           place(i);
