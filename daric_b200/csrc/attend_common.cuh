@@ -94,7 +94,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
                : "memory");
 }
 
-// 2^x for x <= 0 (about 2 ulp; results below 2^-126 are 0)
+// 2^x (about 2 ulp; results below 2^-126 are 0)
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -13,7 +13,7 @@
 // their precision down to 2^-29 of the largest and vanish below 2^-40.
 //
 // Bound: the K and V bytes of the cache while group * rows stays small (64
-// sequences of 131 to 8192 tokens, 4 KV heads of 7, fp16: 104 us of kernel, 5.3
+// sequences of 131 to 8192 tokens, 4 KV heads of 7, fp16: 99 us of kernel, 5.5
 // TB/s; 64 rows with 128 pages each of 32K: 95 us, 5.7 TB/s).
 // All query heads of a KV head and all rows of a sequence share one read of
 // K and V. Work is split over the long axis: the (sequence, head, row tile)

@@ -13,7 +13,7 @@
 // neighbours in the grid and open its DRAM pages once.
 //
 // Few rows (16 (row, head) pairs or fewer): weight_stream_kernel. Bound: the K
-// bytes (32 sequences up to 32K, 8 KV heads: 214 us, 5.8 TB/s). Every thread copies its own fragment pieces, and the scores it will
+// bytes (32 sequences up to 32K, 8 KV heads: 213 us, 5.8 TB/s). Every thread copies its own fragment pieces, and the scores it will
 // add to, into its own slots of a ring of three stages.
 // Many rows: weight_block_kernel. A warp keeps 32 keys in registers and all
 // query rows pass by them from shared memory. Bound: the latency of a warp's

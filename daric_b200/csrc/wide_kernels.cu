@@ -25,10 +25,11 @@
 // it have landed, some slots behind the newest.
 //
 // Bound: the K and V bytes, their copies and latency with one tile (16
-// sequences x 16 drafted rows x 4 heads at 8K: 116 us, 4.0 TB/s of K and V; 512
-// rows that list 64 of 512 pages each, from L2: 190 us); with two, per stream
+// sequences x 16 drafted rows x 4 heads at 8K: 115 us, 4.1 TB/s of K and V; 512
+// rows that list 64 of 512 pages each, from L2: 166 us); with two, per stream
 // the chain of product, exponentials, product (8 sequences of 512 pairs at 32K:
-// 98 us, 0.53 PFLOP/s). One group copies all slots in order and one warp
+// 92 us, 0.57 PFLOP/s; 2048 appended rows of a prompt of 8192, 8 heads of 4: 403
+// us, 0.60). One group copies all slots in order and one warp
 // issues all products in order, so that every wait is for the phase next to
 // the one its barrier is in, which is all that parity can tell. Why tcgen05 and not the warp matrix
 // instructions here: from 33 pairs on those need more time per key than its
