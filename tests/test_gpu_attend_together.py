@@ -5,7 +5,8 @@ import threading
 import pytest
 import torch
 
-from daric_b200 import _lib, attend
+from daric_b200 import _lib
+from daric_b200 import attend
 from daric_b200.attend import sparse_attention, tree_attention
 from daric_b200.blocks import new_bounds, page_bounds, select_pages
 from daric_b200.evict import attention_scores
